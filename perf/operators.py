@@ -265,15 +265,16 @@ def _inputs(case, seed):
 
 
 class _Memory:
-    """Device memory of the framework as an array that torch can wrap."""
+    """Device memory of a decoder as an array that torch can wrap; the decoder lives as long as the array."""
 
-    def __init__(self, ptr, nbytes):
+    def __init__(self, owner, ptr, nbytes):
+        self.owner = owner
         self.__cuda_array_interface__ = {"shape": (nbytes,), "typestr": "|u1", "data": (ptr, False), "version": 3}
 
 
-def _wrap(ptr, shape, dtype):
+def _wrap(owner, ptr, shape, dtype):
     nbytes = math.prod(shape) * torch.empty((), dtype=dtype).element_size()
-    return torch.as_tensor(_Memory(ptr, nbytes), device="cuda").view(dtype).view(shape)
+    return torch.as_tensor(_Memory(owner, ptr, nbytes), device="cuda").view(dtype).view(shape)
 
 
 def _own_state(case, st):
@@ -296,11 +297,11 @@ def _own_state(case, st):
         dec.extend(streams[s], upto - grown[s])
         grown[s] = upto
     info = dec.pool_info()
-    pool = _wrap(info["pool"], tuple(st["pool"].shape), st["pool"].dtype)
+    pool = _wrap(dec, info["pool"], tuple(st["pool"].shape), st["pool"].dtype)
     pool.copy_(st["pool"])
     st["pool"] = pool
     if st.get("scales") is not None:
-        _wrap(info["scales"], tuple(st["scales"].shape), torch.float32).copy_(st["scales"])
+        _wrap(dec, info["scales"], tuple(st["scales"].shape), torch.float32).copy_(st["scales"])
     st["dec"], st["pkg"] = dec, pkg
     if case["op"] == "attend":
         st["slots_dev"], st["starts_dev"], st["lens_dev"] = _i32(streams), _i32(st["starts"]), _i32(lens)
