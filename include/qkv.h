@@ -117,9 +117,45 @@ const char *qkv_last_error(const qkv_handle *h);
 
 /* ---- stream table (the reference keeps one stream: cur_len, text-decoder.cpp:186) ---- */
 int qkv_stream_open(qkv_handle *h, int32_t *stream_id);
-int qkv_stream_close(qkv_handle *h, int32_t stream_id);           /* frees the stream's pages */
+int qkv_stream_close(qkv_handle *h, int32_t stream_id);           /* frees the pages no other stream shares */
 int qkv_stream_length(const qkv_handle *h, int32_t stream_id, int32_t *tokens);
 int qkv_pool_stats(const qkv_handle *h, int64_t *free_pages, int64_t *total_pages);
+/* A new stream that starts with the first `tokens` tokens of src (a shared
+ * prompt, a beam, a draft): full pages are shared, each freed with its last
+ * holder, and a partly filled last page is copied.  src keeps everything.  The
+ * copy and the page-table entries are ordered on `stream` (NULL = the legacy
+ * default stream), which must be the one that wrote src's tokens, and before
+ * every later model-level call; nothing is synchronised.  A shared page is
+ * read-only: do not append at a position below `tokens` of either stream.
+ * After a fork at src's full length a decode step may continue from src's
+ * last greedy id.  QKV_ERR_CAPACITY / QKV_ERR_OUT_OF_PAGES without a free
+ * slot / page, QKV_ERR_STATE while `stream` is captured; nothing changed
+ * then. */
+int qkv_stream_fork(qkv_handle *h, int32_t src, int32_t tokens, int32_t *stream_id, void *stream);
+/* Give back the tokens of a stream past the first `tokens` (rejected drafts):
+ * pages that only they used become free.  When the new last page is partly
+ * filled and shared, the stream gets its own copy of it (one free page; the
+ * ones given back count).  Ordering and refusals as for qkv_stream_fork; the
+ * next decode step needs in_ids. */
+int qkv_stream_truncate(qkv_handle *h, int32_t stream_id, int32_t tokens, void *stream);
+/* The handle's pool in device memory, for callers that move pages in or out of
+ * it themselves: [n_layers][n_pages][2 (K,V)][8][16][128] elements of the cache
+ * type, the 8-bit caches' scales ([n_layers][n_pages][2][8][16] f32, else
+ * NULL) and the page table ([max_streams][max_pages_per_stream], read-only).
+ * The pointers are the handle's and live as long as it. */
+typedef struct qkv_pool_view {
+    void *pool;
+    int64_t layer_bytes;
+    int64_t page_bytes;
+    float *scales;
+    int64_t scales_layer_floats;
+    const int32_t *page_table;
+    int32_t max_pages_per_stream;
+    int32_t max_streams;
+    int32_t n_pages;
+    int32_t n_layers;
+} qkv_pool_view;
+int qkv_pool_view_get(const qkv_handle *h, qkv_pool_view *view);
 /* Move live pages to the low end of the pool (device page copies + page-table
  * rewrite); *moved = pages moved. */
 int qkv_compact(qkv_handle *h, int64_t *moved);
@@ -276,6 +312,58 @@ int qkv_prefill_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *s
 int qkv_prefill_attend_q16(qkv_handle *h, int32_t layer, int32_t n, const int32_t *stream_ids, const int32_t *lens,
                            const void *q16_dev, float *out_dev, void *stream);
 
+/* ---- operator level: chunks of several new tokens per stream ----
+ * Device pointers and `stream` as above.  A slot of -1 marks a padding entry,
+ * which is skipped, so that a captured call can serve smaller batches. */
+
+/* qkv_kv_append with a rotary position per axis: row r of qkv[n][Hq*D + 2*Hkv*D]
+ * f32 is stored at token position positions[r] of stream slots[r], and its q
+ * and k heads turn by axes[a][r] (axes_dev: [3][n] int32, any value: time,
+ * height, width), a being the axis of the rotation pair.  sections (host, 3
+ * ints adding up to 64): blocked, the first sections[0] pairs take axis 0, the
+ * next sections[1] axis 1, the rest axis 2; interleaved, pair i takes axis i % 3
+ * while i < 3 * sections[i % 3], else axis 0.  With the three positions equal
+ * this is the plain rotary embedding; rows of a draft tree pass their depth.
+ * q_out[n][Hq*D] as f32 or bf16 (q_dtype), unscaled.  qkv and q_out 16-byte
+ * aligned.  Two rows must not name the same (slot, position).  Extends
+ * text-decoder.cpp:375-433, which knows one axis. */
+int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slots_dev, const int32_t *positions_dev,
+                     const int32_t *axes_dev, const int32_t *sections, int32_t interleaved, const float *qkv_dev,
+                     void *q_out_dev, int32_t q_dtype, void *stream);
+
+/* Attention of a chunk of new tokens per stream over its pages.  Stream i of
+ * n (<= 1024) has the query rows starts[i] .. starts[i + 1] - 1 (starts: n + 1
+ * ascending ints; an empty chunk is skipped), which are the last of its lens[i]
+ * cached tokens, already appended.  Each row sees the tokens before the chunk
+ * and, inside it, those up to its own; with mask (uint64 per row, nullable;
+ * chunks of at most 64 rows), bit b says whether it sees the chunk's token b.
+ * A row that sees nothing gives zeros.  q and out: [rows][Hq*D] bf16, 16-byte
+ * aligned, q post-RoPE and unscaled; rows outside every chunk are left as they
+ * are.  K and V of the lens[i] tokens must be finite; what lies behind them is
+ * not read.  A slot may be listed more than once.  QKV_ERR_STATE for an f32
+ * cache (qkv_prefill_attend serves it).  Uses the handle's workspace: calls on
+ * one handle, captured ones too, must not overlap.  The prompt half of
+ * text-decoder.cpp:322-334 for any number of rows at any context. */
+int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slots_dev, const int32_t *starts_dev,
+                     const int32_t *lens_dev, int32_t rows, const uint64_t *mask_dev, const void *q_dev, void *out_dev,
+                     void *stream);
+
+/* Copy page src[i] to page dst[i], i < n, in every layer, scales included.  A
+ * dst page must be listed once and not be a src. */
+int qkv_pages_copy(qkv_handle *h, int32_t n, const int32_t *src_dev, const int32_t *dst_dev, void *stream);
+
+/* Copy listed tokens to consecutive positions, in every layer, scales
+ * included: of group i (n <= 65535), token src_bases[i] + keep[starts[i] + k]
+ * of stream src_slots[i] goes to position dst_bases[i] + k of stream
+ * dst_slots[i].  keep[rows] ascends within a group.  The two streams may be the
+ * same with dst_bases[i] <= src_bases[i]: the accepted path of a draft tree
+ * moves together before qkv_stream_truncate drops the rest.  Groups must not
+ * touch each other's tokens.  A group outside these rules is reported and not
+ * moved. */
+int qkv_tokens_move(qkv_handle *h, int32_t n, const int32_t *src_slots_dev, const int32_t *src_bases_dev,
+                    const int32_t *dst_slots_dev, const int32_t *dst_bases_dev, const int32_t *starts_dev, int32_t rows,
+                    const int32_t *keep_dev, void *stream);
+
 /* One KV-cache step of the microbench: for each of the n streams append one
  * token and attend, for every layer.  qkv[n_layers][n][Hq*D+2*Hkv*D] f32,
  * out[n_layers][n][Hq*D] f32 (layer-major), device pointers; the streams'
@@ -431,11 +519,15 @@ int qkv_pager_append(qkv_pager *p, int32_t stream_id, int32_t tokens, int32_t *n
 int qkv_pager_length(const qkv_pager *p, int32_t stream_id, int32_t *tokens);
 int qkv_pager_pages(const qkv_pager *p, int32_t stream_id, int32_t *pages_out, int32_t cap,
                     int32_t *n);
+/* As qkv_stream_fork / qkv_stream_truncate on the page lists alone: the caller
+ * copies page *copy_src to *copy_dst (both -1: nothing to copy). */
+int qkv_pager_fork(qkv_pager *p, int32_t src, int32_t tokens, int32_t *stream_id, int32_t *copy_src, int32_t *copy_dst);
+int qkv_pager_truncate(qkv_pager *p, int32_t stream_id, int32_t tokens, int32_t *copy_src, int32_t *copy_dst);
 int64_t qkv_pager_free_pages(const qkv_pager *p);
 /* Plan a compaction: live pages above the live count move down into free
  * slots.  Writes up to cap (src, dst) pairs and rewrites the page lists. */
 int qkv_pager_compact(qkv_pager *p, int32_t *src, int32_t *dst, int64_t cap, int64_t *n_moves);
-/* Consistency check (every page owned once, free list disjoint): 0 if sound. */
+/* Consistency check (every page free or counting its holders, free list disjoint): 0 if sound. */
 int qkv_pager_check(const qkv_pager *p);
 
 #ifdef __cplusplus

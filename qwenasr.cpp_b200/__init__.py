@@ -37,6 +37,12 @@ class RuntimeConfig(C.Structure):
                 ("max_pages", C.c_int64), ("max_batch_tokens", C.c_int32), ("page_order_seed", C.c_uint32)]
 
 
+class PoolView(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("layer_bytes", C.c_int64), ("page_bytes", C.c_int64), ("scales", C.c_void_p),
+                ("scales_layer_floats", C.c_int64), ("page_table", C.c_void_p), ("max_pages_per_stream", C.c_int32),
+                ("max_streams", C.c_int32), ("n_pages", C.c_int32), ("n_layers", C.c_int32)]
+
+
 class QkvError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"{STATUS.get(code, code)}: {msg}")
@@ -74,6 +80,13 @@ SIGNATURES = {
     "qkv_layer_forward": (C.c_int, [_P, C.c_int32, C.c_int32, _F32P, _F32P]),
     "qkv_kv_append": (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P, _P, _P, _P]),
     "qkv_kv_attend": (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P, _P, _P, _P]),
+    "qkv_chunk_append": (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P, _P, _I32P, C.c_int32, _P, _P, C.c_int32, _P]),
+    "qkv_chunk_attend": (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P, _P, C.c_int32, _P, _P, _P, _P]),
+    "qkv_pages_copy": (C.c_int, [_P, C.c_int32, _P, _P, _P]),
+    "qkv_tokens_move": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, _P, C.c_int32, _P, _P]),
+    "qkv_stream_fork": (C.c_int, [_P, C.c_int32, C.c_int32, _I32P, _P]),
+    "qkv_stream_truncate": (C.c_int, [_P, C.c_int32, C.c_int32, _P]),
+    "qkv_pool_view_get": (C.c_int, [_P, C.POINTER(PoolView)]),
     "qkv_kv_step": (C.c_int, [_P, C.c_int32, _I32P, _P, _P, _P]),
     "qkv_kv_step_host": (C.c_int, [_P, C.c_int32, _I32P, _P, _P]),
     "qkv_stream_extend": (C.c_int, [_P, C.c_int32, C.c_int32]),
@@ -110,6 +123,8 @@ SIGNATURES = {
     "qkv_pager_append": (C.c_int, [_P, C.c_int32, C.c_int32, _I32P]),
     "qkv_pager_length": (C.c_int, [_P, C.c_int32, _I32P]),
     "qkv_pager_pages": (C.c_int, [_P, C.c_int32, _I32P, C.c_int32, _I32P]),
+    "qkv_pager_fork": (C.c_int, [_P, C.c_int32, C.c_int32, _I32P, _I32P, _I32P]),
+    "qkv_pager_truncate": (C.c_int, [_P, C.c_int32, C.c_int32, _I32P, _I32P]),
     "qkv_pager_free_pages": (C.c_int64, [_P]),
     "qkv_pager_compact": (C.c_int, [_P, _I32P, _I32P, C.c_int64, _I64P]),
     "qkv_pager_check": (C.c_int, [_P]),
@@ -320,6 +335,22 @@ class Decoder:
         self._check(lib.qkv_compact(self.h, C.byref(m)))
         return m.value
 
+    def fork(self, src: int, tokens: int, stream=None) -> int:
+        """A new stream that starts with the first `tokens` tokens of src (qkv_stream_fork)."""
+        s = C.c_int32()
+        self._check(lib.qkv_stream_fork(self.h, src, tokens, C.byref(s), stream))
+        return s.value
+
+    def truncate(self, s: int, tokens: int, stream=None):
+        """Give back the tokens of s past the first `tokens` (qkv_stream_truncate)."""
+        self._check(lib.qkv_stream_truncate(self.h, s, tokens, stream))
+
+    def pool_info(self) -> dict:
+        """Device addresses and sizes of the pool, its scales and the page table (qkv_pool_view)."""
+        v = PoolView()
+        self._check(lib.qkv_pool_view_get(self.h, C.byref(v)))
+        return {f: getattr(v, f) for f, _ in PoolView._fields_}
+
     def pages(self, s: int) -> np.ndarray:
         n = C.c_int32()
         buf = np.zeros(4096, np.int32)
@@ -446,6 +477,30 @@ class Decoder:
         self._check(lib.qkv_prefill_attend_q16(self.h, layer, len(streams), _ptr(streams, C.c_int32),
                                                _ptr(lens, C.c_int32), q16_ptr, out_ptr, stream))
 
+    def chunk_append(self, layer, n, slots_ptr, pos_ptr, axes_ptr, sections, interleaved, qkv_ptr, q_out_ptr, q_dtype,
+                     stream=None):
+        """kv_append with a rotary position per axis (axes_ptr: [3][n]); q out as q_dtype (F32 or BF16)."""
+        sec = _i32(sections)
+        if sec.shape != (3,):
+            raise ValueError("sections: three counts of rotation pairs")
+        self._check(lib.qkv_chunk_append(self.h, layer, n, slots_ptr, pos_ptr, axes_ptr, _ptr(sec, C.c_int32),
+                                         int(interleaved), qkv_ptr, q_out_ptr, q_dtype, stream))
+
+    def chunk_attend(self, layer, n, slots_ptr, starts_ptr, lens_ptr, rows, mask_ptr, q_ptr, out_ptr, stream=None):
+        """Attention of a chunk of new tokens per stream (q and out bf16; mask_ptr None: causal)."""
+        self._check(lib.qkv_chunk_attend(self.h, layer, n, slots_ptr, starts_ptr, lens_ptr, rows, mask_ptr, q_ptr,
+                                         out_ptr, stream))
+
+    def pages_copy(self, n, src_ptr, dst_ptr, stream=None):
+        """Pages src[i] -> dst[i] in every layer."""
+        self._check(lib.qkv_pages_copy(self.h, n, src_ptr, dst_ptr, stream))
+
+    def tokens_move(self, n, src_slots_ptr, src_bases_ptr, dst_slots_ptr, dst_bases_ptr, starts_ptr, rows, keep_ptr,
+                    stream=None):
+        """Listed tokens of each group to consecutive positions, in every layer."""
+        self._check(lib.qkv_tokens_move(self.h, n, src_slots_ptr, src_bases_ptr, dst_slots_ptr, dst_bases_ptr,
+                                        starts_ptr, rows, keep_ptr, stream))
+
     def kv_step(self, streams, qkv_ptr: int, out_ptr: int, stream=None):
         streams = _i32(streams)
         self._check(lib.qkv_kv_step(self.h, len(streams), _ptr(streams, C.c_int32), qkv_ptr, out_ptr, stream))
@@ -511,6 +566,22 @@ class Pager:
         if rc:
             raise QkvError(rc, "append")
         return n.value
+
+    def fork(self, src, tokens) -> tuple[int, tuple[int, int] | None]:
+        """(new stream, (page to copy, its copy) or None)."""
+        s, a, b = C.c_int32(), C.c_int32(), C.c_int32()
+        rc = lib.qkv_pager_fork(self.p, src, tokens, C.byref(s), C.byref(a), C.byref(b))
+        if rc:
+            raise QkvError(rc, "fork")
+        return s.value, (a.value, b.value) if a.value >= 0 else None
+
+    def truncate(self, s, tokens) -> tuple[int, int] | None:
+        """(page to copy, its copy) or None."""
+        a, b = C.c_int32(), C.c_int32()
+        rc = lib.qkv_pager_truncate(self.p, s, tokens, C.byref(a), C.byref(b))
+        if rc:
+            raise QkvError(rc, "truncate")
+        return (a.value, b.value) if a.value >= 0 else None
 
     def length(self, s) -> int:
         t = C.c_int32()

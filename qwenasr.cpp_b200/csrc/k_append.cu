@@ -48,16 +48,6 @@ __global__ void page_gather_kernel(const TC *pool, const int *pages, int n_pages
     }
 }
 
-// Copy whole pages (all layers are separate launches): dst[i] <- src[i].
-__global__ void page_copy_kernel(uint4 *pool, const int *src, const int *dst, int n, size_t page_vec) {
-    for (int i = blockIdx.y; i < n; i += gridDim.y) {
-        const uint4 *s = pool + static_cast<size_t>(src[i]) * page_vec;
-        uint4 *d = pool + static_cast<size_t>(dst[i]) * page_vec;
-        for (size_t e = blockIdx.x * blockDim.x + threadIdx.x; e < page_vec; e += static_cast<size_t>(gridDim.x) * blockDim.x)
-            d[e] = s[e];
-    }
-}
-
 __device__ __forceinline__ uint64_t mix64(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
@@ -131,15 +121,6 @@ cudaError_t launch_page_gather(const void *pool, int kv_dtype, const int *pages,
             break;
         default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
-}
-
-cudaError_t launch_page_copy(void *pool_layer, size_t page_bytes, const int *src, const int *dst, int n,
-                             cudaStream_t st) {
-    if (n <= 0) return cudaSuccess;
-    const size_t vec = page_bytes / sizeof(uint4);
-    dim3 grid(static_cast<unsigned>((vec + 255) / 256 < 64 ? (vec + 255) / 256 : 64), n < 1024 ? n : 1024);
-    page_copy_kernel<<<grid, 256, 0, st>>>(static_cast<uint4 *>(pool_layer), src, dst, n, vec);
     return cudaGetLastError();
 }
 

@@ -126,7 +126,74 @@ struct PrefillAttnParams {
     DevError *err;
 };
 
+// Chunk append: AppendParams with rotary angles from three positions a row.
+// a.rope, a.q16_scale, a.q16_f16 and the slices are not used; q goes to
+// a.q16_out as bf16, unscaled, when q_bf16, else to a.q_out as f32.
+struct ChunkAppendParams {
+    AppendParams a;
+    const int *axes;           // [3][n] rotary positions
+    const double *turns;       // [kHeadDim/2] frequencies in turns per position
+    unsigned char axis_of[kHeadDim / 2];   // axis of each rotation pair
+    int q_bf16;
+};
+
+// Chunk attention: stream i of n has queries starts[i] .. starts[i + 1] - 1 of
+// q, the last of its lens[i] cached tokens.  Slot -1: a padding entry.
+struct ChunkAttendParams {
+    int n;
+    int rows;                  // rows of q and out
+    const int *slots;          // [n]
+    const int *starts;         // [n + 1]
+    const int *lens;           // [n]
+    const unsigned long long *mask;   // [rows] visible chunk tokens of each row, or null: causal
+    const uint16_t *q;         // [rows][kQDim] bf16, post-RoPE
+    uint16_t *out;             // [rows][kQDim] bf16
+    const void *pool;          // this layer's pool
+    const float *scales;
+    const int *page_table;
+    int maxp;
+    int max_streams;
+    int n_pages;
+    float scale_log2;          // log2(e) / sqrt(head_dim)
+    int v_int8;
+    DevError *err;
+};
+
+struct PagesCopyParams {
+    int n;
+    const int *src, *dst;      // [n] page ids, or null: the one pair src0, dst0
+    int src0, dst0;
+    void *pool;                // layer 0's pool
+    size_t layer_bytes, page_bytes;
+    float *scales;             // layer 0's scales (or null)
+    size_t scales_layer_elems;
+    int n_pages;
+    DevError *err;
+};
+
+struct TokensMoveParams {
+    int n;                     // groups
+    int rows;                  // entries of keep
+    const int *src_slots, *src_bases, *dst_slots, *dst_bases;   // [n]
+    const int *starts;         // [n + 1]
+    const int *keep;           // [rows]
+    void *pool;
+    size_t layer_bytes;
+    float *scales;
+    size_t scales_layer_elems;
+    const int *page_table;
+    int maxp;
+    int max_streams;
+    int n_pages;
+    DevError *err;
+};
+
 cudaError_t launch_kv_append(const AppendParams &p, int kv_dtype, cudaStream_t st);
+cudaError_t launch_chunk_append(const ChunkAppendParams &p, int kv_dtype, cudaStream_t st);
+// bf16 and 8-bit caches.
+cudaError_t launch_chunk_attn(const ChunkAttendParams &p, int kv_dtype, cudaStream_t st);
+cudaError_t launch_pages_copy(const PagesCopyParams &p, int n_layers, cudaStream_t st);
+cudaError_t launch_tokens_move(const TokensMoveParams &p, int kv_dtype, int n_layers, cudaStream_t st);
 cudaError_t prepare_decode_attn();
 size_t attn_smem_bytes(int kv_dtype);
 cudaError_t launch_decode_attn(const AttendParams &p, int kv_dtype, bool out_bf16, int grid, cudaStream_t st);
@@ -148,8 +215,6 @@ cudaError_t launch_prefill_attn_tc(const PrefillAttnParams &p, int kv_dtype, con
 cudaError_t launch_q_to16(const float *q, int n, float scale, bool f16, void *out, cudaStream_t st);
 cudaError_t launch_page_gather(const void *pool, int kv_dtype, const int *pages, int n_pages_row, int len,
                                int n_pages, void *k_out, void *v_out, DevError *err, cudaStream_t st);
-cudaError_t launch_page_copy(void *pool_layer, size_t page_bytes, const int *src, const int *dst, int n,
-                             cudaStream_t st);
 cudaError_t launch_page_fill(void *pool_layer, float *scales_layer, int kv_dtype, const int *pages, int n,
                              uint64_t seed, cudaStream_t st);
 

@@ -4,7 +4,11 @@
 // a single stream (text-decoder.cpp:1420-1474, cur_len at :186).  Here a pool
 // of fixed-size pages is shared by many streams: a page holds page_tokens
 // tokens of K and V for every layer and kv head of one stream, and each stream
-// owns an ordered page list (its page table row on the device).
+// owns an ordered page list (its page table row on the device).  Streams made
+// by fork share the full pages of their common tokens: a page counts the
+// streams that hold it and returns to the free list with the last of them.
+// Shared pages are full in every stream that holds them, so appending, which
+// only fills a stream's last page, never touches one.
 #pragma once
 
 #include <cstdint>
@@ -30,17 +34,28 @@ public:
     // Make room for `tokens` more tokens; the new pages (in table order) are
     // appended to *added when it is non-null.  All-or-nothing.
     int append(int32_t stream_id, int32_t tokens, std::vector<int32_t> *added, std::string *err);
+    // A new stream holding the first `tokens` tokens of src: their full pages
+    // are shared, a partly filled last one becomes a page of its own, whose
+    // contents the caller copies (*copy_src -> *copy_dst; both -1: nothing to
+    // copy).  All-or-nothing.
+    int fork(int32_t src, int32_t tokens, int32_t *stream_id, int32_t *copy_src, int32_t *copy_dst, std::string *err);
+    // Give back the tokens past the first `tokens` and the pages only they
+    // used.  A last page left partly filled that other streams share is
+    // replaced by a page of the stream's own (*copy_src -> *copy_dst as in
+    // fork), so later appends do not reach theirs.  All-or-nothing.
+    int truncate(int32_t stream_id, int32_t tokens, int32_t *copy_src, int32_t *copy_dst, std::string *err);
     int length(int32_t stream_id, int32_t *tokens, std::string *err) const;
     const std::vector<int32_t> *pages(int32_t stream_id) const;
     bool is_open(int32_t stream_id) const;
     // Compaction plan: every live page with id >= live count moves to the
-    // lowest free id; page lists are rewritten and the free list becomes
-    // [live, n_pages) in ascending order.
+    // lowest free id (a shared page once); page lists are rewritten and the
+    // free list becomes [live, n_pages) in ascending order.
     void compact(std::vector<int32_t> *src, std::vector<int32_t> *dst);
-    // 0 when every page is owned by exactly one stream or is free.
+    // 0 when every page is free or counts exactly the streams that hold it.
     int check(std::string *err) const;
 
 private:
+    void release(int32_t page);   // one holder less; the last one frees the page
     struct Stream {
         bool open = false;
         int32_t tokens = 0;
@@ -50,6 +65,7 @@ private:
     int32_t page_tokens_;
     int32_t max_streams_;
     int32_t max_pages_per_stream_;
+    std::vector<int32_t> refs_;          // streams holding each page
     std::vector<int32_t> free_;          // stack: back() is handed out next
     std::vector<Stream> streams_;
     std::vector<int32_t> free_slots_;    // stack of closed stream ids

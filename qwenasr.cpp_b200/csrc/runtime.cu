@@ -174,6 +174,14 @@ int setup_common(qkv_handle *h, bool with_model_scratch) {
     CK(cudaMalloc(&h->d_rope, rope.size() * sizeof(float2)));
     CK(cudaMemcpy(h->d_rope, rope.data(), rope.size() * sizeof(float2), cudaMemcpyHostToDevice));
 
+    // The chunk append's rotary frequencies in turns (angle / 2 pi) per position.
+    double turns[kHeadDim / 2];
+    for (int i = 0; i < kHeadDim / 2; ++i)
+        turns[i] = std::exp(-log_theta * static_cast<double>(2 * i) / static_cast<double>(kHeadDim)) / (2.0 * std::acos(-1.0));
+    CK(cudaMalloc(&h->d_turns, sizeof turns));
+    CK(cudaMemcpy(h->d_turns, turns, sizeof turns, cudaMemcpyHostToDevice));
+    CK(cudaEventCreateWithFlags(&h->order_ev, cudaEventDisableTiming));
+
     h->pager = new Pager(h->n_pages, kPageTokens, h->rt.max_streams, h->maxp, h->rt.page_order_seed);
     h->last_id.assign(static_cast<size_t>(h->rt.max_streams), -1);
 
@@ -281,6 +289,8 @@ void destroy(qkv_handle *h) {
     cudaFree(h->ap_norm_w); cudaFree(h->ap_norm_b); cudaFree(h->ap_w0); cudaFree(h->ap_b0); cudaFree(h->ap_w1);
     cudaFree(h->ap_b1);
     cudaFree(h->pool); cudaFree(h->scales); cudaFree(h->d_page_table); cudaFree(h->d_rope);
+    cudaFree(h->d_turns);
+    if (h->order_ev) cudaEventDestroy(h->order_ev);
     cudaFree(h->x); cudaFree(h->qkv); cudaFree(h->res_sl); cudaFree(h->sk_ws); cudaFree(h->sk_flags); cudaFree(h->q); cudaFree(h->q_alt); cudaFree(h->gu); cudaFree(h->logits);
     cudaFree(h->am_v); cudaFree(h->am_i); cudaFree(h->am_cnt);
     cudaFree(h->am_keys); cudaFree(h->am_rcnt); cudaFree(h->d_wout_norm);
@@ -774,6 +784,12 @@ int check_streams(qkv_handle *h, int n, const int32_t *streams) {
     return QKV_OK;
 }
 
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Rows one chunk attention takes: its work arithmetic stays inside 32 bits
+// well past it.
+constexpr int kChunkMaxRows = 1 << 20;
+
 // Softmax scale folded into q: 1 / sqrt(head dim) in the log2 domain.
 float attn_scale_log2() { return static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kHeadDim))); }
 
@@ -826,6 +842,51 @@ AttendParams attend_params(qkv_handle *h, int layer, int n, const int *slots, co
     p.scale_log2 = attn_scale_log2();
     p.err = h->d_err;
     return p;
+}
+
+PagesCopyParams pages_copy_params(qkv_handle *h) {
+    PagesCopyParams p{};
+    p.pool = h->pool;
+    p.layer_bytes = h->pool_layer_bytes;
+    p.page_bytes = h->page_bytes;
+    p.scales = h->scales;
+    p.scales_layer_elems = h->scales_layer_elems;
+    p.n_pages = h->n_pages;
+    p.err = h->d_err;
+    return p;
+}
+
+// The page copy and page-table entries [first, last) of a stream that fork or
+// truncate left to do, on the caller's stream; the handle's own stream follows.
+int apply_pages(qkv_handle *h, int32_t s, size_t first, size_t last, int copy_src, int copy_dst, cudaStream_t st) {
+    if (copy_src >= 0) {
+        PagesCopyParams pc = pages_copy_params(h);
+        pc.n = 1;
+        pc.src0 = copy_src;
+        pc.dst0 = copy_dst;
+        CK(launch_pages_copy(pc, h->cfg.n_layers, st));
+        h->launches += 1;
+    }
+    const std::vector<int32_t> *pg = h->pager->pages(s);
+    int *row = h->h_page_table + static_cast<size_t>(s) * h->maxp;
+    for (size_t k = first; k < last; ++k) row[k] = k < pg->size() ? (*pg)[k] : -1;
+    if (last > first)
+        CK(cudaMemcpyAsync(h->d_page_table + static_cast<size_t>(s) * h->maxp + first, row + first,
+                           (last - first) * sizeof(int), cudaMemcpyHostToDevice, st));
+    if (st != h->stream) {
+        CK(cudaEventRecord(h->order_ev, st));
+        CK(cudaStreamWaitEvent(h->stream, h->order_ev, 0));
+    }
+    return QKV_OK;
+}
+
+// Calls that change the page lists on the host cannot be part of a captured graph.
+int refuse_capture(qkv_handle *h, cudaStream_t st, const char *what) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    CK(cudaStreamIsCapturing(st, &cs));
+    if (cs != cudaStreamCaptureStatusNone)
+        return fail(h, QKV_ERR_STATE, std::string(what) + ": the stream is being captured");
+    return QKV_OK;
 }
 
 // Append + attend for `n` decode rows of one layer (rows: slots/pos/lens device arrays).
@@ -1289,14 +1350,11 @@ int qkv_compact(qkv_handle *h, int64_t *moved) {
         int *d_moves = static_cast<int *>(moves.p);
         CK(cudaMemcpy(d_moves, src.data(), src.size() * sizeof(int), cudaMemcpyHostToDevice));
         CK(cudaMemcpy(d_moves + src.size(), dst.data(), dst.size() * sizeof(int), cudaMemcpyHostToDevice));
-        for (int l = 0; l < h->cfg.n_layers; ++l) {
-            CK(launch_page_copy(static_cast<uint8_t *>(h->pool) + h->pool_layer_bytes * static_cast<size_t>(l),
-                                h->page_bytes, d_moves, d_moves + src.size(), static_cast<int>(src.size()), h->stream));
-            if (h->scales) {
-                CK(launch_page_copy(h->scales + h->scales_layer_elems * static_cast<size_t>(l), kPageScales * sizeof(float),
-                                    d_moves, d_moves + src.size(), static_cast<int>(src.size()), h->stream));
-            }
-        }
+        PagesCopyParams pc = pages_copy_params(h);
+        pc.n = static_cast<int>(src.size());
+        pc.src = d_moves;
+        pc.dst = d_moves + src.size();
+        CK(launch_pages_copy(pc, h->cfg.n_layers, h->stream));
         CK(cudaStreamSynchronize(h->stream));
     }
     // Rewrite the whole page table from the pager.
@@ -1758,6 +1816,184 @@ int qkv_prefill_attend_q16(qkv_handle *h, int32_t layer, int32_t n, const int32_
     return prefill_attend_op(h, layer, n, stream_ids, lens, nullptr, q16_dev, out_dev, stream);
 }
 
+int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slots_dev, const int32_t *positions_dev,
+                     const int32_t *axes_dev, const int32_t *sections, int32_t interleaved, const float *qkv_dev,
+                     void *q_out_dev, int32_t q_dtype, void *stream) {
+    if (!h) return QKV_ERR_INVALID_ARG;
+    if (layer < 0 || layer >= h->cfg.n_layers || n < 0 || !sections ||
+        (n > 0 && (!slots_dev || !positions_dev || !axes_dev || !qkv_dev || !q_out_dev)))
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_append: bad layer, count or pointer");
+    if (q_dtype != QKV_F32 && q_dtype != QKV_BF16)
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_append: q goes out as f32 or bf16");
+    if (sections[0] < 0 || sections[1] < 0 || sections[2] < 0 ||
+        static_cast<int64_t>(sections[0]) + sections[1] + sections[2] != kHeadDim / 2)
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_append: the three sections must add up to 64 rotation pairs");
+    if (interleaved && (sections[1] > 21 || sections[2] > 21))   // pairs 1, 4, .. and 2, 5, .. below 64
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_append: interleaved sections do not fit in 64 rotation pairs");
+    if (!aligned16(qkv_dev) || !aligned16(q_out_dev))
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_append: qkv and q_out must be 16-byte aligned");
+    if (n == 0) return QKV_OK;
+    CK(cudaSetDevice(h->device));
+    const qkv_handle::Layer &L = h->layers[static_cast<size_t>(layer)];
+    ChunkAppendParams p{};
+    p.a = append_params(h, layer, n, slots_dev, positions_dev, qkv_dev, nullptr, L.q_norm, L.k_norm);
+    p.q_bf16 = q_dtype == QKV_BF16 ? 1 : 0;
+    if (p.q_bf16) p.a.q16_out = q_out_dev;
+    else p.a.q_out = static_cast<float *>(q_out_dev);
+    p.axes = axes_dev;
+    p.turns = h->d_turns;
+    for (int i = 0; i < kHeadDim / 2; ++i) {
+        int axis;
+        if (interleaved) axis = i % 3 != 0 && i < 3 * sections[i % 3] ? i % 3 : 0;
+        else axis = i < sections[0] ? 0 : (i < sections[0] + sections[1] ? 1 : 2);
+        p.axis_of[i] = static_cast<unsigned char>(axis);
+    }
+    CK(launch_chunk_append(p, h->rt.kv_dtype, static_cast<cudaStream_t>(stream)));
+    h->launches += 1;
+    return QKV_OK;
+}
+
+int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slots_dev, const int32_t *starts_dev,
+                     const int32_t *lens_dev, int32_t rows, const uint64_t *mask_dev, const void *q_dev, void *out_dev,
+                     void *stream) {
+    if (!h) return QKV_ERR_INVALID_ARG;
+    if (layer < 0 || layer >= h->cfg.n_layers || n < 0 || rows < 0 ||
+        (n > 0 && rows > 0 && (!slots_dev || !starts_dev || !lens_dev || !q_dev || !out_dev)))
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_attend: bad layer, count or pointer");
+    if (h->rt.kv_dtype == QKV_F32) return fail(h, QKV_ERR_STATE, "chunk_attend: needs a bf16 or 8-bit cache");
+    if (n > kAttnMaxRows) return fail(h, QKV_ERR_CAPACITY, "chunk_attend: more than 1024 streams");
+    if (rows > kChunkMaxRows) return fail(h, QKV_ERR_CAPACITY, "chunk_attend: more than 2^20 rows");
+    if (!aligned16(q_dev) || !aligned16(out_dev))
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_attend: q and out must be 16-byte aligned");
+    if (n == 0 || rows == 0) return QKV_OK;
+    CK(cudaSetDevice(h->device));
+    ChunkAttendParams p{};
+    p.n = n;
+    p.rows = rows;
+    p.slots = slots_dev;
+    p.starts = starts_dev;
+    p.lens = lens_dev;
+    p.mask = reinterpret_cast<const unsigned long long *>(mask_dev);
+    p.q = static_cast<const uint16_t *>(q_dev);
+    p.out = static_cast<uint16_t *>(out_dev);
+    p.pool = static_cast<const uint8_t *>(h->pool) + h->pool_layer_bytes * static_cast<size_t>(layer);
+    p.scales = h->scales ? h->scales + h->scales_layer_elems * static_cast<size_t>(layer) : nullptr;
+    p.page_table = h->d_page_table;
+    p.maxp = h->maxp;
+    p.max_streams = h->rt.max_streams;
+    p.n_pages = h->n_pages;
+    p.scale_log2 = attn_scale_log2();
+    p.v_int8 = h->rt.kv_dtype == QKV_E4M3K_I8V ? 1 : 0;
+    p.err = h->d_err;
+    CK(launch_chunk_attn(p, h->rt.kv_dtype, static_cast<cudaStream_t>(stream)));
+    h->launches += 1;
+    return QKV_OK;
+}
+
+int qkv_pages_copy(qkv_handle *h, int32_t n, const int32_t *src_dev, const int32_t *dst_dev, void *stream) {
+    if (!h) return QKV_ERR_INVALID_ARG;
+    if (n < 0 || (n > 0 && (!src_dev || !dst_dev))) return fail(h, QKV_ERR_INVALID_ARG, "pages_copy: bad count or pointer");
+    if (n == 0) return QKV_OK;
+    CK(cudaSetDevice(h->device));
+    PagesCopyParams p = pages_copy_params(h);
+    p.n = n;
+    p.src = src_dev;
+    p.dst = dst_dev;
+    CK(launch_pages_copy(p, h->cfg.n_layers, static_cast<cudaStream_t>(stream)));
+    h->launches += 1;
+    return QKV_OK;
+}
+
+int qkv_tokens_move(qkv_handle *h, int32_t n, const int32_t *src_slots_dev, const int32_t *src_bases_dev,
+                    const int32_t *dst_slots_dev, const int32_t *dst_bases_dev, const int32_t *starts_dev, int32_t rows,
+                    const int32_t *keep_dev, void *stream) {
+    if (!h) return QKV_ERR_INVALID_ARG;
+    if (n < 0 || rows < 0 ||
+        (n > 0 && rows > 0 &&
+         (!src_slots_dev || !src_bases_dev || !dst_slots_dev || !dst_bases_dev || !starts_dev || !keep_dev)))
+        return fail(h, QKV_ERR_INVALID_ARG, "tokens_move: bad count or pointer");
+    if (n > 65535) return fail(h, QKV_ERR_CAPACITY, "tokens_move: more than 65535 groups");
+    if (n == 0 || rows == 0) return QKV_OK;
+    CK(cudaSetDevice(h->device));
+    TokensMoveParams p{};
+    p.n = n;
+    p.rows = rows;
+    p.src_slots = src_slots_dev;
+    p.src_bases = src_bases_dev;
+    p.dst_slots = dst_slots_dev;
+    p.dst_bases = dst_bases_dev;
+    p.starts = starts_dev;
+    p.keep = keep_dev;
+    p.pool = h->pool;
+    p.layer_bytes = h->pool_layer_bytes;
+    p.scales = h->scales;
+    p.scales_layer_elems = h->scales_layer_elems;
+    p.page_table = h->d_page_table;
+    p.maxp = h->maxp;
+    p.max_streams = h->rt.max_streams;
+    p.n_pages = h->n_pages;
+    p.err = h->d_err;
+    CK(launch_tokens_move(p, h->rt.kv_dtype, h->cfg.n_layers, static_cast<cudaStream_t>(stream)));
+    h->launches += 1;
+    return QKV_OK;
+}
+
+int qkv_stream_fork(qkv_handle *h, int32_t src, int32_t tokens, int32_t *stream_id, void *stream) {
+    if (!h) return QKV_ERR_INVALID_ARG;
+    if (!stream_id) return fail(h, QKV_ERR_INVALID_ARG, "stream_fork: stream_id is null");
+    CK(cudaSetDevice(h->device));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int rc = refuse_capture(h, st, "stream_fork");
+    if (rc) return rc;
+    return host_alloc_guard(h, [&]() -> int {
+        std::string e;
+        int32_t from = -1, to = -1, s = -1;
+        int r = h->pager->fork(src, tokens, &s, &from, &to, &e);
+        if (r) return fail(h, r, e);
+        // The next decode step continues from src's last greedy id only where
+        // the whole of src is shared.
+        h->last_id[static_cast<size_t>(s)] = tokens == stream_len(h, src) ? h->last_id[static_cast<size_t>(src)] : -1;
+        if ((r = apply_pages(h, s, 0, h->pager->pages(s)->size(), from, to, st))) return r;
+        *stream_id = s;
+        return QKV_OK;
+    });
+}
+
+int qkv_stream_truncate(qkv_handle *h, int32_t stream_id, int32_t tokens, void *stream) {
+    if (!h) return QKV_ERR_INVALID_ARG;
+    CK(cudaSetDevice(h->device));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int rc = refuse_capture(h, st, "stream_truncate");
+    if (rc) return rc;
+    return host_alloc_guard(h, [&]() -> int {
+        std::string e;
+        int32_t from = -1, to = -1;
+        const std::vector<int32_t> *pg = h->pager->pages(stream_id);
+        const size_t before = pg ? pg->size() : 0;
+        const int had = pg ? stream_len(h, stream_id) : 0;
+        const int r = h->pager->truncate(stream_id, tokens, &from, &to, &e);
+        if (r) return fail(h, r, e);
+        if (tokens != had) h->last_id[static_cast<size_t>(stream_id)] = -1;
+        const size_t after = h->pager->pages(stream_id)->size();
+        return apply_pages(h, stream_id, from >= 0 ? after - 1 : after, before, from, to, st);
+    });
+}
+
+int qkv_pool_view_get(const qkv_handle *h, qkv_pool_view *view) {
+    if (!h || !view) return QKV_ERR_INVALID_ARG;
+    view->pool = h->pool;
+    view->layer_bytes = static_cast<int64_t>(h->pool_layer_bytes);
+    view->page_bytes = static_cast<int64_t>(h->page_bytes);
+    view->scales = h->scales;
+    view->scales_layer_floats = static_cast<int64_t>(h->scales_layer_elems);
+    view->page_table = h->d_page_table;
+    view->max_pages_per_stream = h->maxp;
+    view->max_streams = h->rt.max_streams;
+    view->n_pages = h->n_pages;
+    view->n_layers = h->cfg.n_layers;
+    return QKV_OK;
+}
+
 int qkv_kv_step(qkv_handle *h, int32_t n, const int32_t *stream_ids, const float *qkv_dev, float *out_dev, void *stream) {
     const TraceRange trace("qkv_kv_step");
     if (!h) return QKV_ERR_INVALID_ARG;
@@ -2186,6 +2422,17 @@ int qkv_pager_pages(const qkv_pager *p, int32_t stream_id, int32_t *pages_out, i
     *n = static_cast<int32_t>(pg->size());
     for (int32_t i = 0; i < cap && i < *n; ++i) pages_out[i] = (*pg)[static_cast<size_t>(i)];
     return QKV_OK;
+}
+int qkv_pager_fork(qkv_pager *p, int32_t src, int32_t tokens, int32_t *stream_id, int32_t *copy_src, int32_t *copy_dst) {
+    if (!p) return QKV_ERR_INVALID_ARG;
+    try {
+        return reinterpret_cast<Pager *>(p)->fork(src, tokens, stream_id, copy_src, copy_dst, nullptr);
+    } catch (const std::exception &) {
+        return QKV_ERR_HOST_MEMORY;
+    }
+}
+int qkv_pager_truncate(qkv_pager *p, int32_t stream_id, int32_t tokens, int32_t *copy_src, int32_t *copy_dst) {
+    return p ? reinterpret_cast<Pager *>(p)->truncate(stream_id, tokens, copy_src, copy_dst, nullptr) : QKV_ERR_INVALID_ARG;
 }
 int64_t qkv_pager_free_pages(const qkv_pager *p) { return p ? reinterpret_cast<const Pager *>(p)->free_pages() : -1; }
 int qkv_pager_compact(qkv_pager *p, int32_t *src, int32_t *dst, int64_t cap, int64_t *n_moves) {

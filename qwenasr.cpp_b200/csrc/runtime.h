@@ -61,6 +61,8 @@ struct qkv_handle {
     int *h_page_table = nullptr;    // pinned mirror [max_streams][maxp]
     float2 *d_rope = nullptr;
     int rope_len = 0;
+    double *d_turns = nullptr;  // [kHeadDim/2] rotary frequencies in turns per position
+    cudaEvent_t order_ev = nullptr;   // orders the handle's stream behind a caller's (fork, truncate)
     qkv::Pager *pager = nullptr;
 
     // scratch (rows = max(max_batch_tokens, max_streams))
