@@ -137,6 +137,12 @@ struct ChunkAppendParams {
     int q_bf16;
 };
 
+// A unit of the chunk attention that starts in one CTA and ends in CTA c_last
+// (-1: none): its query rows, kv head and mode.
+struct ChunkSplit {
+    int row0, nq, g, pair, c_last;
+};
+
 // Chunk attention: stream i of n has queries starts[i] .. starts[i + 1] - 1 of
 // q, the last of its lens[i] cached tokens.  Slot -1: a padding entry.
 struct ChunkAttendParams {
@@ -157,6 +163,14 @@ struct ChunkAttendParams {
     float scale_log2;          // log2(e) / sqrt(head_dim)
     int v_int8;
     DevError *err;
+    // workspace (chunk_workspace): two pieces per CTA of rows cut between CTAs
+    float *part_o;
+    float2 *part_ml;           // (reference maximum in log2, sum)
+    ChunkSplit *splits;        // [CTAs]
+};
+
+struct ChunkWorkspace {
+    size_t part_o, part_ml, splits;   // elements
 };
 
 struct PagesCopyParams {
@@ -191,7 +205,9 @@ struct TokensMoveParams {
 cudaError_t launch_kv_append(const AppendParams &p, int kv_dtype, cudaStream_t st);
 cudaError_t launch_chunk_append(const ChunkAppendParams &p, int kv_dtype, cudaStream_t st);
 // bf16 and 8-bit caches.
-cudaError_t launch_chunk_attn(const ChunkAttendParams &p, int kv_dtype, cudaStream_t st);
+ChunkWorkspace chunk_workspace(int num_sms);
+cudaError_t prepare_chunk_attn();
+cudaError_t launch_chunk_attn(const ChunkAttendParams &p, int kv_dtype, int num_sms, cudaStream_t st);
 cudaError_t launch_pages_copy(const PagesCopyParams &p, int n_layers, cudaStream_t st);
 cudaError_t launch_tokens_move(const TokensMoveParams &p, int kv_dtype, int n_layers, cudaStream_t st);
 cudaError_t prepare_decode_attn();

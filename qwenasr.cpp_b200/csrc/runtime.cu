@@ -252,6 +252,13 @@ int setup_common(qkv_handle *h, bool with_model_scratch) {
     CK(cudaMalloc(&h->part_ml, slots * kHq * 2 * sizeof(float)));
     CK(cudaMalloc(&h->counters, static_cast<size_t>(kAttnMaxRows) * kHkv * sizeof(int)));
     CK(cudaMemset(h->counters, 0, static_cast<size_t>(kAttnMaxRows) * kHkv * sizeof(int)));
+    if (h->rt.kv_dtype != QKV_F32) {
+        const ChunkWorkspace ws = chunk_workspace(h->num_sms);
+        CK(cudaMalloc(&h->chunk_o, ws.part_o * sizeof(float)));
+        CK(cudaMalloc(&h->chunk_ml, ws.part_ml * sizeof(float2)));
+        CK(cudaMalloc(&h->chunk_splits, ws.splits * sizeof(ChunkSplit)));
+        CK(prepare_chunk_attn());
+    }
     CK(cudaMalloc(&h->d_err, sizeof(DevError)));
     CK(cudaMemset(h->d_err, 0, sizeof(DevError)));
     CK(cudaMallocHost(&h->h_err, sizeof(DevError)));
@@ -289,7 +296,7 @@ void destroy(qkv_handle *h) {
     cudaFree(h->ap_norm_w); cudaFree(h->ap_norm_b); cudaFree(h->ap_w0); cudaFree(h->ap_b0); cudaFree(h->ap_w1);
     cudaFree(h->ap_b1);
     cudaFree(h->pool); cudaFree(h->scales); cudaFree(h->d_page_table); cudaFree(h->d_rope);
-    cudaFree(h->d_turns);
+    cudaFree(h->d_turns); cudaFree(h->chunk_o); cudaFree(h->chunk_ml); cudaFree(h->chunk_splits);
     if (h->order_ev) cudaEventDestroy(h->order_ev);
     cudaFree(h->x); cudaFree(h->qkv); cudaFree(h->res_sl); cudaFree(h->sk_ws); cudaFree(h->sk_flags); cudaFree(h->q); cudaFree(h->q_alt); cudaFree(h->gu); cudaFree(h->logits);
     cudaFree(h->am_v); cudaFree(h->am_i); cudaFree(h->am_cnt);
@@ -1885,8 +1892,11 @@ int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
     p.scale_log2 = attn_scale_log2();
     p.v_int8 = h->rt.kv_dtype == QKV_E4M3K_I8V ? 1 : 0;
     p.err = h->d_err;
-    CK(launch_chunk_attn(p, h->rt.kv_dtype, static_cast<cudaStream_t>(stream)));
-    h->launches += 1;
+    p.part_o = h->chunk_o;
+    p.part_ml = h->chunk_ml;
+    p.splits = h->chunk_splits;
+    CK(launch_chunk_attn(p, h->rt.kv_dtype, h->num_sms, static_cast<cudaStream_t>(stream)));
+    h->launches += 2;
     return QKV_OK;
 }
 

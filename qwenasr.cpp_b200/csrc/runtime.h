@@ -147,6 +147,10 @@ struct qkv_handle {
     int max_items = 0;
     float *part_o = nullptr, *part_ml = nullptr;
     int *counters = nullptr;
+    // qkv_chunk_attend's workspace (bf16 and 8-bit caches)
+    float *chunk_o = nullptr;
+    float2 *chunk_ml = nullptr;
+    qkv::ChunkSplit *chunk_splits = nullptr;
     qkv::DevError *d_err = nullptr;
     qkv::DevError *h_err = nullptr;
     std::vector<int32_t> last_id;   // per slot: last greedy id
