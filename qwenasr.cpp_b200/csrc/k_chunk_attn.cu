@@ -5,38 +5,44 @@
 // out[r] = sum_k softmax_k(q_r . k / sqrt(128)) v over the visible tokens; zero
 // where none is visible.  bf16 and 8-bit caches, tensor cores (tcgen05, TMEM).
 //
-// Tiles.  A query tile is 128 MMA rows: 64 queries x the two q heads of a kv
-// head g (row 2 i + h), so a K/V tile of 128 keys (8 pages) is fetched once for
-// both heads.  S = Q K^T and O += P V are 128 x 128 x 128 each; S and O lie in
-// TMEM, P goes back into S's columns as bf16 and is the A operand of P V from
-// there.  Two lanes (a softmax warpgroup, an S/P region and an O region each)
-// take turns on the tensor cores, so that one lane's MMAs run under the other's
-// softmax:
-//   pair       (more than 64 queries) the lanes hold query tiles q0 and q0 + 64
-//              and both go over every key tile;
-//   alternate  (at most 64 queries) both lanes hold the one query tile, lane 0
-//              takes the even key tiles of the segment and lane 1 the odd ones;
-//              their (max, sum, O) are joined at the segment's end.  A short
-//              chunk is bound by reading its context; with half the tiles each,
-//              the two lanes' latencies overlap.
+// A K/V tile is 128 keys (8 pages) of one kv head g, fetched once for the two q
+// heads it serves.  Two lanes (a softmax warpgroup, an S region and an O region
+// of TMEM each) take turns on the tensor cores, so that one lane's MMAs run
+// under the other's softmax.  A unit, (stream, g, up to 128 queries), runs in
+// one of three modes by its number of queries:
+//   pair       65..128: each lane holds a query tile of 128 MMA rows (64 queries
+//              x 2 heads, row 2 i + h) and both go over every key tile;
+//   alternate  17..64: both lanes hold the one query tile, lane 0 takes the even
+//              key tiles of the segment and lane 1 the odd ones;
+//   thin       1..16: the lanes alternate too, but with keys and queries
+//              exchanged, S' = K Q' and O' = V' P' (128 keys x 16 or 32 columns).
+// In pair and alternate mode S = Q K', thread = query row; P goes back over S as
+// bf16 and is the A operand of P V in TMEM.  That costs a thread 128
+// exponentials a tile however few rows are real, which a short chunk, bound by
+// reading its context, cannot hide (186 us where 53 us are read: 64 draft trees
+// of 3 to 12 rows); in thin mode a thread has one key and computes 16 or 32.
 //
-// Work split.  A unit is (stream, kv head, 128-query block), its work w T: T
-// key tiles, w = 2 in pair mode and 1 in alternate mode.  All units laid end to
-// end are cut into equal parts, one per CTA (one CTA per SM), wherever the cuts
-// fall; a unit cut into pieces leaves (max, sum, unnormalised O) per piece in
-// the workspace, and a second kernel joins them in order.  The cuts follow
-// from the lengths in device memory alone, so a captured call serves other
-// lengths.  Every role walks its CTA's segments by the same arithmetic.
+// Work split.  A unit's work is w T: T key tiles, w = 2 in pair mode and 1
+// elsewhere.  All units laid end to end are cut into equal parts, one per CTA
+// (one CTA per SM), wherever the cuts fall; a unit cut into pieces leaves (max,
+// sum, unnormalised O) per piece in the workspace, and a second kernel joins
+// them in order.  The cuts follow from the lengths in device memory alone, so a
+// captured call serves other lengths.  Every role walks its CTA's segments by
+// the same arithmetic.
 //
-// Softmax: thread = row.  P is taken against a reference maximum that moves
-// only when a tile exceeds it by more than 2^8 (then O and the sum are
-// rescaled); so P <= 2^8, rounded to bf16 once (2^-9 of the weight on average),
-// the sum kept in f32 from the unrounded values.  8-bit caches: the codes are
-// exact in bf16; a key's scale multiplies its scores, a value's scale its P.
+// Softmax.  P is taken against a reference that moves only when a tile exceeds
+// it by more than 2^kRescaleLog2 (then O and the sum are rescaled); P, the sum
+// and O are floating-point numbers and lose nothing to a common factor.  P is
+// rounded to bf16 once (2^-8 of the weight at most); sums stay in f32 and take
+// the unrounded values.  8-bit caches: the codes are exact in bf16; a key's
+// scale multiplies its scores, a value's scale its P.
 //
 // Roles: warps 0..3 loaders (cp.async into the swizzled tiles; 8-bit codes are
 // converted on the way), warps 4..7 lane 0, warps 8..11 lane 1, warp 12 MMA.
-// All waits bounded.
+// All waits bounded; a softmax warp whose wait ran out goes on without waiting,
+// so that the named barriers stay matched.
+#include <type_traits>
+
 #include "kernels.h"
 
 #include "ktc.cuh"
@@ -51,7 +57,13 @@ constexpr int kMmaWarp = 12;
 constexpr int kThreads = 13 * 32;
 constexpr uint32_t kTmemCols = 512;        // S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512)
 constexpr uint32_t kTmemO = 256;
-constexpr float kRescaleLog2 = 8.0f;
+constexpr float kRescaleLog2 = 30.0f;
+constexpr int kThinQueries = 16;           // most queries of thin mode
+enum Mode { kThin = 0, kAlternate = 1, kPair = 2 };
+// The two 32 KB areas before the stages: a query tile each, or area 1 split
+// between thin mode's two query buffers (32 rows) and the lanes' P tiles.
+constexpr uint32_t kThinQ = kTileBytes, kThinQBytes = 8192, kThinQBlk = 4096;
+constexpr uint32_t kThinP = kTileBytes + 16384, kThinPBytes = 8192;
 constexpr int kMinCost = 2;                // least work of a CTA (tiles of alternate mode)
 constexpr int kPieceRows = 256;            // rows of a workspace piece (pair mode: both lanes)
 
@@ -69,10 +81,12 @@ template <bool k8> struct Layout {
     static constexpr size_t kTailOff = kRawScaleOff + kRaw * 2 * kKeys * sizeof(float);
 };
 
-struct Tail {
-    uint64_t q_full[2], q_empty[2], full[5], empty[5], s_full[2], p_full[2], pv_done[2], epi_done, x_ready, mma_done;
+struct alignas(16) Tail {
+    uint64_t q_full[2], seg_done[2];       // of a segment, by its parity
+    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], epi_done, mma_done;
     uint64_t scale_full[4];                // 8-bit: the scales of a tile are in the ring
-    float2 ml[2][128];                     // alternate mode: (max, sum) of each lane's rows
+    float2 ml[2][128];                     // (reference, sum) of each lane's rows, at a segment's end
+    float thin_ref[2][32];                 // thin mode: the lane's reference per column
     long long warp_sum[kThreads / 32];
     int warp_max[kThreads / 32];
     long long pre0;                        // work before entry i0, where this CTA's part starts
@@ -125,10 +139,18 @@ __device__ __forceinline__ Entry load_entry(const ChunkAttendParams &p, int i, i
 struct Segment {
     int slot, g, row0, nq, q0pos, base, len_end;   // query rows row0.., the first at position q0pos; keys [0, len_end)
     int t0, t1;                                    // key tiles
-    bool pair, first, last;                        // holds the unit's first / last tile
+    int mode, cols;                                // cols: thin mode's columns (2 nq rounded up to 16)
+    bool first, last;                              // holds the unit's first / last tile
     long long ustart;
     int tiles;                                     // of the unit
+    __device__ __forceinline__ bool pair() const { return mode == kPair; }
 };
+
+// Areas that a segment's Q (thin: and P) takes, as a bit set, after a segment
+// with `prev`; an alternate segment avoids its predecessor's.
+__device__ __forceinline__ uint32_t q_areas(int mode, uint32_t prev) {
+    return mode == kPair ? 3u : (mode == kThin ? 2u : (prev & 1u ? 2u : 1u));
+}
 
 struct Walk {
     Entry e;
@@ -176,7 +198,8 @@ struct Walk {
             s.q0pos = e.base + b * 2 * kQueries;
             // with a mask a row may see any token of its chunk; causal blocks end at their last query
             s.len_end = s.q0pos + cnt;
-            s.pair = w == 2;
+            s.mode = w == 2 ? kPair : (cnt > kThinQueries ? kAlternate : kThin);
+            s.cols = cnt > 8 ? 32 : 16;
             s.first = s.t0 == 0;
             s.last = s.t1 == s.tiles;
             s.ustart = ustart;
@@ -196,7 +219,7 @@ struct Walk {
 // earlier.
 __device__ __forceinline__ int lane_tiles(const Segment &s, int lane) {
     const int n = s.t1 - s.t0;
-    if (!s.pair) return (n + 1 - lane) >> 1;
+    if (!s.pair()) return (n + 1 - lane) >> 1;
     if (lane == 1) return n;
     return max(0, min(s.t1, (s.q0pos + kQueries + kKeys - 1) / kKeys) - s.t0);
 }
@@ -238,6 +261,105 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src, uint32_t s
                  : "memory");
 }
 
+// Packed pairs of f32 (two lanes of one instruction).
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void un_f2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Named barriers of a softmax warpgroup (128 threads) and of both (256).
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    asm volatile("barrier.cta.sync.aligned %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool bar_any(int id, int threads, bool pred) {
+    int r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred.aligned q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(static_cast<int>(pred)), "r"(id), "r"(threads)
+        : "memory");
+    return r != 0;
+}
+constexpr int kBarLane = 1, kBarBoth = 3;   // ids kBarLane + lane, kBarBoth
+
+// kCols TMEM columns of this thread's lane; usable after tmem_wait_ld_regs.
+template <int kCols> __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[kCols]) {
+    static_assert(kCols == 8 || kCols == 16 || kCols == 32, "");
+    if constexpr (kCols == 32) {
+        tmem_ld32_issue(taddr, r);
+    } else if constexpr (kCols == 16) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+            "%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr));
+    } else {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(taddr));
+    }
+}
+template <int kCols> __device__ __forceinline__ void tmem_wait_ld_regs(uint32_t (&r)[kCols]) {
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) asm volatile("" : "+r"(r[j]));   // no use moves ahead of the wait
+}
+
+// Thin mode's P (bf16, [128 keys][kCols], columns contiguous: MN-major B):
+// rows of 32 or 64 bytes, swizzled over 256 or 512 bytes.
+__device__ __forceinline__ uint64_t desc_thin_p(uint32_t addr, int cols) {
+    return ((addr >> 4) & 0x3FFFull) | (1ull << 16) | (static_cast<uint64_t>(cols) << 32) | (1ull << 46) |
+           ((cols == 16 ? 6ull : 4ull) << 61);   // 8-key groups 16 cols bytes apart
+}
+__device__ __forceinline__ uint32_t idesc_thin(int cols) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(cols >> 3) << 17) | ((128u >> 4) << 24);
+}
+constexpr uint32_t kIdescTransposeAB = (1u << 15) | (1u << 16);
+
+// Sum of each of kCols registers over the warp's 32 lanes: afterwards v[0]
+// holds column lane / (32 / kCols).
+template <int kCols> __device__ __forceinline__ void warp_column_sums(float (&v)[kCols], int lane) {
+    int o = 16;
+#pragma unroll
+    for (int cnt = kCols / 2; cnt >= 1; cnt >>= 1, o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int j = 0; j < cnt; ++j) {
+            const float send = up ? v[j] : v[j + cnt], keep = up ? v[j + cnt] : v[j];
+            v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    }
+    for (; o >= 1; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+}
+
+// Largest of x over the warp (redux on the order-preserving integer image).
+__device__ __forceinline__ float warp_max(float x) {
+    int i = __float_as_int(x);
+    i ^= (i >> 31) & 0x7fffffff;
+    i = __reduce_max_sync(0xffffffffu, i);
+    i ^= (i >> 31) & 0x7fffffff;
+    return __int_as_float(i);
+}
+
 // Order of the loader's items in a segment of n tiles: K_0, then K_{i+1}, V_i
 // for every i (the MMA order), V_{n-1} last; each takes the next stage.
 __device__ __forceinline__ uint32_t item_of_k(int i) { return i == 0 ? 0 : 2 * i - 1; }
@@ -264,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tail->q_full[b], 128);
-            mbar_init(&tail->q_empty[b], 1);
+            mbar_init(&tail->seg_done[b], 1);
             mbar_init(&tail->s_full[b], 1);
             mbar_init(&tail->p_full[b], 128);
             mbar_init(&tail->pv_done[b], 1);
@@ -274,7 +396,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
             mbar_init(&tail->empty[b], 1);
         }
         mbar_init(&tail->epi_done, 256);
-        mbar_init(&tail->x_ready, 256);
         mbar_init(&tail->mma_done, 1);
         for (int b = 0; b < L::kScaleRing; ++b) mbar_init(&tail->scale_full[b], 128);
         tail->failed = 0;
@@ -352,18 +473,21 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
     if (warp < 4) {
         // ================= loaders =================
         const int t = tid;
-        uint32_t u = 0, q_fill[2] = {0, 0}, tile_no = 0;
-        int qb = 1;
-        bool ok = true;
+        uint32_t u = 0, seg = 0, areas = 0, tile_no = 0;
+        bool ok = true, was_thin = false;
         // bf16: barriers of the items issued and not yet signalled, oldest first.
-        // 8-bit: the items in the raw ring instead, as scale slot x 2 + K|V.
+        // 8-bit: the items in the raw ring instead, as scale slot x 2 + K|V, and
+        // the barrier of a Q in flight with the copies committed behind it.
         uint64_t *pend[L::kLag] = {};
         uint32_t meta[3] = {0, 0, 0};
-        int waiting = 0;
+        int waiting = 0, behind_q = 0;
+        uint64_t *q_bar = nullptr;
         uint32_t u_conv = 0;
         auto signal_all = [&]() {
             cp_async_wait<0>();
             fence_async_smem();
+            if (k8 && q_bar) mbar_arrive(q_bar);
+            q_bar = nullptr;
 #pragma unroll
             for (int j = 0; j < L::kLag; ++j) {
                 if (pend[j]) mbar_arrive(pend[j]);
@@ -433,37 +557,48 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
         while (ok && walk.next(p, s) && !*failed) {
             const int *pt = p.page_table + static_cast<size_t>(s.slot) * p.maxp;
             const int key_pages = (s.len_end + kPageTokens - 1) / kPageTokens;
-            // Q rows: row 2 i + h, 256 bytes each; rows past the queries are not read by anyone
-            for (int j = 0; ok && j < (s.pair ? 2 : 1); ++j) {
-                qb = s.pair ? j : qb ^ 1;
-                if constexpr (k8) {
-                    // Q may be held by tiles that still lie unconverted here
-                    if (!mbar_try_wait(&tail->q_empty[qb], (q_fill[qb] & 1u) ^ 1u)) {
-                        cp_async_wait<0>();
-                        while (ok && waiting > 0) ok = convert();
-                    }
+            // Q takes the areas of an earlier segment: the one before last has always ended (its Q barrier is
+            // reused), the last one if they meet.
+            const uint32_t prev = areas;
+            areas = q_areas(s.mode, prev);
+            const bool meets = (areas & prev) && !(s.mode == kThin && was_thin);
+            was_thin = s.mode == kThin;
+            for (int back = 2; ok && back >= (meets ? 1 : 2); --back) {
+                if (seg < static_cast<uint32_t>(back)) continue;
+                uint64_t *bar = &tail->seg_done[(seg - back) & 1u];
+                const uint32_t par = ((seg - back) >> 1) & 1u;
+                if (k8 && !mbar_try_wait(bar, par)) {   // tiles of that segment may still lie unconverted here
+                    signal_all();
+                    while (ok && waiting > 0) ok = convert();
                 }
-                if (!(ok = ok && wait_empty(&tail->q_empty[qb], (q_fill[qb] & 1u) ^ 1u))) break;
-                ++q_fill[qb];
-                const int rows = 2 * min(kQueries, s.nq - j * kQueries);
-                uint8_t *dst = smem + qb * kTileBytes + ((t & 15) >> 3) * kBlkBytes;
+                ok = ok && wait_empty(bar, par);
+            }
+            if (!ok) break;
+            // Q rows: row 2 i + h, 256 bytes each.  Rows past the queries: zero in thin mode, where they are
+            // columns beside real ones; elsewhere no one reads them.
+            for (int j = 0; j < (s.pair() ? 2 : 1); ++j) {
+                const bool thin = s.mode == kThin;
+                const int rows = 2 * min(kQueries, s.nq - j * kQueries), fill = thin ? s.cols : rows;
+                const uint32_t blk = thin ? kThinQBlk : kBlkBytes;
+                uint8_t *dst = smem + (thin ? kThinQ + (seg & 1u) * kThinQBytes
+                                            : (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes)) +
+                               ((t & 15) >> 3) * blk;
                 const uint16_t *src = p.q + static_cast<size_t>(s.row0 + j * kQueries) * kQDim + 2 * s.g * kHeadDim + 8 * (t & 15);
 #pragma unroll
                 for (int m = 0; m < 16; ++m) {
                     const int row = (t >> 4) + 8 * m;
-                    if (row < rows)
-                        cp_async16(dst + swz(row, t & 7), src + static_cast<size_t>(row >> 1) * kQDim + (row & 1) * kHeadDim, 16u);
-                }
-                if constexpr (k8) {
-                    cp_async_commit();
-                    cp_async_wait<0>();
-                    fence_async_smem();
-                    mbar_arrive(&tail->q_full[qb]);
-                } else {
-                    issued(&tail->q_full[qb]);
+                    if (row < fill)
+                        cp_async16(dst + swz(row, t & 7), src + (row < rows ? static_cast<size_t>(row >> 1) * kQDim + (row & 1) * kHeadDim : 0),
+                                   row < rows ? 16u : 0u);
                 }
             }
-            if (!ok) break;
+            if constexpr (k8) {
+                cp_async_commit();
+                q_bar = &tail->q_full[seg & 1u];
+                behind_q = 0;
+            } else {
+                issued(&tail->q_full[seg & 1u]);
+            }
             const int n = s.t1 - s.t0;
             // pages of the tile whose K / V comes next: V runs one tile behind K
             int pg_k[8], pg_v[8];
@@ -522,7 +657,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
                     if (waiting == 0) meta[0] = mt;
                     else if (waiting == 1) meta[1] = mt;
                     else meta[2] = mt;
-                    if (++waiting == L::kRaw) cp_async_wait<(L::kRaw > 0 ? L::kRaw - 1 : 0)>();
+                    ++waiting;
+                    cp_async_wait<(L::kRaw > 0 ? L::kRaw - 1 : 0)>();
+                    if (q_bar && ++behind_q == L::kRaw - 1) {   // Q has landed
+                        fence_async_smem();
+                        mbar_arrive(q_bar);
+                        q_bar = nullptr;
+                    }
                 }
                 ++u;
                 if (bad) {
@@ -544,52 +685,50 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
                 ok = ok && load(s.t0 + i, 1, pg_v, (tile_no + i) % L::kScaleRing);
             }
             tile_no += n;
+            ++seg;
         }
+        signal_all();
         if constexpr (k8) {
-            cp_async_wait<0>();
             while (ok && waiting > 0) ok = convert();
-        } else {
-            signal_all();
         }
         cp_async_wait<0>();   // no copy outlives the CTA
     } else if (warp == kMmaWarp) {
         // ================= MMA issuer =================
         if (lane == 0) {
             bool ok = true;
-            uint32_t u0 = 0, q_use[2] = {0, 0}, p_cnt[2] = {0, 0}, seg = 0;
-            int qb = 1;
+            uint32_t u0 = 0, p_cnt[2] = {0, 0}, seg = 0, areas = 0;
             while (ok && walk.next(p, s)) {
                 const int n = s.t1 - s.t0;
-                const int n_l[2] = {lane_tiles(s, 0), lane_tiles(s, 1)};
-                int qbuf[2];
-                if (s.pair) {
-                    qb = 1;
-                    qbuf[0] = 0;
-                    qbuf[1] = 1;
-                } else {
-                    qb ^= 1;
-                    qbuf[0] = qbuf[1] = qb;
-                }
-                for (int b = 0; b < 2; ++b) {
-                    if (!(s.pair || b == qb)) continue;
-                    ok = ok && wait_bar(&tail->q_full[b], q_use[b] & 1u, failed);
-                    ++q_use[b];
-                }
-                if (!ok) break;
+                const int n0 = lane_tiles(s, 0);
+                areas = q_areas(s.mode, areas);
+                if (!(ok = wait_bar(&tail->q_full[seg & 1u], (seg >> 1) & 1u, failed))) break;
                 auto stage_of = [&](uint32_t item) { return (u0 + item) % L::kStages; };
                 auto wait_item = [&](uint32_t item) {
                     return wait_bar(&tail->full[(u0 + item) % L::kStages], ((u0 + item) / L::kStages) & 1u, failed);
                 };
+                const bool thin = s.mode == kThin;
+                const uint32_t aQ0 = smem_u32(smem) + (thin ? kThinQ + (seg & 1u) * kThinQBytes
+                                                            : (s.pair() ? 0u : (areas >> 1) * kTileBytes));
+                const uint32_t id_thin = idesc_thin(s.cols);
                 // S of the lane's tile from K stage `stage`
                 auto issue_s = [&](int l, uint32_t stage) {
                     fence_after();
-                    const uint32_t aQ = smem_u32(smem + qbuf[l] * kTileBytes);
                     const uint32_t aK = smem_u32(smem + L::kStageOff + stage * kTileBytes);
+                    const uint32_t aQ = aQ0 + (s.pair() ? l * kTileBytes : 0u);
+                    if (thin) {
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        const uint32_t off = static_cast<uint32_t>(kk >> 2) * kBlkBytes;
-                        const uint64_t step = 2ull * static_cast<uint64_t>(kk & 3);
-                        mma(tmem + l * 128u, desc_kmajor(aQ + off) + step, desc_kmajor(aK + off) + step, idesc_s<false>(), kk > 0);
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint64_t step = 2ull * static_cast<uint64_t>(kk & 3);
+                            mma(tmem + l * 128u, desc_kmajor(aK + (kk >> 2) * kBlkBytes) + step,
+                                desc_kmajor(aQ + (kk >> 2) * kThinQBlk) + step, id_thin, kk > 0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint32_t off = static_cast<uint32_t>(kk >> 2) * kBlkBytes;
+                            const uint64_t step = 2ull * static_cast<uint64_t>(kk & 3);
+                            mma(tmem + l * 128u, desc_kmajor(aQ + off) + step, desc_kmajor(aK + off) + step, idesc_s<false>(), kk > 0);
+                        }
                     }
                     commit(&tail->s_full[l]);
                 };
@@ -598,21 +737,26 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
                     ++p_cnt[l];
                     fence_after();
                     const uint32_t aV = smem_u32(smem + L::kStageOff + stage * kTileBytes);
+                    const uint32_t tO = tmem + kTmemO + l * 128u;
+                    if (thin) {
+                        const uint32_t aP = smem_u32(smem + kThinP + l * kThinPBytes);
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        mma_ta(tmem + kTmemO + l * 128u, tmem + l * 128u + 8u * kk, desc_mnmajor(aV + static_cast<uint32_t>(kk) * 2048u),
-                               idesc_pv<false>(), (acc || kk > 0) ? 1 : 0);
+                        for (int kk = 0; kk < 8; ++kk)
+                            mma(tO, desc_mnmajor(aV + static_cast<uint32_t>(kk) * 2048u), desc_thin_p(aP + kk * 32u * s.cols, s.cols),
+                                id_thin | kIdescTransposeAB, (acc || kk > 0) ? 1 : 0);
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            mma_ta(tO, tmem + l * 128u + 8u * kk, desc_mnmajor(aV + static_cast<uint32_t>(kk) * 2048u),
+                                   idesc_pv<false>(), (acc || kk > 0) ? 1 : 0);
+                    }
                     commit(&tail->pv_done[l]);
                     return true;
                 };
-                auto q_done = [&]() {   // the segment's last S is issued
-                    commit(&tail->q_empty[s.pair ? 0 : qb]);
-                    if (s.pair) commit(&tail->q_empty[1]);
-                };
                 // first tiles
                 if (!(ok = wait_item(0))) break;
-                if (s.pair) {
-                    if (n_l[0] > 0) issue_s(0, stage_of(0));
+                if (s.pair()) {
+                    if (n0 > 0) issue_s(0, stage_of(0));
                     issue_s(1, stage_of(0));
                     commit(&tail->empty[stage_of(0)]);
                 } else {
@@ -624,18 +768,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
                         commit(&tail->empty[stage_of(1)]);
                     }
                 }
-                if (n == (s.pair ? 1 : (n > 1 ? 2 : 1))) q_done();
                 // the previous segment's O has been read
                 if (seg > 0 && !(ok = wait_bar(&tail->epi_done, (seg - 1) & 1u, failed))) break;
                 for (int i = 0; ok && i < n; ++i) {
                     const uint32_t vi = item_of_v(i, n);
                     if (!(ok = wait_item(vi))) break;
-                    if (s.pair) {
+                    if (s.pair()) {
                         const bool more = i + 1 < n;
                         const uint32_t ki = item_of_k(i + 1);
-                        if (i < n_l[0]) {
+                        if (i < n0) {
                             if (!(ok = issue_pv(0, stage_of(vi), i > 0))) break;
-                            if (i + 1 < n_l[0]) {
+                            if (i + 1 < n0) {
                                 if (!(ok = wait_item(ki))) break;
                                 issue_s(0, stage_of(ki));
                             }
@@ -646,7 +789,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
                             if (!(ok = wait_item(ki))) break;
                             issue_s(1, stage_of(ki));
                             commit(&tail->empty[stage_of(ki)]);
-                            if (i + 2 == n) q_done();
                         }
                     } else {
                         if (!(ok = issue_pv(i & 1, stage_of(vi), i > 1))) break;
@@ -656,10 +798,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
                             if (!(ok = wait_item(ki))) break;
                             issue_s(i & 1, stage_of(ki));
                             commit(&tail->empty[stage_of(ki)]);
-                            if (i + 3 == n) q_done();
                         }
                     }
                 }
+                if (!ok) break;
+                commit(&tail->seg_done[seg & 1u]);
                 u0 += 2 * n;
                 ++seg;
             }
@@ -673,232 +816,404 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
         }
         __syncwarp();
     } else {
-        // ================= softmax and epilogue: lane l, thread = row =================
-        const int l = (warp - 4) >> 2, quad = warp & 3, r = 32 * quad + lane, h = r & 1;
+        // ================= softmax and epilogue of lane l =================
+        const int l = (warp - 4) >> 2, quad = warp & 3, r = 32 * quad + lane;   // r: TMEM lane
         const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * quad) << 16);
         const uint32_t tS = lane_addr + l * 128u, tO = lane_addr + kTmemO + l * 128u;
-        uint32_t cnt = 0, xcnt = 0, tile_no = 0;
-        bool go = true;
-        while (walk.next(p, s)) {
-            const int n = s.t1 - s.t0, mine = lane_tiles(s, l);
-            const int qoff = s.pair ? kQueries * l : 0;
-            const int nq = min(kQueries, s.nq - qoff);
-            const bool active = 32 * quad < 2 * nq;   // the warp holds a row of a query
-            const int i = min(r >> 1, max(nq - 1, 0));
-            const int pos_min = s.q0pos + qoff, pos = pos_min + i;
-            unsigned long long bits = 0;
-            if (p.mask && active) {
-                bits = p.mask[s.row0 + qoff + i];
-                if (s.nq < 64) bits &= (1ull << s.nq) - 1ull;
-            }
-            float m_ref = -INFINITY, l_run = 0.0f;
-            for (int k = 0; k < mine; ++k) {
-                const int ti = s.pair ? k : 2 * k + l, kt = s.t0 + ti;
-                go = wait_bar(&tail->s_full[l], cnt & 1u, failed);
-                if (!__all_sync(0xffffffffu, go)) break;
-                fence_after();
-                if (active) {
-                    const uint32_t slot = (tile_no + ti) % L::kScaleRing;
-                    const float *ks = scale_ring + slot * 2 * kKeys, *vs = ks + kKeys;
+        uint32_t cnt = 0, tile_no = 0;
+        auto wait = [&](uint64_t *bar, uint32_t par) {
+            if (wait_bar(bar, par, failed)) return;
+            if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 22);
+            *failed = 1;
+        };
+
+        // Key tile kt (the ti-th of the segment) of pair and alternate mode; thread = query row.
+        auto row_tile = [&](auto masked_t, int kt, int ti, int pos, unsigned long long bits, bool start, float &m_ref,
+                            float &l_run) {
+            constexpr bool kMasked = decltype(masked_t)::value;
+            const uint32_t slot = (tile_no + ti) % L::kScaleRing;
+            const float *ks = scale_ring + slot * 2 * kKeys, *vs = ks + kKeys;
+            if constexpr (k8) wait(&tail->scale_full[slot], ((tile_no + ti) / L::kScaleRing) & 1u);
+            // keys of chunk c (32 keys) that the row sees
+            auto seen = [&](int c) -> uint32_t {
+                const int k0 = kt * kKeys + 32 * c;
+                if (!p.mask) {
+                    const int d = pos - k0;
+                    return d >= 31 ? 0xffffffffu : (d < 0 ? 0u : (2u << d) - 1u);
+                }
+                const int d = k0 - s.base;   // chunk token of the first key
+                if (d <= -32) return 0xffffffffu;
+                if (d < 0) return ((1u << -d) - 1u) | static_cast<uint32_t>(bits << -d);
+                return d < 64 ? static_cast<uint32_t>(bits >> d) : 0u;
+            };
+            // pass 1: the row's largest score
+            float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            uint32_t sr[2][32];
+            tmem_ld32_issue(tS, sr[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                tmem_wait_ld32(sr[c & 1]);
+                tmem_ld32_issue(tS + 32u * ((c + 1) & 3), sr[(c + 1) & 1]);   // after chunk 3: chunk 0 for pass 2
+                const uint32_t w = kMasked ? seen(c) : 0u;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    float v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) v[q] = __uint_as_float(sr[c & 1][j + q]);
                     if constexpr (k8) {
-                        go = wait_bar(&tail->scale_full[slot], ((tile_no + ti) / L::kScaleRing) & 1u, failed);
-                        if (!__all_sync(0xffffffffu, go)) break;
+                        const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                        un_f2(mul_f2(f2(v[0], v[1]), f2(f.x, f.y)), v[0], v[1]);
+                        un_f2(mul_f2(f2(v[2], v[3]), f2(f.z, f.w)), v[2], v[3]);
                     }
-                    // keys a row sees, 32 at a time; a tile that every row sees whole needs none of it
-                    const bool masked = kt * kKeys + kKeys - 1 > (p.mask ? s.base - 1 : pos_min);
-                    auto seen = [&](int c) -> uint32_t {
-                        if (!masked) return 0xffffffffu;
-                        const int k0 = kt * kKeys + 32 * c;
-                        if (!p.mask) {
-                            const int d = pos - k0;
-                            return d >= 31 ? 0xffffffffu : (d < 0 ? 0u : (2u << d) - 1u);
-                        }
-                        const int d = k0 - s.base;   // chunk token of the first key
-                        if (d <= -32) return 0xffffffffu;
-                        if (d < 0) return ((1u << -d) - 1u) | static_cast<uint32_t>(bits << -d);
-                        return d < 64 ? static_cast<uint32_t>(bits >> d) : 0u;
-                    };
-                    // pass 1: the row's largest score
-                    float top = -INFINITY;
-                    uint32_t sr[2][32];
-                    tmem_ld32_issue(tS, sr[0]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_wait_ld32(sr[c & 1]);
-                        if (c < 3) tmem_ld32_issue(tS + 32u * (c + 1), sr[(c + 1) & 1]);
-                        const uint32_t w = seen(c);
-                        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
-                            if constexpr (k8) f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
-                            const float fs[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                float v = __uint_as_float(sr[c & 1][j + q]);
-                                if constexpr (k8) v *= fs[q];
-                                if (masked) v = (w >> (j + q)) & 1u ? v : -INFINITY;
-                                t4[q] = fmaxf(t4[q], v);
-                            }
-                        }
-                        top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+                    for (int q = 0; q < 4; ++q) {
+                        if (kMasked && !((w >> (j + q)) & 1u)) v[q] = -INFINITY;
                     }
-                    if constexpr (!k8) top *= p.scale_log2;
-                    // the first chunk again, under the decision about the reference
-                    tmem_ld32_issue(tS, sr[0]);
-                    float alpha = 1.0f;
-                    bool rescale = false;
-                    if (k == 0) {
-                        m_ref = top;
-                    } else if (top > m_ref + kRescaleLog2) {
-                        alpha = ex2_approx(m_ref - top);   // 0 where nothing was seen so far
-                        m_ref = top;
-                        l_run *= alpha;
-                        rescale = true;
-                    }
-                    // P V of the lane's previous tile has completed: O is at rest
-                    if (k > 0) go = wait_bar(&tail->pv_done[l], (cnt - 1u) & 1u, failed);
-                    if (!__all_sync(0xffffffffu, go)) break;
-                    if (__any_sync(0xffffffffu, rescale)) {
-                        tmem_wait_ld32(sr[0]);
-                        fence_after();
+                    t4[0] = fmaxf(t4[0], fmaxf(v[0], v[1]));
+                    t4[1] = fmaxf(t4[1], fmaxf(v[2], v[3]));
+                }
+            }
+            float top = fmaxf(t4[0], t4[1]);
+            if constexpr (!k8) top *= p.scale_log2;
+            float alpha = 1.0f;
+            bool rescale = false;
+            if (start) {
+                m_ref = top;
+            } else if (top > m_ref + kRescaleLog2) {
+                alpha = ex2_approx(m_ref - top);   // 0 where nothing was seen so far
+                m_ref = top;
+                l_run *= alpha;
+                rescale = true;
+            }
+            // P V of the lane's previous tile has completed: O is at rest
+            if (!start) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
+            if (__any_sync(0xffffffffu, rescale)) {
+                tmem_wait_ld32(sr[0]);
+                fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < 4; ++c) {
-                            float o[32];
-                            tmem_ld32(tO + 32u * c, o);
+                for (int c = 0; c < 4; ++c) {
+                    float o[32];
+                    tmem_ld32(tO + 32u * c, o);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] *= alpha;
-                            tmem_st32(tO + 32u * c, o);
+                    for (int j = 0; j < 32; ++j) o[j] *= alpha;
+                    tmem_st32(tO + 32u * c, o);
+                }
+                tmem_wait_st();
+                tmem_ld32_issue(tS, sr[0]);
+            }
+            // pass 2: P into S's first 64 columns; chunk c's 16 columns lie in chunks already read
+            const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
+            const uint64_t nsub2 = f2(-sub, -sub), c2 = f2(p.scale_log2, p.scale_log2);
+            uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                tmem_wait_ld32(sr[c & 1]);
+                if (c < 3) tmem_ld32_issue(tS + 32u * (c + 1), sr[(c + 1) & 1]);
+                const uint32_t w = kMasked ? seen(c) : 0u;
+                uint32_t pk[16];
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    uint64_t fa = c2, fb = c2;
+                    if constexpr (k8) {
+                        const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                        fa = f2(f.x, f.y);
+                        fb = f2(f.z, f.w);
+                    }
+                    float e[4];
+                    un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j]), __uint_as_float(sr[c & 1][j + 1])), fa, nsub2), e[0], e[1]);
+                    un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j + 2]), __uint_as_float(sr[c & 1][j + 3])), fb, nsub2), e[2], e[3]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (kMasked && !((w >> (j + q)) & 1u)) e[q] = -INFINITY;
+                        e[q] = ex2_approx(e[q]);
+                    }
+                    acc[0] = add_f2(acc[0], f2(e[0], e[1]));
+                    acc[1] = add_f2(acc[1], f2(e[2], e[3]));
+                    if constexpr (k8) {
+                        const float4 f = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
+                        un_f2(mul_f2(f2(e[0], e[1]), f2(f.x, f.y)), e[0], e[1]);
+                        un_f2(mul_f2(f2(e[2], e[3]), f2(f.z, f.w)), e[2], e[3]);
+                    }
+                    pk[j / 2] = pack_bf16x2(e[0], e[1]);
+                    pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                }
+                tmem_st16(tS + 16u * c, pk);
+            }
+            float s0, s1, s2, s3;
+            un_f2(acc[0], s0, s1);
+            un_f2(acc[1], s2, s3);
+            l_run += (s0 + s1) + (s2 + s3);
+            tmem_wait_st();
+        };
+
+        // A segment of thin mode: thread = key of a tile, then = output dim.  Columns n < 2 nq are row 2 i + h.
+        auto thin_segment = [&](auto cols_t) {
+            constexpr int kCols = decltype(cols_t)::value;
+            const int n = s.t1 - s.t0, mine = lane_tiles(s, l);
+            uint8_t *const sP = smem + kThinP + l * kThinPBytes;
+            float *const ref = tail->thin_ref[l];
+            float lsum[kCols];
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) lsum[j] = 0.0f;
+            for (int k = 0; k < mine; ++k) {
+                const int ti = 2 * k + l, kt = s.t0 + ti, key = kt * kKeys + r;
+                float kscale = p.scale_log2, vscale = 1.0f;
+                if constexpr (k8) {
+                    const uint32_t slot = (tile_no + ti) % L::kScaleRing;
+                    wait(&tail->scale_full[slot], ((tile_no + ti) / L::kScaleRing) & 1u);
+                    kscale = scale_ring[slot * 2 * kKeys + r];
+                    vscale = scale_ring[slot * 2 * kKeys + kKeys + r];
+                }
+                wait(&tail->s_full[l], cnt & 1u);
+                fence_after();
+                uint32_t sr[kCols];
+                tmem_ld_cols<kCols>(tS, sr);
+                tmem_wait_ld_regs<kCols>(sr);
+                float x[kCols];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) x[j] = __uint_as_float(sr[j]) * kscale;
+                if (kt * kKeys + kKeys > s.q0pos) {     // the tile reaches the unit's queries
+                    const int d = key - s.q0pos;        // this key among them (with a mask: among the chunk's tokens)
+                    if (!p.mask) {
+#pragma unroll
+                        for (int j = 0; j < kCols; ++j) x[j] = (j >> 1) >= d ? x[j] : -INFINITY;
+                    } else if (d >= 0) {
+#pragma unroll
+                        for (int j = 0; j < kCols; ++j) {
+                            const bool see = j < 2 * s.nq && d < s.nq && ((__ldg(p.mask + s.row0 + (j >> 1)) >> d) & 1ull);
+                            x[j] = see ? x[j] : -INFINITY;
+                        }
+                    }
+                }
+                // P V of the lane's previous tile has completed: its P may go, O is at rest
+                if (k > 0) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
+                bool move = k == 0;
+                if (k > 0) {
+                    float over = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) over = fmaxf(over, x[j] - ref[j]);   // -inf - -inf: NaN, not the maximum
+                    move = bar_any(kBarLane + l, 128, over > kRescaleLog2);
+                }
+                if (move) {
+                    // New references: each column's maximum over the tile's keys, by warp, then over the four warps
+                    // (scratch in the P tile).
+                    float *const wmax = reinterpret_cast<float *>(sP);
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) {
+                        const float m = warp_max(x[j]);
+                        if (lane == 0) wmax[quad * kCols + j] = m;
+                    }
+                    bar_sync(kBarLane + l, 128);
+                    float alpha[kCols];
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) {
+                        const float m = fmaxf(fmaxf(wmax[j], wmax[kCols + j]), fmaxf(wmax[2 * kCols + j], wmax[3 * kCols + j]));
+                        const float old = k > 0 ? ref[j] : -INFINITY;
+                        alpha[j] = m > old ? ex2_approx(old - m) : 1.0f;
+                        lsum[j] *= alpha[j];
+                    }
+                    bar_sync(kBarLane + l, 128);        // everyone has read the old references
+                    if (r < kCols) {
+                        const float m = fmaxf(fmaxf(wmax[r], wmax[kCols + r]), fmaxf(wmax[2 * kCols + r], wmax[3 * kCols + r]));
+                        ref[r] = k > 0 ? fmaxf(ref[r], m) : m;
+                    }
+                    if (k > 0) {
+                        fence_after();
+                        uint32_t o[kCols];
+                        tmem_ld_cols<kCols>(tO, o);
+                        tmem_wait_ld_regs<kCols>(o);
+                        if constexpr (kCols == 32) {
+                            float f[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(o[j]) * alpha[j];
+                            tmem_st32(tO, f);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha[j]);
+                            tmem_st16(tO, o);
                         }
                         tmem_wait_st();
-                        tmem_ld32_issue(tS, sr[0]);
                     }
-                    // pass 2: P into S's first 64 columns; chunk c's 16 columns lie in chunks already read
-                    const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
-                    float acc[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_wait_ld32(sr[c & 1]);
-                        if (c < 3) tmem_ld32_issue(tS + 32u * (c + 1), sr[(c + 1) & 1]);
-                        const uint32_t w = seen(c);
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            float4 f = make_float4(1.f, 1.f, 1.f, 1.f), fv = f;
-                            if constexpr (k8) {
-                                f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
-                                fv = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
-                            }
-                            const float fs[4] = {f.x, f.y, f.z, f.w}, fvs[4] = {fv.x, fv.y, fv.z, fv.w};
-                            float e[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                float v = __uint_as_float(sr[c & 1][j + q]);
-                                v = fmaf(v, k8 ? fs[q] : p.scale_log2, -sub);
-                                if (masked) v = (w >> (j + q)) & 1u ? v : -INFINITY;
-                                e[q] = ex2_approx(v);
-                            }
-                            acc[0] += e[0] + e[1];
-                            acc[1] += e[2] + e[3];
-                            if constexpr (k8) {
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) e[q] *= fvs[q];
-                            }
-                            pk[j / 2] = pack_bf16x2(e[0], e[1]);
-                            pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
-                        }
-                        tmem_st16(tS + 16u * c, pk);
-                    }
-                    l_run += acc[0] + acc[1];
-                    tmem_wait_st();
-                } else if (k > 0) {
-                    go = wait_bar(&tail->pv_done[l], (cnt - 1u) & 1u, failed);
-                    if (!__all_sync(0xffffffffu, go)) break;
+                    bar_sync(kBarLane + l, 128);        // the references are written, the scratch is read
                 }
+                // P: this key's row of columns, swizzled in 16-byte chunks
+                uint32_t pk[kCols / 2];
+#pragma unroll
+                for (int j = 0; j < kCols; j += 4) {
+                    const float4 m = *reinterpret_cast<const float4 *>(ref + j);
+                    const float ms[4] = {m.x, m.y, m.z, m.w};
+                    float e[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        e[q] = ex2_approx(x[j + q] - (ms[q] == -INFINITY ? 0.0f : ms[q]));
+                        lsum[j + q] += e[q];
+                        if constexpr (k8) e[q] *= vscale;
+                    }
+                    pk[j / 2] = pack_bf16x2(e[0], e[1]);
+                    pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                }
+                const int turn = kCols == 16 ? (r >> 2) & 1 : (r >> 1) & 3;
+#pragma unroll
+                for (int c = 0; c < kCols / 8; ++c)
+                    *reinterpret_cast<uint4 *>(sP + r * (2 * kCols) + ((c ^ turn) << 4)) =
+                        make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+                fence_async_smem();
                 fence_before();
                 mbar_arrive(&tail->p_full[l]);
                 ++cnt;
             }
-            if (!__all_sync(0xffffffffu, go)) break;
-            // the lane's last P V
-            if (mine > 0) go = wait_bar(&tail->pv_done[l], (cnt - 1u) & 1u, failed);
-            if (!__all_sync(0xffffffffu, go)) break;
-            // Where this row goes: its dims [d0, d1) of the output row or of the piece's row.
-            const bool whole = s.first && s.last;
-            float a0 = 1.0f, a1 = 0.0f, m_tot = m_ref, l_tot = l_run;
-            if (!s.pair) {
-                // lane 1 has nothing to say for a single tile (and must not: lane 0 may still read its last entry)
-                if (mine > 0) tail->ml[l][r] = make_float2(m_ref, l_run);
-                fence_before();
-                mbar_arrive(&tail->x_ready);
-                go = wait_bar(&tail->x_ready, xcnt & 1u, failed);
-                ++xcnt;
-                if (!__all_sync(0xffffffffu, go)) break;
-                const float2 v0 = tail->ml[0][r], v1 = n > 1 ? tail->ml[1][r] : make_float2(-INFINITY, 0.0f);
-                m_tot = fmaxf(v0.x, v1.x);
-                a0 = v0.y > 0.0f ? ex2_approx(v0.x - m_tot) : 0.0f;
-                a1 = v1.y > 0.0f ? ex2_approx(v1.x - m_tot) : 0.0f;
-                l_tot = a0 * v0.y + a1 * v1.y;
+            if (mine > 0) {
+                wait(&tail->pv_done[l], (cnt - 1u) & 1u);
+                // Column sums over the lane's 128 threads.  (Not by way of the P tile: with the last P V done, the
+                // loaders may already put a later segment's Q there.)
+                float *const wsum = reinterpret_cast<float *>(&tail->ml[l][64]);
+                warp_column_sums<kCols>(lsum, lane);
+                if (lane % (32 / kCols) == 0) wsum[quad * kCols + lane / (32 / kCols)] = lsum[0];
+                bar_sync(kBarLane + l, 128);
+                if (r < kCols)
+                    tail->ml[l][r] = make_float2(ref[r], (wsum[r] + wsum[kCols + r]) + (wsum[2 * kCols + r] + wsum[3 * kCols + r]));
             }
+            fence_before();
+            bar_sync(kBarBoth, 256);
             fence_after();
-            const bool real = r < 2 * nq;
-            if (active) {
-                const float norm = whole ? (l_tot > 0.0f ? 1.0f / l_tot : 0.0f) : 1.0f;
-                a0 *= norm;
-                a1 *= norm;
-                const int c0 = s.pair ? 0 : 2 * l, c1 = s.pair ? 4 : c0 + 2;   // 32-column chunks
-                const uint32_t o0 = s.pair ? tO : lane_addr + kTmemO, o1 = lane_addr + kTmemO + 128u;
-                const bool own0 = s.pair ? mine > 0 : true, two = !s.pair && n > 1;
-                uint16_t *const out = p.out + static_cast<size_t>(s.row0 + qoff + i) * kQDim + (2 * s.g + h) * kHeadDim;
-                const size_t piece = 2 * static_cast<size_t>(blockIdx.x) + (s.first ? 1 : 0);
-                const int prow = (s.pair ? 128 * l : 0) + r;
-                float *const part = p.part_o + piece * (kPieceRows * kHeadDim) + prow * 4;
-#pragma unroll 1
-                for (int c = c0; c < c1; ++c) {
-                    float o[32];
-                    if (own0) {
-                        tmem_ld32(o0 + 32u * c, o);
+            // dims as threads: lane l finishes columns [l kCols / 2, (l + 1) kCols / 2)
+            const bool whole = s.first && s.last;
+            constexpr int kHalf = kCols / 2;
+            uint32_t o0[kHalf], o1[kHalf];
+            tmem_ld_cols<kHalf>(lane_addr + kTmemO + l * kHalf, o0);
+            tmem_wait_ld_regs<kHalf>(o0);
+            if (n > 1) {
+                tmem_ld_cols<kHalf>(lane_addr + kTmemO + 128u + l * kHalf, o1);
+                tmem_wait_ld_regs<kHalf>(o1);
+            }
+            const size_t piece = 2 * static_cast<size_t>(blockIdx.x) + (s.first ? 1 : 0);
+            const int real = *failed ? 0 : 2 * s.nq;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = a0 == 0.0f ? 0.0f : o[j] * a0;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = 0.0f;
-                    }
-                    if (two) {
-                        float o2[32];
-                        tmem_ld32(o1 + 32u * c, o2);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] += a1 == 0.0f ? 0.0f : o2[j] * a1;
-                    }
-                    if (!real) continue;
-                    if (whole) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 8)
-                            *reinterpret_cast<uint4 *>(out + 32 * c + j) =
-                                make_uint4(pack_bf16x2(o[j], o[j + 1]), pack_bf16x2(o[j + 2], o[j + 3]),
-                                           pack_bf16x2(o[j + 4], o[j + 5]), pack_bf16x2(o[j + 6], o[j + 7]));
-                    } else {
-                        // a piece keeps four dims of all its rows together: [dims / 4][row][4]
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            *reinterpret_cast<float4 *>(part + static_cast<size_t>(8 * c + j / 4) * (kPieceRows * 4)) =
-                                make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                    }
+            for (int j = 0; j < kHalf; ++j) {
+                const int col = l * kHalf + j;
+                if (col >= real) continue;
+                const float2 v0 = tail->ml[0][col], v1 = n > 1 ? tail->ml[1][col] : make_float2(-INFINITY, 0.0f);
+                const float m = fmaxf(v0.x, v1.x);
+                const float a0 = v0.y > 0.0f ? ex2_approx(v0.x - m) : 0.0f, a1 = v1.y > 0.0f ? ex2_approx(v1.x - m) : 0.0f;
+                const float sum = a0 * v0.y + a1 * v1.y;
+                float o = a0 > 0.0f ? a0 * __uint_as_float(o0[j]) : 0.0f;
+                if (a1 > 0.0f) o += a1 * __uint_as_float(o1[j]);
+                if (whole) {
+                    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                    reinterpret_cast<__nv_bfloat16 *>(p.out)[static_cast<size_t>(s.row0 + (col >> 1)) * kQDim +
+                                                             (2 * s.g + (col & 1)) * kHeadDim + r] = __float2bfloat16_rn(o * inv);
+                } else {
+                    p.part_o[piece * (kPieceRows * kHeadDim) + col * kHeadDim + r] = o;
+                    if (r == 0) p.part_ml[piece * kPieceRows + col] = make_float2(m, sum);
                 }
-                if (!whole && real && (s.pair || l == 0))
-                    p.part_ml[piece * kPieceRows + prow] = make_float2(m_tot, l_tot);
+            }
+        };
+
+        while (walk.next(p, s)) {
+            const int n = s.t1 - s.t0;
+            if (s.mode == kThin) {
+                if (s.cols == 16) thin_segment(std::integral_constant<int, 16>{});
+                else thin_segment(std::integral_constant<int, 32>{});
+            } else {
+                const int mine = lane_tiles(s, l), h = r & 1;
+                const int qoff = s.pair() ? kQueries * l : 0;
+                const int nq = min(kQueries, s.nq - qoff);
+                const bool active = 32 * quad < 2 * nq;   // the warp holds a row of a query
+                const int i = min(r >> 1, max(nq - 1, 0));
+                const int pos_min = s.q0pos + qoff, pos = pos_min + i;
+                unsigned long long bits = 0;
+                if (p.mask && active) {
+                    bits = p.mask[s.row0 + qoff + i];
+                    if (s.nq < 64) bits &= (1ull << s.nq) - 1ull;
+                }
+                float m_ref = -INFINITY, l_run = 0.0f;
+                for (int k = 0; k < mine; ++k) {
+                    const int ti = s.pair() ? k : 2 * k + l, kt = s.t0 + ti;
+                    wait(&tail->s_full[l], cnt & 1u);
+                    fence_after();
+                    if (!active) {
+                        if (k > 0) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
+                    } else if (kt * kKeys + kKeys - 1 > (p.mask ? s.base - 1 : pos_min)) {
+                        row_tile(std::true_type{}, kt, ti, pos, bits, k == 0, m_ref, l_run);
+                    } else {
+                        row_tile(std::false_type{}, kt, ti, pos, bits, k == 0, m_ref, l_run);
+                    }
+                    fence_before();
+                    mbar_arrive(&tail->p_full[l]);
+                    ++cnt;
+                }
+                if (mine > 0) wait(&tail->pv_done[l], (cnt - 1u) & 1u);   // the lane's last P V
+                const bool whole = s.first && s.last;
+                float a0 = 1.0f, a1 = 0.0f, m_tot = m_ref, l_tot = l_run;
+                if (!s.pair()) {
+                    // Lane 1 says nothing for a single tile (and must not: lane 0 may still read its last entry).
+                    if (mine > 0) tail->ml[l][r] = make_float2(m_ref, l_run);
+                    fence_before();
+                    bar_sync(kBarBoth, 256);
+                    const float2 v0 = tail->ml[0][r], v1 = n > 1 ? tail->ml[1][r] : make_float2(-INFINITY, 0.0f);
+                    m_tot = fmaxf(v0.x, v1.x);
+                    a0 = v0.y > 0.0f ? ex2_approx(v0.x - m_tot) : 0.0f;
+                    a1 = v1.y > 0.0f ? ex2_approx(v1.x - m_tot) : 0.0f;
+                    l_tot = a0 * v0.y + a1 * v1.y;
+                }
+                fence_after();
+                const bool real = r < 2 * nq && !*failed;
+                if (active) {
+                    const float norm = whole ? (l_tot > 0.0f ? 1.0f / l_tot : 0.0f) : 1.0f;
+                    a0 *= norm;
+                    a1 *= norm;
+                    const int c0 = s.pair() ? 0 : 2 * l, c1 = s.pair() ? 4 : c0 + 2;   // 32-column chunks
+                    const uint32_t o0 = s.pair() ? tO : lane_addr + kTmemO, o1 = lane_addr + kTmemO + 128u;
+                    const bool own0 = s.pair() ? mine > 0 : true, two = !s.pair() && n > 1;
+                    uint16_t *const out = p.out + static_cast<size_t>(s.row0 + qoff + i) * kQDim + (2 * s.g + h) * kHeadDim;
+                    const size_t piece = 2 * static_cast<size_t>(blockIdx.x) + (s.first ? 1 : 0);
+                    const int prow = (s.pair() ? 128 * l : 0) + r;
+                    float *const part = p.part_o + piece * (kPieceRows * kHeadDim) + prow * 4;
+#pragma unroll 1
+                    for (int c = c0; c < c1; ++c) {
+                        float o[32];
+                        if (own0) {
+                            tmem_ld32(o0 + 32u * c, o);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = a0 == 0.0f ? 0.0f : o[j] * a0;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = 0.0f;
+                        }
+                        if (two) {
+                            float o2[32];
+                            tmem_ld32(o1 + 32u * c, o2);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] += a1 == 0.0f ? 0.0f : o2[j] * a1;
+                        }
+                        if (!real) continue;
+                        if (whole) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 8)
+                                *reinterpret_cast<uint4 *>(out + 32 * c + j) =
+                                    make_uint4(pack_bf16x2(o[j], o[j + 1]), pack_bf16x2(o[j + 2], o[j + 3]),
+                                               pack_bf16x2(o[j + 4], o[j + 5]), pack_bf16x2(o[j + 6], o[j + 7]));
+                        } else {
+                            // a piece keeps four dims of all its rows together: [dims / 4][row][4]
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4)
+                                *reinterpret_cast<float4 *>(part + static_cast<size_t>(8 * c + j / 4) * (kPieceRows * 4)) =
+                                    make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        }
+                    }
+                    if (!whole && real && (s.pair() || l == 0))
+                        p.part_ml[piece * kPieceRows + prow] = make_float2(m_tot, l_tot);
+                }
             }
             fence_before();
             mbar_arrive(&tail->epi_done);
             if (s.first && !s.last && warp == 4 && lane == 0) {
                 // the unit goes on in the CTAs up to the one that holds its last tile
-                const long long last = s.ustart + static_cast<long long>(s.pair ? 2 : 1) * (s.tiles - 1);
-                p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.pair ? 1 : 0,
-                                                  static_cast<int>(((last + 1) * parts - 1) / total)};
+                const long long last = s.ustart + static_cast<long long>(s.pair() ? 2 : 1) * (s.tiles - 1);
+                p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.mode, static_cast<int>(((last + 1) * parts - 1) / total)};
             }
             tile_no += n;
         }
-        if (!go) *failed = 1;
     }
     fence_before();
     __syncthreads();
@@ -910,7 +1225,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
 
 // Joins the pieces of the unit that starts in CTA blockIdx.x and goes on
 // elsewhere: o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, pieces in order.
-// Thread = (row, four dims); rows run fastest, as in the pieces.
+// Thread = (row, four dims), in the order the pieces lie in memory: thin mode's
+// row by row, the others' four dims of all rows together.
 constexpr int kJoinThreads = 256;
 
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkAttendParams p) {
@@ -921,7 +1237,9 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_c
     if (d.c_last <= c0) return;
     const int rows = 2 * d.nq;   // pair: lane 0's 128 rows, then lane 1's
     for (int w = blockIdx.y * kJoinThreads + threadIdx.x; w < rows * (kHeadDim / 4); w += gridDim.y * kJoinThreads) {
-        const int r = w % rows, c = w / rows;
+        const bool thin = d.mode == kThin;
+        const int r = thin ? w / (kHeadDim / 4) : w % rows, c = thin ? w % (kHeadDim / 4) : w / rows;
+        const size_t off = thin ? static_cast<size_t>(w) * 4 : static_cast<size_t>(c) * (kPieceRows * 4) + r * 4;
         float m = -INFINITY;
         for (int k = c0; k <= d.c_last; ++k) m = fmaxf(m, p.part_ml[(2 * k + (k == c0 ? 1 : 0)) * kPieceRows + r].x);
         float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -930,8 +1248,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_c
             const float2 ml = p.part_ml[piece * kPieceRows + r];
             if (!(ml.y > 0.0f)) continue;
             const float a = exp2f(ml.x - m);
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + piece * (kPieceRows * kHeadDim) +
-                                                               static_cast<size_t>(c) * (kPieceRows * 4) + r * 4);
+            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + piece * (kPieceRows * kHeadDim) + off);
             l += a * ml.y;
             o[0] += a * v.x;
             o[1] += a * v.y;

@@ -140,7 +140,7 @@ struct ChunkAppendParams {
 // A unit of the chunk attention that starts in one CTA and ends in CTA c_last
 // (-1: none): its query rows, kv head and mode.
 struct ChunkSplit {
-    int row0, nq, g, pair, c_last;
+    int row0, nq, g, mode, c_last;
 };
 
 // Chunk attention: stream i of n has queries starts[i] .. starts[i + 1] - 1 of
