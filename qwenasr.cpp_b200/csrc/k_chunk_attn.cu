@@ -37,10 +37,16 @@
 // the unrounded values.  8-bit caches: the codes are exact in bf16; a key's
 // scale multiplies its scores, a value's scale its P.
 //
-// Roles: warps 0..3 loaders (cp.async into the swizzled tiles; 8-bit codes are
-// converted on the way), warps 4..7 lane 0, warps 8..11 lane 1, warp 12 MMA.
+// Roles: warps 0..3 lane 0, 4..7 lane 1, one MMA warp, one load warp (TMA: a
+// page's 16 keys of a head are a box), and for 8-bit caches four warps that
+// convert the raw tiles.  Staging the tiles by cp.async from four warps took
+// 2700 cycles per 32 KB and bounded every shape; the MMA warp runs its loop as
+// a whole and elects a thread only to issue, so that descriptors stay in
+// uniform registers.
 // All waits bounded; a softmax warp whose wait ran out goes on without waiting,
 // so that the named barriers stay matched.
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "kernels.h"
@@ -53,8 +59,6 @@ namespace {
 
 constexpr int kKeys = 128;                 // keys of a tile
 constexpr int kQueries = 64;               // queries of a query tile
-constexpr int kMmaWarp = 12;
-constexpr int kThreads = 13 * 32;
 constexpr uint32_t kTmemCols = 512;        // S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512)
 constexpr uint32_t kTmemO = 256;
 constexpr float kRescaleLog2 = 30.0f;
@@ -72,23 +76,27 @@ constexpr int kPieceRows = 256;            // rows of a workspace piece (pair mo
 template <bool k8> struct Layout {
     static constexpr int kStages = k8 ? 3 : 5;
     static constexpr int kRaw = k8 ? 3 : 0;
-    static constexpr int kLag = 3;         // bf16: tiles issued ahead of the one signalled (< kStages)
     static constexpr int kScaleRing = 4;
+    static constexpr int kConvWarp = 8;    // four of them (8-bit)
+    static constexpr int kMmaWarp = k8 ? 12 : 8;
+    static constexpr int kLoadWarp = kMmaWarp + 1;
+    static constexpr int kWarps = kLoadWarp + 1, kThreads = 32 * kWarps;
     static constexpr size_t kStageOff = 2 * static_cast<size_t>(kTileBytes);
     static constexpr size_t kRawOff = kStageOff + kStages * static_cast<size_t>(kTileBytes);
     static constexpr size_t kScaleOff = kRawOff + kRaw * static_cast<size_t>(kTileBytes / 2);
     static constexpr size_t kRawScaleOff = kScaleOff + (k8 ? kScaleRing * 2 * kKeys * sizeof(float) : 0);
     static constexpr size_t kTailOff = kRawScaleOff + kRaw * 2 * kKeys * sizeof(float);
 };
+constexpr int kMaxWarps = 14;
 
 struct alignas(16) Tail {
     uint64_t q_full[2], seg_done[2];       // of a segment, by its parity
     uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], epi_done, mma_done;
-    uint64_t scale_full[4];                // 8-bit: the scales of a tile are in the ring
+    uint64_t scale_full[4], raw_full[3], raw_empty[3];   // 8-bit
     float2 ml[2][128];                     // (reference, sum) of each lane's rows, at a segment's end
     float thin_ref[2][32];                 // thin mode: the lane's reference per column
-    long long warp_sum[kThreads / 32];
-    int warp_max[kThreads / 32];
+    long long warp_sum[kMaxWarps];
+    int warp_max[kMaxWarps];
     long long pre0;                        // work before entry i0, where this CTA's part starts
     int i0, runmax0;
     uint32_t tmem;
@@ -252,14 +260,31 @@ __device__ __forceinline__ void u8x4_to_bf16(uint32_t w, uint32_t &lo, uint32_t 
     hi = bf16x2_sub((b & 0x007f007fu) | 0x43004300u, 0x43804380u ^ (b & 0x00800080u));
 }
 
-template <int N> __device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// One box of a tensor map -> shared memory, completing on `bar`; what lies
+// outside the map reads as zero.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async4(void *dst, const void *src, uint32_t src_bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(src_bytes)
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+// A load that stays where it is written, a tile ahead of its use.
+__device__ __forceinline__ int load_early(const int *p) {
+    int v;
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // Packed pairs of f32 (two lanes of one instruction).
 __device__ __forceinline__ uint64_t f2(float a, float b) {
@@ -365,9 +390,18 @@ __device__ __forceinline__ float warp_max(float x) {
 __device__ __forceinline__ uint32_t item_of_k(int i) { return i == 0 ? 0 : 2 * i - 1; }
 __device__ __forceinline__ uint32_t item_of_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
 
+// Tensor maps: the layer's pool as [page][K|V x head x token][dim] with boxes of
+// 16 tokens (bf16: x 64 dims, 128-byte swizzle; 8-bit: x 128 bytes), and q as
+// [row][head][dim] with boxes of 64 and 16 rows x 2 heads x 64 dims.
+struct Maps {
+    CUtensorMap kv, q, q_thin;
+};
+
 template <bool k8>
-__global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_constant__ ChunkAttendParams p) {
+__global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
+    chunk_attn_kernel(const __grid_constant__ ChunkAttendParams p, const __grid_constant__ Maps maps) {
     using L = Layout<k8>;
+    constexpr int kThreads = L::kThreads, kMmaWarp = L::kMmaWarp;
     extern __shared__ uint8_t smem_raw[];
     pdl_trigger();
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -385,19 +419,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
 
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&tail->q_full[b], 128);
+            mbar_init(&tail->q_full[b], 1);
             mbar_init(&tail->seg_done[b], 1);
             mbar_init(&tail->s_full[b], 1);
             mbar_init(&tail->p_full[b], 128);
             mbar_init(&tail->pv_done[b], 1);
         }
         for (int b = 0; b < L::kStages; ++b) {
-            mbar_init(&tail->full[b], 128);
+            mbar_init(&tail->full[b], k8 ? 128 : 1);
             mbar_init(&tail->empty[b], 1);
         }
         mbar_init(&tail->epi_done, 256);
         mbar_init(&tail->mma_done, 1);
         for (int b = 0; b < L::kScaleRing; ++b) mbar_init(&tail->scale_full[b], 128);
+        for (int b = 0; b < L::kRaw; ++b) {
+            mbar_init(&tail->raw_full[b], 1);
+            mbar_init(&tail->raw_empty[b], 128);
+        }
         tail->failed = 0;
         tail->i0 = -1;
         fence_mbar_init();
@@ -443,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
     if (lane == 31) tail->warp_sum[warp] = inc;
     __syncthreads();
     long long pre = inc - sum, total = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
+    for (int w = 0; w < L::kWarps; ++w) {
         if (w < warp) pre += tail->warp_sum[w];
         total += tail->warp_sum[w];
     }
@@ -470,354 +508,325 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
     Segment s;
     walk.start(p, tail, x0, x1);
 
-    if (warp < 4) {
-        // ================= loaders =================
-        const int t = tid;
-        uint32_t u = 0, seg = 0, areas = 0, tile_no = 0;
+    if (warp == L::kLoadWarp) {
+        // ================= loads =================
+        constexpr int kRing = k8 ? L::kRaw : L::kStages;
+        uint64_t *const ring_full = k8 ? tail->raw_full : tail->full, *const ring_empty = k8 ? tail->raw_empty : tail->empty;
+        uint32_t u = 0, seg = 0, areas = 0, q_issued = 0;
         bool ok = true, was_thin = false;
-        // bf16: barriers of the items issued and not yet signalled, oldest first.
-        // 8-bit: the items in the raw ring instead, as scale slot x 2 + K|V, and
-        // the barrier of a Q in flight with the copies committed behind it.
-        uint64_t *pend[L::kLag] = {};
-        uint32_t meta[3] = {0, 0, 0};
-        int waiting = 0, behind_q = 0;
-        uint64_t *q_bar = nullptr;
-        uint32_t u_conv = 0;
-        auto signal_all = [&]() {
-            cp_async_wait<0>();
-            fence_async_smem();
-            if (k8 && q_bar) mbar_arrive(q_bar);
-            q_bar = nullptr;
-#pragma unroll
-            for (int j = 0; j < L::kLag; ++j) {
-                if (pend[j]) mbar_arrive(pend[j]);
-                pend[j] = nullptr;
-            }
-        };
-        auto wait_empty = [&](uint64_t *bar, uint32_t par) -> bool {
-            if (mbar_try_wait(bar, par)) return true;
-            if constexpr (!k8) signal_all();   // what was issued must not wait with us
-            if (wait_bar(bar, par, failed)) return true;
-            if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, static_cast<int>(u));
+        auto wait = [&](uint64_t *bar, uint32_t par) -> bool {
+            const bool done = wait_bar(bar, par, failed);
+            if (__all_sync(0xffffffffu, done)) return true;
+            if (lane == 0 && !*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, static_cast<int>(u));
             *failed = 1;
             return false;
         };
-        auto issued = [&](uint64_t *bar) {     // bf16: bar is signalled once its copies have landed
-            cp_async_commit();
-            cp_async_wait<L::kLag>();
-            if (pend[0]) {
-                fence_async_smem();
-                mbar_arrive(pend[0]);
-            }
-#pragma unroll
-            for (int j = 0; j + 1 < L::kLag; ++j) pend[j] = pend[j + 1];
-            pend[L::kLag - 1] = bar;
-        };
-        // 8-bit: convert the oldest raw tile into its stage.
-        auto convert = [&]() -> bool {
-            const uint32_t stage = u_conv % L::kStages, slot = u_conv % (L::kRaw ? L::kRaw : 1);
-            if (!wait_empty(&tail->empty[stage], ((u_conv / L::kStages) & 1u) ^ 1u)) return false;
-            uint8_t *dst = smem + L::kStageOff + stage * kTileBytes;
-            const uint8_t *raw = smem + L::kRawOff + slot * (kTileBytes / 2);
-            const uint32_t mt = meta[0];
-            const bool i8 = (mt & 1u) && p.v_int8;
-            const int c = t & 7;
-#pragma unroll
-            for (int m = 0; m < 8; ++m) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(raw + (m * 128 + t) * 16);
-                uint32_t h[8];
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (i8) u8x4_to_bf16(ws[k], h[2 * k], h[2 * k + 1]);
-                    else e4m3x4_to_bf16(ws[k], h[2 * k], h[2 * k + 1]);
-                }
-                const int r = (t >> 3) + 16 * m;
-                uint8_t *blk = dst + (c >> 2) * kBlkBytes;
-                const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-                // lanes of the second block start with their odd chunk: no two of 8 lanes meet in a bank
-                const bool odd = c & 4;
-                *reinterpret_cast<uint4 *>(blk + swz(r, 2 * (c & 3) + (odd ? 1 : 0))) = odd ? b : a;
-                *reinterpret_cast<uint4 *>(blk + swz(r, 2 * (c & 3) + (odd ? 0 : 1))) = odd ? a : b;
-            }
-            if (!(mt & 1u)) {   // a K tile brings both scales of its tokens
-                const float *rs = reinterpret_cast<const float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys;
-                scale_ring[(mt >> 1) * 2 * kKeys + t] = rs[t] * p.scale_log2;
-                scale_ring[(mt >> 1) * 2 * kKeys + kKeys + t] = rs[kKeys + t];
-                mbar_arrive(&tail->scale_full[mt >> 1]);
-            }
-            fence_async_smem();
-            mbar_arrive(&tail->full[stage]);
-            ++u_conv;
-            meta[0] = meta[1];
-            meta[1] = meta[2];
-            --waiting;
-            return true;
-        };
+        // This lane's page of a tile.  bf16: lanes 0..15, two boxes of 64 dims a page.  8-bit: lanes 0..7, a box a
+        // page, and lanes 8..23 the pages' scales of K and V.
+        const int ps = k8 ? (lane < 8 ? lane : ((lane - 8) >> 1) & 7) : (lane >> 1) & 7;
         while (ok && walk.next(p, s) && !*failed) {
-            const int *pt = p.page_table + static_cast<size_t>(s.slot) * p.maxp;
-            const int key_pages = (s.len_end + kPageTokens - 1) / kPageTokens;
+            const int *const pt = p.page_table + static_cast<size_t>(s.slot) * p.maxp;
+            const int key_pages = (s.len_end + kPageTokens - 1) / kPageTokens, n = s.t1 - s.t0;
+            auto page_id = [&](int kt) { return kt * 8 + ps < key_pages ? load_early(pt + kt * 8 + ps) : p.n_pages; };
+            // Outside the map's pages a box reads as zero: behind the last page, and for a bad id.
+            auto checked = [&](int id, int kt) {
+                if (static_cast<unsigned>(id) < static_cast<unsigned>(p.n_pages)) return id;
+                if (kt * 8 + ps < key_pages) report_error(p.err, kErrPageIndex, kWhereChunkAttn, s.row0, kt);
+                return p.n_pages;
+            };
+            int id_next = page_id(s.t0);
             // Q takes the areas of an earlier segment: the one before last has always ended (its Q barrier is
             // reused), the last one if they meet.
             const uint32_t prev = areas;
             areas = q_areas(s.mode, prev);
             const bool meets = (areas & prev) && !(s.mode == kThin && was_thin);
             was_thin = s.mode == kThin;
-            for (int back = 2; ok && back >= (meets ? 1 : 2); --back) {
-                if (seg < static_cast<uint32_t>(back)) continue;
-                uint64_t *bar = &tail->seg_done[(seg - back) & 1u];
-                const uint32_t par = ((seg - back) >> 1) & 1u;
-                if (k8 && !mbar_try_wait(bar, par)) {   // tiles of that segment may still lie unconverted here
-                    signal_all();
-                    while (ok && waiting > 0) ok = convert();
-                }
-                ok = ok && wait_empty(bar, par);
-            }
+            if (seg >= 2) ok = wait(&tail->seg_done[seg & 1u], ((seg - 2) >> 1) & 1u);
+            if (ok && meets && seg >= 1) ok = wait(&tail->seg_done[(seg - 1) & 1u], ((seg - 1) >> 1) & 1u);
             if (!ok) break;
-            // Q rows: row 2 i + h, 256 bytes each.  Rows past the queries: zero in thin mode, where they are
-            // columns beside real ones; elsewhere no one reads them.
-            for (int j = 0; j < (s.pair() ? 2 : 1); ++j) {
-                const bool thin = s.mode == kThin;
-                const int rows = 2 * min(kQueries, s.nq - j * kQueries), fill = thin ? s.cols : rows;
-                const uint32_t blk = thin ? kThinQBlk : kBlkBytes;
-                uint8_t *dst = smem + (thin ? kThinQ + (seg & 1u) * kThinQBytes
-                                            : (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes)) +
-                               ((t & 15) >> 3) * blk;
-                const uint16_t *src = p.q + static_cast<size_t>(s.row0 + j * kQueries) * kQDim + 2 * s.g * kHeadDim + 8 * (t & 15);
-#pragma unroll
-                for (int m = 0; m < 16; ++m) {
-                    const int row = (t >> 4) + 8 * m;
-                    if (row < fill)
-                        cp_async16(dst + swz(row, t & 7), src + (row < rows ? static_cast<size_t>(row >> 1) * kQDim + (row & 1) * kHeadDim : 0),
-                                   row < rows ? 16u : 0u);
-                }
-            }
-            if constexpr (k8) {
-                cp_async_commit();
-                q_bar = &tail->q_full[seg & 1u];
-                behind_q = 0;
-            } else {
-                issued(&tail->q_full[seg & 1u]);
-            }
-            const int n = s.t1 - s.t0;
-            // pages of the tile whose K / V comes next: V runs one tile behind K
-            int pg_k[8], pg_v[8];
-            auto pages = [&](int kt, int (&pg)[8]) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int pi = kt * 8 + k;
-                    pg[k] = __ldg(pt + (pi < key_pages ? pi : 0));
-                }
-            };
-            auto load = [&](int kt, int kv, const int (&pg)[8], uint32_t scale_slot) -> bool {
-                const int live_keys = s.len_end - kt * kKeys;   // of this tile; the rest reads as zero
-                bool bad = false;
-                if constexpr (!k8) {
-                    const uint32_t stage = u % L::kStages;
-                    if (!wait_empty(&tail->empty[stage], ((u / L::kStages) & 1u) ^ 1u)) return false;
-                    uint8_t *dst = smem + L::kStageOff + stage * kTileBytes + ((t & 15) >> 3) * kBlkBytes + swz(t >> 4, t & 7);
-                    const uint8_t *src = static_cast<const uint8_t *>(p.pool) + (kv * kHkv + s.g) * (kPageTokens * kHeadDim * 2) +
-                                         (t >> 4) * (kHeadDim * 2) + (t & 15) * 16;
-#pragma unroll
-                    for (int m = 0; m < 16; ++m) {
-                        const int page = pg[m >> 1], r = (t >> 4) + 8 * m;
-                        const bool in = page >= 0 && page < p.n_pages, live = r < live_keys;
-                        bad = bad || (live && !in);
-                        cp_async16(dst + m * 1024,
-                                   src + static_cast<size_t>(in ? page : 0) * (kPageHalfElems * 4) + (m & 1) * (8 * kHeadDim * 2),
-                                   live && in ? 16u : 0u);
-                    }
-                    issued(&tail->full[stage]);
+            // Q rows: row 2 i + h.  Rows behind the unit's queries are some other row's or zero: rows (in thin mode
+            // columns) of S that no one reads.
+            if (lane == 0) {
+                uint64_t *bar = &tail->q_full[seg & 1u];
+                if (s.mode == kThin) {
+                    const uint32_t dst = smem_u32(smem) + kThinQ + (seg & 1u) * kThinQBytes;
+                    mbar_arrive_expect_tx(bar, 2 * kThinQBlk);
+                    tma_load_3d(dst, &maps.q_thin, 0, 2 * s.g, s.row0, bar);
+                    tma_load_3d(dst + kThinQBlk, &maps.q_thin, 64, 2 * s.g, s.row0, bar);
                 } else {
-                    if (waiting == L::kRaw && !convert()) return false;
-                    const uint32_t slot = u % (L::kRaw ? L::kRaw : 1);
-                    uint8_t *raw = smem + L::kRawOff + slot * (kTileBytes / 2);
-                    const uint8_t *src = static_cast<const uint8_t *>(p.pool) + (kv * kHkv + s.g) * (kPageTokens * kHeadDim) +
-                                         (t >> 3) * kHeadDim + (t & 7) * 16;
+                    const int tiles = s.pair() ? 2 : 1;
+                    mbar_arrive_expect_tx(bar, tiles * kTileBytes);
+                    for (int j = 0; j < tiles; ++j) {
+                        const uint32_t dst = smem_u32(smem) + (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes);
+                        tma_load_3d(dst, &maps.q, 0, 2 * s.g, s.row0 + j * kQueries, bar);
+                        tma_load_3d(dst + kBlkBytes, &maps.q, 64, 2 * s.g, s.row0 + j * kQueries, bar);
+                    }
+                }
+            }
+            ++q_issued;
+            auto load = [&](int kt, int kv, int id) -> bool {
+                const uint32_t slot = u % kRing;
+                if (!wait(&ring_empty[slot], ((u / kRing) & 1u) ^ 1u)) return false;
+                uint64_t *const bar = &ring_full[slot];
+                if constexpr (!k8) {
+                    const uint32_t dst = smem_u32(smem) + L::kStageOff + slot * kTileBytes;
+                    // V rows behind the last token must be zero (their weight is zero, but not a NaN's product with
+                    // it): the page the stream ends in comes by plain loads.
+                    const int live = s.len_end - kt * kKeys, rows = live & (kPageTokens - 1), part = live >> 4;
+                    const bool mixed = kv == 1 && live < kKeys && rows != 0;
+                    if (mixed) {
+                        const int page = __shfl_sync(0xffffffffu, id, 2 * part);
+                        uint8_t *const to = smem + L::kStageOff + slot * kTileBytes;
+                        const uint8_t *const from = static_cast<const uint8_t *>(p.pool) +
+                                                    ((static_cast<size_t>(page < p.n_pages ? page : 0) * 2 + 1) * kHkv + s.g) *
+                                                        (kPageTokens * kHeadDim * 2);
 #pragma unroll
-                    for (int m = 0; m < 8; ++m) {
-                        const int page = pg[m], r = (t >> 3) + 16 * m;
-                        const bool in = page >= 0 && page < p.n_pages, live = r < live_keys;
-                        bad = bad || (live && !in);
-                        cp_async16(raw + (m * 128 + t) * 16, src + static_cast<size_t>(in ? page : 0) * (kPageHalfElems * 2),
-                                   live && in ? 16u : 0u);
-                    }
-                    if (kv == 0) {
-                        const int pi = kt * 8 + (t >> 4), page = __ldg(pt + (pi < key_pages ? pi : 0));
-                        const bool in = page >= 0 && page < p.n_pages;
-                        const float *sc = p.scales + (static_cast<size_t>(in ? page : 0) * 2 * kHkv + s.g) * kPageTokens + (t & 15);
-                        float *rs = reinterpret_cast<float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys + t;
-                        const uint32_t live = in && t < live_keys ? 4u : 0u;
-                        cp_async4(rs, sc, live);
-                        cp_async4(rs + kKeys, sc + kHkv * kPageTokens, live);
-                    }
-                    cp_async_commit();
-                    // the raw ring's tiles but the oldest may still be in flight when that one is converted
-                    const uint32_t mt = scale_slot * 2 + kv;
-                    if (waiting == 0) meta[0] = mt;
-                    else if (waiting == 1) meta[1] = mt;
-                    else meta[2] = mt;
-                    ++waiting;
-                    cp_async_wait<(L::kRaw > 0 ? L::kRaw - 1 : 0)>();
-                    if (q_bar && ++behind_q == L::kRaw - 1) {   // Q has landed
+                        for (int j = 0; j < 8; ++j) {
+                            const int row = (lane >> 4) + 2 * j, c = lane & 15;
+                            const uint4 v = row < rows && page < p.n_pages
+                                                ? *reinterpret_cast<const uint4 *>(from + row * (kHeadDim * 2) + c * 16)
+                                                : make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4 *>(to + (c >> 3) * kBlkBytes + swz(part * kPageTokens + row, c & 7)) = v;
+                        }
                         fence_async_smem();
-                        mbar_arrive(q_bar);
-                        q_bar = nullptr;
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(bar, kTileBytes - (mixed ? kTileBytes / 8 : 0));
+                    __syncwarp();
+                    if (lane < 16 && !(mixed && ps == part))
+                        tma_load_3d(dst + (lane & 1) * kBlkBytes + ps * 2048, &maps.kv, (lane & 1) * 64,
+                                    (kv * kHkv + s.g) * kPageTokens, id, bar);
+                } else {
+                    const bool scales = kv == 0 && lane >= 8 && lane < 24 && id < p.n_pages;   // K brings both scales
+                    const uint32_t n_scales = __popc(__ballot_sync(0xffffffffu, scales));
+                    if (lane == 0) mbar_arrive_expect_tx(bar, kTileBytes / 2 + n_scales * (kPageTokens * 4));
+                    __syncwarp();
+                    if (lane < 8)
+                        tma_load_3d(smem_u32(smem) + L::kRawOff + slot * (kTileBytes / 2) + ps * 2048, &maps.kv, 0,
+                                    (kv * kHkv + s.g) * kPageTokens, id, bar);
+                    if (scales) {
+                        const int which = lane & 1;
+                        bulk_load(smem_u32(smem) + L::kRawScaleOff + ((slot * 2 + which) * kKeys + ps * kPageTokens) * 4,
+                                  p.scales + ((static_cast<size_t>(id) * 2 + which) * kHkv + s.g) * kPageTokens, kPageTokens * 4,
+                                  bar);
                     }
                 }
                 ++u;
-                if (bad) {
-                    report_error(p.err, kErrPageIndex, kWhereChunkAttn, s.row0, kt);
-                    *failed = 1;
-                    return false;
-                }
                 return true;
             };
-            pages(s.t0, pg_k);
-            ok = load(s.t0, 0, pg_k, tile_no % L::kScaleRing);
+            int id_k = checked(id_next, s.t0), id_v;
+            if (n > 1) id_next = page_id(s.t0 + 1);
+            ok = load(s.t0, 0, id_k);
             for (int i = 0; ok && i < n; ++i) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) pg_v[k] = pg_k[k];
+                id_v = id_k;
                 if (i + 1 < n) {
-                    pages(s.t0 + i + 1, pg_k);
-                    ok = load(s.t0 + i + 1, 0, pg_k, (tile_no + i + 1) % L::kScaleRing);
+                    id_k = checked(id_next, s.t0 + i + 1);
+                    if (i + 2 < n) id_next = page_id(s.t0 + i + 2);
+                    ok = load(s.t0 + i + 1, 0, id_k);
                 }
-                ok = ok && load(s.t0 + i, 1, pg_v, (tile_no + i) % L::kScaleRing);
+                ok = ok && load(s.t0 + i, 1, id_v);
             }
-            tile_no += n;
             ++seg;
         }
-        signal_all();
-        if constexpr (k8) {
-            while (ok && waiting > 0) ok = convert();
+        if (*failed) {   // no copy outlives the CTA: the last ones issued have landed
+            for (uint32_t k = 1; k <= kRing && k <= u; ++k)
+                mbar_wait(&ring_full[(u - k) % kRing], ((u - k) / kRing) & 1u, kWaitLimitCycles);
+            for (uint32_t k = 1; k <= 2 && k <= q_issued; ++k)
+                mbar_wait(&tail->q_full[(q_issued - k) & 1u], ((q_issued - k) >> 1) & 1u, kWaitLimitCycles);
         }
-        cp_async_wait<0>();   // no copy outlives the CTA
+    } else if (k8 && warp >= L::kConvWarp && warp < L::kConvWarp + 4) {
+        // ================= 8-bit codes -> bf16 tiles =================
+        const int t = tid - 32 * L::kConvWarp, c = t & 7;
+        uint32_t u = 0, tile_no = 0;
+        bool ok = true;
+        auto convert = [&](int kt, int kv, uint32_t tile) -> bool {
+            const uint32_t stage = u % L::kStages, slot = u % (k8 ? L::kRaw : 1);
+            if (!wait_bar(&tail->raw_full[slot], (u / (k8 ? L::kRaw : 1)) & 1u, failed) ||
+                !wait_bar(&tail->empty[stage], ((u / L::kStages) & 1u) ^ 1u, failed)) {
+                if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 20);
+                *failed = 1;
+                return false;
+            }
+            const uint8_t *const raw = smem + L::kRawOff + slot * (kTileBytes / 2) + t * 16;
+            uint8_t *const dst = smem + L::kStageOff + stage * kTileBytes;
+            auto codes = [&](auto int8_t_) {
+                constexpr bool kInt8 = decltype(int8_t_)::value;
+                // lanes of the second block start with their odd chunk: no two of 8 lanes meet in a bank
+                const bool odd = c & 4;
+                uint8_t *const d0 = dst + (c >> 2) * kBlkBytes + swz(t >> 3, 2 * (c & 3) + (odd ? 1 : 0));
+                uint8_t *const d1 = dst + (c >> 2) * kBlkBytes + swz(t >> 3, 2 * (c & 3) + (odd ? 0 : 1));
+#pragma unroll
+                for (int m = 0; m < 8; ++m) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(raw + m * 2048);
+                    uint32_t h[8];
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if constexpr (kInt8) u8x4_to_bf16(ws[k], h[2 * k], h[2 * k + 1]);
+                        else e4m3x4_to_bf16(ws[k], h[2 * k], h[2 * k + 1]);
+                    }
+                    const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+                    *reinterpret_cast<uint4 *>(d0 + m * 2048) = odd ? b : a;   // rows t / 8 + 16 m
+                    *reinterpret_cast<uint4 *>(d1 + m * 2048) = odd ? a : b;
+                }
+            };
+            if (kv == 1 && p.v_int8) codes(std::true_type{});
+            else codes(std::false_type{});
+            if (kv == 0) {   // a K tile brings both scales of its tokens; none behind the last one
+                const float *const rs = reinterpret_cast<const float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys;
+                const bool live = kt * kKeys + t < s.len_end;
+                const uint32_t ring = tile % L::kScaleRing;
+                scale_ring[ring * 2 * kKeys + t] = live ? rs[t] * p.scale_log2 : 0.0f;
+                scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kKeys + t] : 0.0f;
+                mbar_arrive(&tail->scale_full[ring]);
+            }
+            fence_async_smem();
+            mbar_arrive(&tail->full[stage]);
+            mbar_arrive(&tail->raw_empty[slot]);
+            ++u;
+            return true;
+        };
+        while (ok && walk.next(p, s)) {
+            const int n = s.t1 - s.t0;
+            ok = convert(s.t0, 0, tile_no);
+            for (int i = 0; ok && i < n; ++i) {
+                if (i + 1 < n) ok = convert(s.t0 + i + 1, 0, tile_no + i + 1);
+                ok = ok && convert(s.t0 + i, 1, tile_no + i);
+            }
+            tile_no += n;
+        }
     } else if (warp == kMmaWarp) {
         // ================= MMA issuer =================
-        if (lane == 0) {
-            bool ok = true;
-            uint32_t u0 = 0, p_cnt[2] = {0, 0}, seg = 0, areas = 0;
-            while (ok && walk.next(p, s)) {
-                const int n = s.t1 - s.t0;
-                const int n0 = lane_tiles(s, 0);
-                areas = q_areas(s.mode, areas);
-                if (!(ok = wait_bar(&tail->q_full[seg & 1u], (seg >> 1) & 1u, failed))) break;
-                auto stage_of = [&](uint32_t item) { return (u0 + item) % L::kStages; };
-                auto wait_item = [&](uint32_t item) {
-                    return wait_bar(&tail->full[(u0 + item) % L::kStages], ((u0 + item) / L::kStages) & 1u, failed);
-                };
-                const bool thin = s.mode == kThin;
-                const uint32_t aQ0 = smem_u32(smem) + (thin ? kThinQ + (seg & 1u) * kThinQBytes
-                                                            : (s.pair() ? 0u : (areas >> 1) * kTileBytes));
-                const uint32_t id_thin = idesc_thin(s.cols);
-                // S of the lane's tile from K stage `stage`
-                auto issue_s = [&](int l, uint32_t stage) {
-                    fence_after();
-                    const uint32_t aK = smem_u32(smem + L::kStageOff + stage * kTileBytes);
-                    const uint32_t aQ = aQ0 + (s.pair() ? l * kTileBytes : 0u);
+        bool ok = true;
+        const bool leader = elect_one();
+        uint32_t u0 = 0, p_cnt0 = 0, p_cnt1 = 0, seg = 0, areas = 0;
+        auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, wait_bar(bar, par, failed)) != 0; };
+        while (ok && walk.next(p, s)) {
+            // warp-uniform copies: what the descriptors are made of
+            const int n = uniform(s.t1 - s.t0), n0 = uniform(lane_tiles(s, 0)), mode = uniform(s.mode), cols = uniform(s.cols);
+            const bool pair = mode == kPair, thin = mode == kThin;
+            areas = uniform(q_areas(mode, areas));
+            if (!(ok = wait(&tail->q_full[seg & 1u], (seg >> 1) & 1u))) break;
+            auto stage_of = [&](uint32_t item) { return (u0 + item) % L::kStages; };
+            auto wait_item = [&](uint32_t item) {
+                return wait(&tail->full[(u0 + item) % L::kStages], ((u0 + item) / L::kStages) & 1u);
+            };
+            const uint32_t aQ0 = smem_u32(smem) + (thin ? kThinQ + (seg & 1u) * kThinQBytes : (pair ? 0u : (areas >> 1) * kTileBytes));
+            const uint32_t id_thin = idesc_thin(cols);
+            auto free_stage = [&](uint32_t stage) {
+                if (leader) commit(&tail->empty[stage]);
+            };
+            // S of the lane's tile from K stage `stage`
+            auto issue_s = [&](int l, uint32_t stage) {
+                fence_after();
+                const Desc k(desc_kmajor(smem_u32(smem + L::kStageOff + stage * kTileBytes)));
+                const Desc q(desc_kmajor(aQ0 + (pair ? l * kTileBytes : 0u)));
+                if (leader) {
                     if (thin) {
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            const uint64_t step = 2ull * static_cast<uint64_t>(kk & 3);
-                            mma(tmem + l * 128u, desc_kmajor(aK + (kk >> 2) * kBlkBytes) + step,
-                                desc_kmajor(aQ + (kk >> 2) * kThinQBlk) + step, id_thin, kk > 0);
-                        }
+                        for (int kk = 0; kk < 8; ++kk)
+                            mma(tmem + l * 128u, k, (kk >> 2) * (kBlkBytes >> 4) + 2 * (kk & 3), q,
+                                (kk >> 2) * (kThinQBlk >> 4) + 2 * (kk & 3), id_thin, kk > 0);
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk) {
-                            const uint32_t off = static_cast<uint32_t>(kk >> 2) * kBlkBytes;
-                            const uint64_t step = 2ull * static_cast<uint64_t>(kk & 3);
-                            mma(tmem + l * 128u, desc_kmajor(aQ + off) + step, desc_kmajor(aK + off) + step, idesc_s<false>(), kk > 0);
+                            const uint32_t off = (kk >> 2) * (kBlkBytes >> 4) + 2 * (kk & 3);
+                            mma(tmem + l * 128u, q, off, k, off, idesc_s<false>(), kk > 0);
                         }
                     }
                     commit(&tail->s_full[l]);
-                };
-                auto issue_pv = [&](int l, uint32_t stage, bool acc) -> bool {
-                    if (!wait_bar(&tail->p_full[l], p_cnt[l] & 1u, failed)) return false;
-                    ++p_cnt[l];
-                    fence_after();
-                    const uint32_t aV = smem_u32(smem + L::kStageOff + stage * kTileBytes);
-                    const uint32_t tO = tmem + kTmemO + l * 128u;
+                }
+                __syncwarp();
+            };
+            auto issue_pv = [&](int l, uint32_t stage, bool acc) -> bool {
+                const uint32_t par = l ? p_cnt1++ : p_cnt0++;
+                if (!wait(&tail->p_full[l], par & 1u)) return false;
+                fence_after();
+                const Desc v(desc_mnmajor(smem_u32(smem + L::kStageOff + stage * kTileBytes)));   // 2 KB per 16 keys
+                const uint32_t tO = tmem + kTmemO + l * 128u;
+                if (leader) {
                     if (thin) {
-                        const uint32_t aP = smem_u32(smem + kThinP + l * kThinPBytes);
+                        const Desc pt(desc_thin_p(smem_u32(smem + kThinP + l * kThinPBytes), cols));
+                        const uint32_t p16 = 2u * cols;   // 16 keys of P, in 16-byte units
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma(tO, desc_mnmajor(aV + static_cast<uint32_t>(kk) * 2048u), desc_thin_p(aP + kk * 32u * s.cols, s.cols),
-                                id_thin | kIdescTransposeAB, (acc || kk > 0) ? 1 : 0);
+                            mma(tO, v, kk * 128u, pt, kk * p16, id_thin | kIdescTransposeAB, (acc || kk > 0) ? 1 : 0);
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_ta(tO, tmem + l * 128u + 8u * kk, desc_mnmajor(aV + static_cast<uint32_t>(kk) * 2048u),
-                                   idesc_pv<false>(), (acc || kk > 0) ? 1 : 0);
+                            mma_ta(tO, tmem + l * 128u + 8u * kk, v, kk * 128u, idesc_pv<false>(), (acc || kk > 0) ? 1 : 0);
                     }
                     commit(&tail->pv_done[l]);
-                    return true;
-                };
-                // first tiles
-                if (!(ok = wait_item(0))) break;
-                if (s.pair()) {
-                    if (n0 > 0) issue_s(0, stage_of(0));
-                    issue_s(1, stage_of(0));
-                    commit(&tail->empty[stage_of(0)]);
+                }
+                __syncwarp();
+                return true;
+            };
+            // first tiles
+            if (!(ok = wait_item(0))) break;
+            if (pair) {
+                if (n0 > 0) issue_s(0, stage_of(0));
+                issue_s(1, stage_of(0));
+                free_stage(stage_of(0));
+            } else {
+                issue_s(0, stage_of(0));
+                free_stage(stage_of(0));
+                if (n > 1) {
+                    if (!(ok = wait_item(1))) break;
+                    issue_s(1, stage_of(1));
+                    free_stage(stage_of(1));
+                }
+            }
+            // the previous segment's O has been read
+            if (seg > 0 && !(ok = wait(&tail->epi_done, (seg - 1) & 1u))) break;
+            for (int i = 0; ok && i < n; ++i) {
+                const uint32_t vi = item_of_v(i, n);
+                if (!(ok = wait_item(vi))) break;
+                if (pair) {
+                    const uint32_t ki = item_of_k(i + 1);
+                    if (i < n0) {
+                        if (!(ok = issue_pv(0, stage_of(vi), i > 0))) break;
+                        if (i + 1 < n0) {
+                            if (!(ok = wait_item(ki))) break;
+                            issue_s(0, stage_of(ki));
+                        }
+                    }
+                    if (!(ok = issue_pv(1, stage_of(vi), i > 0))) break;
+                    free_stage(stage_of(vi));
+                    if (i + 1 < n) {
+                        if (!(ok = wait_item(ki))) break;
+                        issue_s(1, stage_of(ki));
+                        free_stage(stage_of(ki));
+                    }
                 } else {
-                    issue_s(0, stage_of(0));
-                    commit(&tail->empty[stage_of(0)]);
-                    if (n > 1) {
-                        if (!(ok = wait_item(1))) break;
-                        issue_s(1, stage_of(1));
-                        commit(&tail->empty[stage_of(1)]);
+                    const int l = i & 1;
+                    if (!(ok = issue_pv(l, stage_of(vi), i > 1))) break;
+                    free_stage(stage_of(vi));
+                    if (i + 2 < n) {
+                        const uint32_t ki = item_of_k(i + 2);
+                        if (!(ok = wait_item(ki))) break;
+                        issue_s(l, stage_of(ki));
+                        free_stage(stage_of(ki));
                     }
                 }
-                // the previous segment's O has been read
-                if (seg > 0 && !(ok = wait_bar(&tail->epi_done, (seg - 1) & 1u, failed))) break;
-                for (int i = 0; ok && i < n; ++i) {
-                    const uint32_t vi = item_of_v(i, n);
-                    if (!(ok = wait_item(vi))) break;
-                    if (s.pair()) {
-                        const bool more = i + 1 < n;
-                        const uint32_t ki = item_of_k(i + 1);
-                        if (i < n0) {
-                            if (!(ok = issue_pv(0, stage_of(vi), i > 0))) break;
-                            if (i + 1 < n0) {
-                                if (!(ok = wait_item(ki))) break;
-                                issue_s(0, stage_of(ki));
-                            }
-                        }
-                        if (!(ok = issue_pv(1, stage_of(vi), i > 0))) break;
-                        commit(&tail->empty[stage_of(vi)]);
-                        if (more) {
-                            if (!(ok = wait_item(ki))) break;
-                            issue_s(1, stage_of(ki));
-                            commit(&tail->empty[stage_of(ki)]);
-                        }
-                    } else {
-                        if (!(ok = issue_pv(i & 1, stage_of(vi), i > 1))) break;
-                        commit(&tail->empty[stage_of(vi)]);
-                        if (i + 2 < n) {
-                            const uint32_t ki = item_of_k(i + 2);
-                            if (!(ok = wait_item(ki))) break;
-                            issue_s(i & 1, stage_of(ki));
-                            commit(&tail->empty[stage_of(ki)]);
-                        }
-                    }
-                }
-                if (!ok) break;
-                commit(&tail->seg_done[seg & 1u]);
-                u0 += 2 * n;
-                ++seg;
             }
-            if (!ok) {
-                if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 21);
-                *failed = 1;
-            }
-            // Every MMA issued has completed before TMEM is freed (error path too).
+            if (!ok) break;
+            if (leader) commit(&tail->seg_done[seg & 1u]);
+            u0 += 2 * n;
+            ++seg;
+        }
+        if (!ok) {
+            if (lane == 0 && !*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 21);
+            *failed = 1;
+        }
+        // Every MMA issued has completed before TMEM is freed (error path too).
+        if (leader) {
             commit(&tail->mma_done);
             mbar_wait(&tail->mma_done, 0, kWaitLimitCycles);
         }
         __syncwarp();
     } else {
         // ================= softmax and epilogue of lane l =================
-        const int l = (warp - 4) >> 2, quad = warp & 3, r = 32 * quad + lane;   // r: TMEM lane
+        const int l = warp >> 2, quad = warp & 3, r = 32 * quad + lane;   // r: TMEM lane
         const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * quad) << 16);
         const uint32_t tS = lane_addr + l * 128u, tO = lane_addr + kTmemO + l * 128u;
         uint32_t cnt = 0, tile_no = 0;
@@ -1207,7 +1216,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_kernel(const __grid_co
             }
             fence_before();
             mbar_arrive(&tail->epi_done);
-            if (s.first && !s.last && warp == 4 && lane == 0) {
+            if (s.first && !s.last && tid == 0) {
                 // the unit goes on in the CTAs up to the one that holds its last tile
                 const long long last = s.ustart + static_cast<long long>(s.pair() ? 2 : 1) * (s.tiles - 1);
                 p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.mode, static_cast<int>(((last + 1) * parts - 1) / total)};
@@ -1271,6 +1280,42 @@ cudaError_t smem_optin(int *optin) {
     return e != cudaSuccess ? e : cudaDeviceGetAttribute(optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+bool encode_3d(CUtensorMap *m, CUtensorMapDataType type, const void *ptr, const cuuint64_t (&dims)[3],
+               const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+    const auto enc = reinterpret_cast<EncodeTiled>(tensor_map_encoder());
+    const cuuint32_t step[3] = {1, 1, 1};
+    return enc && enc(m, type, 3, const_cast<void *>(ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool encode_maps(Maps *m, const ChunkAttendParams &p, bool k8) {
+    const cuuint64_t elem = k8 ? 1 : 2, page_rows = 2 * kHkv * kPageTokens;
+    const cuuint64_t kv_dims[3] = {kHeadDim, page_rows, static_cast<cuuint64_t>(p.n_pages)};
+    const cuuint64_t kv_strides[2] = {kHeadDim * elem, kHeadDim * elem * page_rows};
+    const cuuint32_t kv_box[3] = {k8 ? 128u : 64u, kPageTokens, 1};
+    const cuuint64_t q_dims[3] = {kHeadDim, kHq, static_cast<cuuint64_t>(p.rows)};
+    const cuuint64_t q_strides[2] = {kHeadDim * 2, kQDim * 2};
+    const cuuint32_t q_box[3] = {64, kHq / kHkv, kQueries}, thin_box[3] = {64, kHq / kHkv, kThinQueries};
+    return encode_3d(&m->kv, k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.pool, kv_dims, kv_strides,
+                     kv_box, k8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B) &&
+           encode_3d(&m->q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.q, q_dims, q_strides, q_box, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           encode_3d(&m->q_thin, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.q, q_dims, q_strides, thin_box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <bool k8> cudaError_t launch_main(const ChunkAttendParams &p, int num_sms, cudaStream_t st) {
+    int optin = 0;
+    const cudaError_t e = smem_optin(&optin);
+    if (e != cudaSuccess) return e;
+    Maps maps;
+    if (!encode_maps(&maps, p, k8)) return cudaErrorInvalidValue;
+    return launch_pdl(chunk_attn_kernel<k8>, dim3(num_sms), dim3(Layout<k8>::kThreads), smem_capped(smem_want<k8>(), optin), st, p,
+                      maps);
+}
+
 }  // namespace
 
 ChunkWorkspace chunk_workspace(int num_sms) {
@@ -1291,15 +1336,9 @@ cudaError_t prepare_chunk_attn() {
 
 cudaError_t launch_chunk_attn(const ChunkAttendParams &p, int kv_dtype, int num_sms, cudaStream_t st) {
     if (p.n <= 0 || p.rows <= 0) return cudaSuccess;
-    int optin = 0;
-    cudaError_t e = smem_optin(&optin);
-    if (e != cudaSuccess) return e;
-    if (kv_dtype == kKvBF16)
-        e = launch_pdl(chunk_attn_kernel<false>, dim3(num_sms), dim3(kThreads), smem_capped(smem_want<false>(), optin), st, p);
-    else if (kv_is_8bit(kv_dtype))
-        e = launch_pdl(chunk_attn_kernel<true>, dim3(num_sms), dim3(kThreads), smem_capped(smem_want<true>(), optin), st, p);
-    else
-        return cudaErrorInvalidValue;
+    cudaError_t e = cudaErrorInvalidValue;
+    if (kv_dtype == kKvBF16) e = launch_main<false>(p, num_sms, st);
+    else if (kv_is_8bit(kv_dtype)) e = launch_main<true>(p, num_sms, st);
     if (e != cudaSuccess) return e;
     return launch_pdl(chunk_join_kernel, dim3(num_sms, 8), dim3(kJoinThreads), 0, st, p);
 }

@@ -739,6 +739,8 @@ GemmPlan plan_gemm(int M, int N, int K, int num_sms, bool no_split = false, bool
 
 }  // namespace
 
+void *tensor_map_encoder() { return reinterpret_cast<void *>(encoder()); }
+
 bool tc_tensor_map(CUtensorMap *out, const void *ptr, int rows, int K, int box_rows) {
     return cached_map(out, ptr, rows, K, box_rows);
 }

@@ -267,6 +267,8 @@ cudaError_t launch_embed(const int *ids, int n, const void *embd, int w_dtype, i
 // epilogue 0: store, 1: accumulate into C (residual add).
 cudaError_t launch_gemm(const void *X, int x_dtype, const void *W, int w_dtype, float *C, int M, int N, int K,
                         int epilogue, cudaStream_t st);
+// cuTensorMapEncodeTiled of the driver, or null (resolved once).
+void *tensor_map_encoder();
 // tcgen05 path (bf16 X and W, K % 64 == 0): C (+)= X . W^T, split-K with f32
 // red.add when the tile grid is smaller than the SM count.
 cudaError_t prepare_gemm_tc();

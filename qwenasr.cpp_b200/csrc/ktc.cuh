@@ -33,12 +33,27 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-// The same with A in TMEM (lane = row, a 32-bit column holds two K elements).
-__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+// The same from descriptors as (low, high) words.  A tile's descriptors differ
+// in their low words alone (the address), so one thread issuing a run of MMAs
+// adds a constant to a register per operand instead of building 64-bit words.
+struct Desc {
+    uint32_t lo, hi;
+    __device__ __forceinline__ explicit Desc(uint64_t d) : lo(static_cast<uint32_t>(d)), hi(static_cast<uint32_t>(d >> 32)) {}
+};
+__device__ __forceinline__ void mma(uint32_t d, const Desc &a, uint32_t a_add, const Desc &b, uint32_t b_add, uint32_t idesc,
+                                    int acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %6, 0;\n\tmov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%3, %4};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+        "r"(a.lo + a_add), "r"(a.hi), "r"(b.lo + b_add), "r"(b.hi), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// A in TMEM (lane = row, a 32-bit column holds two K elements).
+__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, const Desc &b, uint32_t b_add, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b.lo + b_add), "r"(b.hi), "r"(idesc), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t *bar) {
@@ -130,6 +145,9 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, uint32_t src_bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(src_bytes)
                  : "memory");
+}
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 // Arrive on `bar` once every cp.async this thread issued so far has landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
