@@ -69,6 +69,7 @@ enum Mode { kThin = 0, kAlternate = 1, kPair = 2 };
 constexpr uint32_t kThinQ = kTileBytes, kThinQBytes = 8192, kThinQBlk = 4096;
 constexpr uint32_t kThinP = kTileBytes + 16384, kThinPBytes = 8192;
 constexpr int kMinCost = 2;                // least work of a CTA (tiles of alternate mode)
+constexpr int kUnitCost = 2;               // work of a unit besides its tiles
 constexpr int kPieceRows = 256;            // rows of a workspace piece (pair mode: both lanes)
 
 // K and V tiles in flight; 8-bit caches hold raw tiles besides (kRaw) and the
@@ -89,6 +90,12 @@ template <bool k8> struct Layout {
 };
 constexpr int kMaxWarps = 14;
 
+// Where a CTA's part starts: the entry, the largest end before it, the work before it.
+struct Start {
+    int i, runmax;
+    long long pre;
+};
+
 struct alignas(16) Tail {
     uint64_t q_full[2], seg_done[2];       // of a segment, by its parity
     uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], epi_done, mma_done;
@@ -97,8 +104,7 @@ struct alignas(16) Tail {
     float thin_ref[2][32];                 // thin mode: the lane's reference per column
     long long warp_sum[kMaxWarps];
     int warp_max[kMaxWarps];
-    long long pre0;                        // work before entry i0, where this CTA's part starts
-    int i0, runmax0;
+    Start from;
     uint32_t tmem;
     int failed;
 };
@@ -108,6 +114,12 @@ static_assert(Layout<true>::kTailOff + sizeof(Tail) <= 227 * 1024, "8-bit layout
 // ---- work split ----
 
 // One listed chunk: its rows, and the work of one kv head.
+// Unsigned quotient; by 32 bits where that does (a 64-bit one takes hundreds of cycles).
+__device__ __forceinline__ long long quot(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 struct Entry {
     int slot, first, m, base, nb;
     long long head_cost;
@@ -139,7 +151,8 @@ __device__ __forceinline__ Entry load_entry(const ChunkAttendParams &p, int i, i
         const long long full = e.nb - 1, p0 = (static_cast<long long>(e.base) + kKeys - 1) / kKeys;
         // full blocks end on a multiple of 128 queries: T_b = p0 + b + 1
         e.head_cost = 2 * (full * p0 + full * (full + 1) / 2) +
-                      static_cast<long long>(block_queries(e, e.nb - 1) > kQueries ? 2 : 1) * block_tiles(e, e.nb - 1);
+                      static_cast<long long>(block_queries(e, e.nb - 1) > kQueries ? 2 : 1) * block_tiles(e, e.nb - 1) +
+                      static_cast<long long>(kUnitCost) * e.nb;
     }
     return e;
 }
@@ -149,7 +162,7 @@ struct Segment {
     int t0, t1;                                    // key tiles
     int mode, cols;                                // cols: thin mode's columns (2 nq rounded up to 16)
     bool first, last;                              // holds the unit's first / last tile
-    long long ustart;
+    long long ustart;                              // position of the unit's first tile in the work
     int tiles;                                     // of the unit
     __device__ __forceinline__ bool pair() const { return mode == kPair; }
 };
@@ -165,19 +178,19 @@ struct Walk {
     int i, runmax, g, b;
     long long x, x1, ustart;
 
-    __device__ __forceinline__ void start(const ChunkAttendParams &p, const Tail *t, long long from, long long to) {
+    __device__ __forceinline__ void start(const ChunkAttendParams &p, const Start &f, long long from, long long to) {
         x = from;
         x1 = to;
         if (x >= x1) return;
-        i = t->i0;
-        runmax = t->runmax0;
+        i = f.i;
+        runmax = f.runmax;
         e = load_entry(p, i, runmax);
-        long long rem = x - t->pre0;
-        g = static_cast<int>(rem / e.head_cost);
+        long long rem = x - f.pre;
+        g = static_cast<int>(quot(rem, e.head_cost));
         rem -= g * e.head_cost;
         b = 0;
         while (b < e.nb - 1) {
-            const long long c = 2ll * block_tiles(e, b);
+            const long long c = 2ll * block_tiles(e, b) + kUnitCost;
             if (rem < c) break;
             rem -= c;
             ++b;
@@ -195,9 +208,10 @@ struct Walk {
             }
             const int cnt = block_queries(e, b), w = cnt > kQueries ? 2 : 1;
             s.tiles = block_tiles(e, b);
-            const long long uend = ustart + static_cast<long long>(w) * s.tiles;
-            s.t0 = static_cast<int>((x - ustart + w - 1) / w);
-            s.t1 = static_cast<int>(min(static_cast<long long>(s.tiles), (x1 - ustart + w - 1) / w));
+            // tile t is the CTA's that holds position `at` + w t
+            const long long at = ustart + kUnitCost, uend = at + static_cast<long long>(w) * s.tiles;
+            s.t0 = static_cast<int>(max(0ll, x - at + w - 1) >> (w - 1));
+            s.t1 = static_cast<int>(min(static_cast<long long>(s.tiles), max(0ll, x1 - at + w - 1) >> (w - 1)));
             s.slot = e.slot;
             s.g = g;
             s.row0 = e.first + b * 2 * kQueries;
@@ -210,7 +224,7 @@ struct Walk {
             s.cols = cnt > 8 ? 32 : 16;
             s.first = s.t0 == 0;
             s.last = s.t1 == s.tiles;
-            s.ustart = ustart;
+            s.ustart = at;
             x = uend;
             ustart = uend;
             if (++b == e.nb) {
@@ -268,10 +282,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 // A load that stays where it is written, a tile ahead of its use.
 __device__ __forceinline__ int load_early(const int *p) {
@@ -395,6 +413,7 @@ __device__ __forceinline__ uint32_t item_of_v(int i, int n) { return i == n - 1 
 // [row][head][dim] with boxes of 64 and 16 rows x 2 heads x 64 dims.
 struct Maps {
     CUtensorMap kv, q, q_thin;
+    CUtensorMap scales;   // 8-bit: [page][K|V][head][token], boxes of one head's K and V scales
 };
 
 template <bool k8>
@@ -437,8 +456,14 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             mbar_init(&tail->raw_empty[b], 128);
         }
         tail->failed = 0;
-        tail->i0 = -1;
+        tail->from = Start{0, 0, 0};
         fence_mbar_init();
+    }
+    if (warp == L::kLoadWarp && lane == 0) {
+        prefetch_map(&maps.kv);
+        prefetch_map(&maps.q);
+        prefetch_map(&maps.q_thin);
+        if (k8) prefetch_map(&maps.scales);
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail->tmem)),
@@ -449,55 +474,99 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     fence_before();
     pdl_wait();   // the entries, q rows and pages come from earlier kernels and copies
 
-    // ---- this CTA's part [x0, x1) of the work: running maximum of the ends, then running sum of the costs ----
-    const int per = (p.n + kThreads - 1) / kThreads, e0 = tid * per, e1 = min(p.n, e0 + per);
-    int mx = 0;
-    for (int i = e0; i < e1; ++i) mx = max(mx, __ldg(p.starts + i + 1));
-    int mx_inc = mx;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, mx_inc, o);
-        if (lane >= o) mx_inc = max(mx_inc, v);
-    }
-    if (lane == 31) tail->warp_max[warp] = mx_inc;
-    __syncthreads();
-    int runmax = __shfl_up_sync(0xffffffffu, mx_inc, 1);
-    if (lane == 0) runmax = 0;
-    for (int w = 0; w < warp; ++w) runmax = max(runmax, tail->warp_max[w]);
-    const int runmax_first = runmax;
-    long long sum = 0;
-    for (int i = e0; i < e1; ++i) {
-        const Entry e = load_entry(p, i, runmax);
-        if (e.bad && blockIdx.x == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, i, e.first);
-        sum += kHkv * e.head_cost;
-        runmax = max(runmax, __ldg(p.starts + i + 1));
-    }
-    long long inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-    }
-    if (lane == 31) tail->warp_sum[warp] = inc;
-    __syncthreads();
-    long long pre = inc - sum, total = 0;
-    for (int w = 0; w < L::kWarps; ++w) {
-        if (w < warp) pre += tail->warp_sum[w];
-        total += tail->warp_sum[w];
-    }
-    const long long parts = max(1ll, min(static_cast<long long>(gridDim.x), total / kMinCost));
-    const long long x0 = blockIdx.x < parts ? blockIdx.x * total / parts : 0;
-    const long long x1 = blockIdx.x < parts ? (blockIdx.x + 1) * total / parts : 0;
-    runmax = runmax_first;
-    for (int i = e0; i < e1; ++i) {
-        const long long c = kHkv * load_entry(p, i, runmax).head_cost;
-        if (pre <= x0 && x0 < pre + c) {
-            tail->i0 = i;
-            tail->pre0 = pre;
-            tail->runmax0 = runmax;
+    // ---- this CTA's part [x0, x1) of the work ----
+    // Running maximum of the ends and running sum of the costs over the entries, four to a thread (n <= 1024); one
+    // warp alone holds up to 32 entries, and every warp then does the same without a barrier.
+    long long x0 = 0, x1 = 0, parts = 1, total = 0;
+    auto part_of = [&]() {
+        parts = max(1ll, min(static_cast<long long>(gridDim.x), total / kMinCost));
+        if (blockIdx.x < parts) {
+            x0 = quot(blockIdx.x * total, parts);
+            x1 = quot((blockIdx.x + 1) * total, parts);
         }
-        pre += c;
-        runmax = max(runmax, __ldg(p.starts + i + 1));
+    };
+    Start from{0, 0, 0};
+    if (p.n <= 32) {
+        const int end = lane < p.n ? __ldg(p.starts + lane + 1) : 0;
+        int mx = end;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, mx, o);
+            if (lane >= o) mx = max(mx, v);
+        }
+        mx = __shfl_up_sync(0xffffffffu, mx, 1);
+        const int runmax = lane == 0 ? 0 : max(mx, 0);
+        long long c = 0;
+        if (lane < p.n) {
+            const Entry e = load_entry(p, lane, runmax);
+            if (e.bad && blockIdx.x == 0 && warp == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, lane, e.first);
+            c = kHkv * e.head_cost;
+        }
+        long long inc = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        total = __shfl_sync(0xffffffffu, inc, 31);
+        part_of();
+        const unsigned mine = __ballot_sync(0xffffffffu, inc - c <= x0 && x0 < inc);
+        const int i0 = mine ? __ffs(mine) - 1 : 0;
+        from = Start{i0, __shfl_sync(0xffffffffu, runmax, i0), __shfl_sync(0xffffffffu, inc - c, i0)};
+    } else {
+        constexpr int kPer = (kAttnMaxRows + kThreads - 1) / kThreads;
+        const int e0 = tid * kPer;
+        int ends[kPer], mx = 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) ends[k] = e0 + k < p.n ? __ldg(p.starts + e0 + k + 1) : 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) mx = max(mx, ends[k]);
+        int mx_inc = mx;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, mx_inc, o);
+            if (lane >= o) mx_inc = max(mx_inc, v);
+        }
+        if (lane == 31) tail->warp_max[warp] = mx_inc;
+        __syncthreads();
+        int runmax = __shfl_up_sync(0xffffffffu, mx_inc, 1);
+        if (lane == 0) runmax = 0;
+        for (int w = 0; w < warp; ++w) runmax = max(runmax, tail->warp_max[w]);
+        long long cost[kPer], sum = 0;
+        int maxes[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            cost[k] = 0;
+            maxes[k] = runmax;
+            if (e0 + k < p.n) {
+                const Entry e = load_entry(p, e0 + k, runmax);
+                if (e.bad && blockIdx.x == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, e0 + k, e.first);
+                cost[k] = kHkv * e.head_cost;
+            }
+            sum += cost[k];
+            runmax = max(runmax, ends[k]);
+        }
+        long long inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) tail->warp_sum[warp] = inc;
+        __syncthreads();
+        long long pre = inc - sum;
+        for (int w = 0; w < L::kWarps; ++w) {
+            if (w < warp) pre += tail->warp_sum[w];
+            total += tail->warp_sum[w];
+        }
+        part_of();
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (pre <= x0 && x0 < pre + cost[k]) tail->from = Start{e0 + k, maxes[k], pre};
+            pre += cost[k];
+        }
+        __syncthreads();
+        from = tail->from;
     }
     if (tid == 0) p.splits[blockIdx.x].c_last = -1;   // no unit starts here and goes on elsewhere (so far)
     __syncthreads();
@@ -506,7 +575,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
 
     Walk walk;
     Segment s;
-    walk.start(p, tail, x0, x1);
+    walk.start(p, from, x0, x1);
 
     if (warp == L::kLoadWarp) {
         // ================= loads =================
@@ -521,9 +590,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             *failed = 1;
             return false;
         };
-        // This lane's page of a tile.  bf16: lanes 0..15, two boxes of 64 dims a page.  8-bit: lanes 0..7, a box a
-        // page, and lanes 8..23 the pages' scales of K and V.
-        const int ps = k8 ? (lane < 8 ? lane : ((lane - 8) >> 1) & 7) : (lane >> 1) & 7;
+        const bool leader = elect_one();
+        const int ps = lane & 7;   // this lane's page of a tile
         while (ok && walk.next(p, s) && !*failed) {
             const int *const pt = p.page_table + static_cast<size_t>(s.slot) * p.maxp;
             const int key_pages = (s.len_end + kPageTokens - 1) / kPageTokens, n = s.t1 - s.t0;
@@ -546,26 +614,33 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             if (!ok) break;
             // Q rows: row 2 i + h.  Rows behind the unit's queries are some other row's or zero: rows (in thin mode
             // columns) of S that no one reads.
-            if (lane == 0) {
+            const int g2 = uniform(2 * s.g), row0 = uniform(s.row0);
+            if (leader) {
                 uint64_t *bar = &tail->q_full[seg & 1u];
                 if (s.mode == kThin) {
                     const uint32_t dst = smem_u32(smem) + kThinQ + (seg & 1u) * kThinQBytes;
                     mbar_arrive_expect_tx(bar, 2 * kThinQBlk);
-                    tma_load_3d(dst, &maps.q_thin, 0, 2 * s.g, s.row0, bar);
-                    tma_load_3d(dst + kThinQBlk, &maps.q_thin, 64, 2 * s.g, s.row0, bar);
+                    tma_load_3d(dst, &maps.q_thin, 0, g2, row0, bar);
+                    tma_load_3d(dst + kThinQBlk, &maps.q_thin, 64, g2, row0, bar);
                 } else {
                     const int tiles = s.pair() ? 2 : 1;
                     mbar_arrive_expect_tx(bar, tiles * kTileBytes);
                     for (int j = 0; j < tiles; ++j) {
                         const uint32_t dst = smem_u32(smem) + (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes);
-                        tma_load_3d(dst, &maps.q, 0, 2 * s.g, s.row0 + j * kQueries, bar);
-                        tma_load_3d(dst + kBlkBytes, &maps.q, 64, 2 * s.g, s.row0 + j * kQueries, bar);
+                        tma_load_3d(dst, &maps.q, 0, g2, row0 + j * kQueries, bar);
+                        tma_load_3d(dst + kBlkBytes, &maps.q, 64, g2, row0 + j * kQueries, bar);
                     }
                 }
             }
             ++q_issued;
+            // One thread issues a tile's boxes from warp-uniform page ids: as many lanes issuing one each took 90 cycles
+            // a box.
             auto load = [&](int kt, int kv, int id) -> bool {
                 const uint32_t slot = u % kRing;
+                int ids[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) ids[k] = __shfl_sync(0xffffffffu, id, k);
+                const int y = kv * (kHkv * kPageTokens) + g2 * (kPageTokens / 2);
                 if (!wait(&ring_empty[slot], ((u / kRing) & 1u) ^ 1u)) return false;
                 uint64_t *const bar = &ring_full[slot];
                 if constexpr (!k8) {
@@ -575,7 +650,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     const int live = s.len_end - kt * kKeys, rows = live & (kPageTokens - 1), part = live >> 4;
                     const bool mixed = kv == 1 && live < kKeys && rows != 0;
                     if (mixed) {
-                        const int page = __shfl_sync(0xffffffffu, id, 2 * part);
+                        const int page = __shfl_sync(0xffffffffu, id, part);
                         uint8_t *const to = smem + L::kStageOff + slot * kTileBytes;
                         const uint8_t *const from = static_cast<const uint8_t *>(p.pool) +
                                                     ((static_cast<size_t>(page < p.n_pages ? page : 0) * 2 + 1) * kHkv + s.g) *
@@ -591,26 +666,29 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         fence_async_smem();
                         __syncwarp();
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(bar, kTileBytes - (mixed ? kTileBytes / 8 : 0));
-                    __syncwarp();
-                    if (lane < 16 && !(mixed && ps == part))
-                        tma_load_3d(dst + (lane & 1) * kBlkBytes + ps * 2048, &maps.kv, (lane & 1) * 64,
-                                    (kv * kHkv + s.g) * kPageTokens, id, bar);
+                    if (leader) {
+                        mbar_arrive_expect_tx(bar, kTileBytes - (mixed ? kTileBytes / 8 : 0));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            if (mixed && k == part) continue;
+                            tma_load_3d(dst + k * 2048, &maps.kv, 0, y, ids[k], bar);
+                            tma_load_3d(dst + kBlkBytes + k * 2048, &maps.kv, 64, y, ids[k], bar);
+                        }
+                    }
                 } else {
-                    const bool scales = kv == 0 && lane >= 8 && lane < 24 && id < p.n_pages;   // K brings both scales
-                    const uint32_t n_scales = __popc(__ballot_sync(0xffffffffu, scales));
-                    if (lane == 0) mbar_arrive_expect_tx(bar, kTileBytes / 2 + n_scales * (kPageTokens * 4));
-                    __syncwarp();
-                    if (lane < 8)
-                        tma_load_3d(smem_u32(smem) + L::kRawOff + slot * (kTileBytes / 2) + ps * 2048, &maps.kv, 0,
-                                    (kv * kHkv + s.g) * kPageTokens, id, bar);
-                    if (scales) {
-                        const int which = lane & 1;
-                        bulk_load(smem_u32(smem) + L::kRawScaleOff + ((slot * 2 + which) * kKeys + ps * kPageTokens) * 4,
-                                  p.scales + ((static_cast<size_t>(id) * 2 + which) * kHkv + s.g) * kPageTokens, kPageTokens * 4,
-                                  bar);
+                    const uint32_t dst = smem_u32(smem) + L::kRawOff + slot * (kTileBytes / 2);
+                    const uint32_t dst_s = smem_u32(smem) + L::kRawScaleOff + slot * (2 * kKeys * 4);
+                    if (leader) {
+                        // a K tile brings both scales of its tokens
+                        mbar_arrive_expect_tx(bar, kTileBytes / 2 + (kv == 0 ? 2 * kKeys * 4 : 0));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            tma_load_3d(dst + k * 2048, &maps.kv, 0, y, ids[k], bar);
+                            if (kv == 0) tma_load_4d(dst_s + k * (2 * kPageTokens * 4), &maps.scales, 0, g2 >> 1, 0, ids[k], bar);
+                        }
                     }
                 }
+                __syncwarp();
                 ++u;
                 return true;
             };
@@ -673,11 +751,12 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             if (kv == 1 && p.v_int8) codes(std::true_type{});
             else codes(std::false_type{});
             if (kv == 0) {   // a K tile brings both scales of its tokens; none behind the last one
-                const float *const rs = reinterpret_cast<const float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys;
+                const float *const rs = reinterpret_cast<const float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys +
+                                        (t >> 4) * (2 * kPageTokens) + (t & 15);
                 const bool live = kt * kKeys + t < s.len_end;
                 const uint32_t ring = tile % L::kScaleRing;
-                scale_ring[ring * 2 * kKeys + t] = live ? rs[t] * p.scale_log2 : 0.0f;
-                scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kKeys + t] : 0.0f;
+                scale_ring[ring * 2 * kKeys + t] = live ? rs[0] * p.scale_log2 : 0.0f;
+                scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kPageTokens] : 0.0f;
                 mbar_arrive(&tail->scale_full[ring]);
             }
             fence_async_smem();
@@ -1219,7 +1298,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             if (s.first && !s.last && tid == 0) {
                 // the unit goes on in the CTAs up to the one that holds its last tile
                 const long long last = s.ustart + static_cast<long long>(s.pair() ? 2 : 1) * (s.tiles - 1);
-                p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.mode, static_cast<int>(((last + 1) * parts - 1) / total)};
+                p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.mode, static_cast<int>(quot((last + 1) * parts - 1, total))};
             }
             tile_no += n;
         }
@@ -1300,6 +1379,16 @@ bool encode_maps(Maps *m, const ChunkAttendParams &p, bool k8) {
     const cuuint64_t q_dims[3] = {kHeadDim, kHq, static_cast<cuuint64_t>(p.rows)};
     const cuuint64_t q_strides[2] = {kHeadDim * 2, kQDim * 2};
     const cuuint32_t q_box[3] = {64, kHq / kHkv, kQueries}, thin_box[3] = {64, kHq / kHkv, kThinQueries};
+    if (k8) {
+        const auto enc = reinterpret_cast<EncodeTiled>(tensor_map_encoder());
+        const cuuint64_t dims[4] = {kPageTokens, kHkv, 2, static_cast<cuuint64_t>(p.n_pages)};
+        const cuuint64_t strides[3] = {kPageTokens * 4, kHkv * kPageTokens * 4, 2 * kHkv * kPageTokens * 4};
+        const cuuint32_t box[4] = {kPageTokens, 1, 2, 1}, step[4] = {1, 1, 1, 1};
+        if (!enc || enc(&m->scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, const_cast<float *>(p.scales), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    }
     return encode_3d(&m->kv, k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.pool, kv_dims, kv_strides,
                      kv_box, k8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B) &&
            encode_3d(&m->q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.q, q_dims, q_strides, q_box, CU_TENSOR_MAP_SWIZZLE_128B) &&
@@ -1310,7 +1399,7 @@ template <bool k8> cudaError_t launch_main(const ChunkAttendParams &p, int num_s
     int optin = 0;
     const cudaError_t e = smem_optin(&optin);
     if (e != cudaSuccess) return e;
-    Maps maps;
+    Maps maps{};
     if (!encode_maps(&maps, p, k8)) return cudaErrorInvalidValue;
     return launch_pdl(chunk_attn_kernel<k8>, dim3(num_sms), dim3(Layout<k8>::kThreads), smem_capped(smem_want<k8>(), optin), st, p,
                       maps);
