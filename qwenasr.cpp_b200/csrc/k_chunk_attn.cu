@@ -37,8 +37,8 @@
 // the unrounded values.  8-bit caches: the codes are exact in bf16; a key's
 // scale multiplies its scores, a value's scale its P.
 //
-// Roles: warps 0..3 lane 0, 4..7 lane 1, one MMA warp, one load warp (TMA: a
-// page's 16 keys of a head are a box), and for 8-bit caches four warps that
+// Roles: warps 0..3 lane 0, 4..7 lane 1, one MMA warp, two load warps (TMA: a
+// page's 16 keys of a head are a box; one warp K and Q, one V), and for 8-bit caches four warps that
 // convert the raw tiles.  Staging the tiles by cp.async from four warps took
 // 2700 cycles per 32 KB and bounded every shape; the MMA warp runs its loop as
 // a whole and elects a thread only to issue, so that descriptors stay in
@@ -80,15 +80,15 @@ template <bool k8> struct Layout {
     static constexpr int kScaleRing = 4;
     static constexpr int kConvWarp = 8;    // four of them (8-bit)
     static constexpr int kMmaWarp = k8 ? 12 : 8;
-    static constexpr int kLoadWarp = kMmaWarp + 1;
-    static constexpr int kWarps = kLoadWarp + 1, kThreads = 32 * kWarps;
+    static constexpr int kLoadWarp = kMmaWarp + 1;   // K tiles and Q; the next one V tiles
+    static constexpr int kWarps = kLoadWarp + 2, kThreads = 32 * kWarps;
     static constexpr size_t kStageOff = 2 * static_cast<size_t>(kTileBytes);
     static constexpr size_t kRawOff = kStageOff + kStages * static_cast<size_t>(kTileBytes);
     static constexpr size_t kScaleOff = kRawOff + kRaw * static_cast<size_t>(kTileBytes / 2);
     static constexpr size_t kRawScaleOff = kScaleOff + (k8 ? kScaleRing * 2 * kKeys * sizeof(float) : 0);
     static constexpr size_t kTailOff = kRawScaleOff + kRaw * 2 * kKeys * sizeof(float);
 };
-constexpr int kMaxWarps = 14;
+constexpr int kMaxWarps = 15;
 
 // Where a CTA's part starts: the entry, the largest end before it, the work before it.
 struct Start {
@@ -107,6 +107,7 @@ struct alignas(16) Tail {
     Start from;
     uint32_t tmem;
     int failed;
+    uint32_t issued[5], q_issued;          // last item of each ring slot and last Q, plus one
 };
 static_assert(Layout<false>::kTailOff + sizeof(Tail) <= 227 * 1024, "bf16 layout");
 static_assert(Layout<true>::kTailOff + sizeof(Tail) <= 227 * 1024, "8-bit layout");
@@ -456,6 +457,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             mbar_init(&tail->raw_empty[b], 128);
         }
         tail->failed = 0;
+        for (int b = 0; b < 5; ++b) tail->issued[b] = 0;
+        tail->q_issued = 0;
         tail->from = Start{0, 0, 0};
         fence_mbar_init();
     }
@@ -577,16 +580,17 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     Segment s;
     walk.start(p, from, x0, x1);
 
-    if (warp == L::kLoadWarp) {
+    if (warp >= L::kLoadWarp) {
         // ================= loads =================
+        const int kv = warp - L::kLoadWarp;
         constexpr int kRing = k8 ? L::kRaw : L::kStages;
         uint64_t *const ring_full = k8 ? tail->raw_full : tail->full, *const ring_empty = k8 ? tail->raw_empty : tail->empty;
-        uint32_t u = 0, seg = 0, areas = 0, q_issued = 0;
+        uint32_t u0 = 0, seg = 0, areas = 0;
         bool ok = true, was_thin = false;
         auto wait = [&](uint64_t *bar, uint32_t par) -> bool {
             const bool done = wait_bar(bar, par, failed);
             if (__all_sync(0xffffffffu, done)) return true;
-            if (lane == 0 && !*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, static_cast<int>(u));
+            if (lane == 0 && !*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, static_cast<int>(u0));
             *failed = 1;
             return false;
         };
@@ -603,39 +607,41 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 return p.n_pages;
             };
             int id_next = page_id(s.t0);
-            // Q takes the areas of an earlier segment: the one before last has always ended (its Q barrier is
-            // reused), the last one if they meet.
-            const uint32_t prev = areas;
-            areas = q_areas(s.mode, prev);
-            const bool meets = (areas & prev) && !(s.mode == kThin && was_thin);
-            was_thin = s.mode == kThin;
-            if (seg >= 2) ok = wait(&tail->seg_done[seg & 1u], ((seg - 2) >> 1) & 1u);
-            if (ok && meets && seg >= 1) ok = wait(&tail->seg_done[(seg - 1) & 1u], ((seg - 1) >> 1) & 1u);
-            if (!ok) break;
-            // Q rows: row 2 i + h.  Rows behind the unit's queries are some other row's or zero: rows (in thin mode
-            // columns) of S that no one reads.
             const int g2 = uniform(2 * s.g), row0 = uniform(s.row0);
-            if (leader) {
-                uint64_t *bar = &tail->q_full[seg & 1u];
-                if (s.mode == kThin) {
-                    const uint32_t dst = smem_u32(smem) + kThinQ + (seg & 1u) * kThinQBytes;
-                    mbar_arrive_expect_tx(bar, 2 * kThinQBlk);
-                    tma_load_3d(dst, &maps.q_thin, 0, g2, row0, bar);
-                    tma_load_3d(dst + kThinQBlk, &maps.q_thin, 64, g2, row0, bar);
-                } else {
-                    const int tiles = s.pair() ? 2 : 1;
-                    mbar_arrive_expect_tx(bar, tiles * kTileBytes);
-                    for (int j = 0; j < tiles; ++j) {
-                        const uint32_t dst = smem_u32(smem) + (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes);
-                        tma_load_3d(dst, &maps.q, 0, g2, row0 + j * kQueries, bar);
-                        tma_load_3d(dst + kBlkBytes, &maps.q, 64, g2, row0 + j * kQueries, bar);
+            if (kv == 0) {
+                // Q takes the areas of an earlier segment: the one before last has always ended (its Q barrier is
+                // reused), the last one if they meet.
+                const uint32_t prev = areas;
+                areas = q_areas(s.mode, prev);
+                const bool meets = (areas & prev) && !(s.mode == kThin && was_thin);
+                was_thin = s.mode == kThin;
+                if (seg >= 2) ok = wait(&tail->seg_done[seg & 1u], ((seg - 2) >> 1) & 1u);
+                if (ok && meets && seg >= 1) ok = wait(&tail->seg_done[(seg - 1) & 1u], ((seg - 1) >> 1) & 1u);
+                // Q rows: row 2 i + h.  Rows behind the unit's queries are some other row's or zero: rows (in thin mode
+                // columns) of S that no one reads.
+                if (ok && leader) {
+                    uint64_t *bar = &tail->q_full[seg & 1u];
+                    if (s.mode == kThin) {
+                        const uint32_t dst = smem_u32(smem) + kThinQ + (seg & 1u) * kThinQBytes;
+                        mbar_arrive_expect_tx(bar, 2 * kThinQBlk);
+                        tma_load_3d(dst, &maps.q_thin, 0, g2, row0, bar);
+                        tma_load_3d(dst + kThinQBlk, &maps.q_thin, 64, g2, row0, bar);
+                    } else {
+                        const int tiles = s.pair() ? 2 : 1;
+                        mbar_arrive_expect_tx(bar, tiles * kTileBytes);
+                        for (int j = 0; j < tiles; ++j) {
+                            const uint32_t dst = smem_u32(smem) + (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes);
+                            tma_load_3d(dst, &maps.q, 0, g2, row0 + j * kQueries, bar);
+                            tma_load_3d(dst + kBlkBytes, &maps.q, 64, g2, row0 + j * kQueries, bar);
+                        }
                     }
                 }
+                if (!ok) break;
+                if (leader) tail->q_issued = seg + 1;
             }
-            ++q_issued;
             // One thread issues a tile's boxes from warp-uniform page ids: as many lanes issuing one each took 90 cycles
             // a box.
-            auto load = [&](int kt, int kv, int id) -> bool {
+            auto load = [&](int kt, uint32_t u, int id) -> bool {
                 const uint32_t slot = u % kRing;
                 int ids[8];
 #pragma unroll
@@ -688,29 +694,17 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         }
                     }
                 }
+                if (leader) tail->issued[slot] = u + 1;
                 __syncwarp();
-                ++u;
                 return true;
             };
-            int id_k = checked(id_next, s.t0), id_v;
-            if (n > 1) id_next = page_id(s.t0 + 1);
-            ok = load(s.t0, 0, id_k);
             for (int i = 0; ok && i < n; ++i) {
-                id_v = id_k;
-                if (i + 1 < n) {
-                    id_k = checked(id_next, s.t0 + i + 1);
-                    if (i + 2 < n) id_next = page_id(s.t0 + i + 2);
-                    ok = load(s.t0 + i + 1, 0, id_k);
-                }
-                ok = ok && load(s.t0 + i, 1, id_v);
+                const int id = checked(id_next, s.t0 + i);
+                if (i + 1 < n) id_next = page_id(s.t0 + i + 1);
+                ok = load(s.t0 + i, u0 + (kv ? item_of_v(i, n) : item_of_k(i)), id);
             }
+            u0 += 2 * n;
             ++seg;
-        }
-        if (*failed) {   // no copy outlives the CTA: the last ones issued have landed
-            for (uint32_t k = 1; k <= kRing && k <= u; ++k)
-                mbar_wait(&ring_full[(u - k) % kRing], ((u - k) / kRing) & 1u, kWaitLimitCycles);
-            for (uint32_t k = 1; k <= 2 && k <= q_issued; ++k)
-                mbar_wait(&tail->q_full[(q_issued - k) & 1u], ((q_issued - k) >> 1) & 1u, kWaitLimitCycles);
         }
     } else if (k8 && warp >= L::kConvWarp && warp < L::kConvWarp + 4) {
         // ================= 8-bit codes -> bf16 tiles =================
@@ -727,6 +721,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             }
             const uint8_t *const raw = smem + L::kRawOff + slot * (kTileBytes / 2) + t * 16;
             uint8_t *const dst = smem + L::kStageOff + stage * kTileBytes;
+            uint4 in[8];   // all of it before the first store: the compiler cannot tell the tiles apart
+#pragma unroll
+            for (int m = 0; m < 8; ++m) in[m] = *reinterpret_cast<const uint4 *>(raw + m * 2048);
             auto codes = [&](auto int8_t_) {
                 constexpr bool kInt8 = decltype(int8_t_)::value;
                 // lanes of the second block start with their odd chunk: no two of 8 lanes meet in a bank
@@ -735,7 +732,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 uint8_t *const d1 = dst + (c >> 2) * kBlkBytes + swz(t >> 3, 2 * (c & 3) + (odd ? 0 : 1));
 #pragma unroll
                 for (int m = 0; m < 8; ++m) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(raw + m * 2048);
+                    const uint4 w = in[m];
                     uint32_t h[8];
                     const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -1305,6 +1302,16 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     }
     fence_before();
     __syncthreads();
+    if (warp == L::kLoadWarp && *failed) {   // no copy outlives the CTA: the last ones issued have landed
+        constexpr uint32_t kRing = k8 ? L::kRaw : L::kStages;
+        uint64_t *const ring_full = k8 ? tail->raw_full : tail->full;
+        for (uint32_t k = 0; k < kRing; ++k) {
+            const uint32_t item = tail->issued[k];
+            if (item > 0) mbar_wait(&ring_full[k], ((item - 1) / kRing) & 1u, kWaitLimitCycles);
+        }
+        for (uint32_t q = tail->q_issued, k = 0; k < 2 && q > 0; ++k, --q)
+            mbar_wait(&tail->q_full[(q - 1) & 1u], ((q - 1) >> 1) & 1u, kWaitLimitCycles);
+    }
     if (warp == kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
