@@ -78,17 +78,21 @@ template <bool k8> struct Layout {
     static constexpr int kStages = k8 ? 3 : 5;
     static constexpr int kRaw = k8 ? 3 : 0;
     static constexpr int kScaleRing = 4;
-    static constexpr int kConvWarp = 8;    // four of them (8-bit)
-    static constexpr int kMmaWarp = k8 ? 12 : 8;
+    static constexpr int kConvWarp = 8, kConvWarps = k8 ? 8 : 0;
+    static constexpr int kMmaWarp = kConvWarp + kConvWarps;
     static constexpr int kLoadWarp = kMmaWarp + 1;   // K tiles and Q; the next one V tiles
-    static constexpr int kWarps = kLoadWarp + 2, kThreads = 32 * kWarps;
+    static constexpr int kWarps = kMmaWarp + 4, kThreads = 32 * kWarps;   // whole warpgroups: one warp is idle
+    // Registers: the launch gives every thread kRegs (65536 over the threads, in eights); the warpgroups then trade
+    // them.  bf16: 12 warps x 168 = 2 x 4 x 208 + 4 x 80 (and some left); 8-bit: 20 x 96 = 2 x 4 x 144 + 3 x 4 x 64.
+    static constexpr int kSoftmaxRegs = k8 ? 144 : 208, kOtherRegs = k8 ? 64 : 80, kRegs = k8 ? 96 : 168;
+    static_assert(8 * kSoftmaxRegs + (kWarps - 8) * kOtherRegs <= kWarps * kRegs, "register split");
     static constexpr size_t kStageOff = 2 * static_cast<size_t>(kTileBytes);
     static constexpr size_t kRawOff = kStageOff + kStages * static_cast<size_t>(kTileBytes);
     static constexpr size_t kScaleOff = kRawOff + kRaw * static_cast<size_t>(kTileBytes / 2);
     static constexpr size_t kRawScaleOff = kScaleOff + (k8 ? kScaleRing * 2 * kKeys * sizeof(float) : 0);
     static constexpr size_t kTailOff = kRawScaleOff + kRaw * 2 * kKeys * sizeof(float);
 };
-constexpr int kMaxWarps = 15;
+constexpr int kMaxWarps = 20;
 
 // Where a CTA's part starts: the entry, the largest end before it, the work before it.
 struct Start {
@@ -261,11 +265,17 @@ __device__ __forceinline__ uint32_t bf16x2_sub(uint32_t a, uint32_t b) {
 }
 // Four e4m3 codes -> bf16, exactly: sign, exponent and mantissa bits moved to
 // their places in a bf16 read 2^-120 of the value (biases 7 and 127), codes
-// below the normal range included; 0x7B80 is 2^120.
+// below the normal range included; 0x7B80 is 2^120.  A code times 16 has
+// exponent and mantissa in place and the sign at bit 11; 15 times that bit more
+// puts it at bit 15.  (Multiplications, because the pipe for shifts and logic is
+// the one that a tile's softmax fills.)
+__device__ __forceinline__ uint32_t e4m3x2_to_bf16(uint32_t two) {   // one code in the low byte of each half
+    const uint32_t y = two * 16u;
+    return bf16x2_mul((y & 0x08000800u) * 15u + y, 0x7B807B80u);
+}
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);   // each byte atop 16 bits
-    lo = bf16x2_mul(((a & 0x7f007f00u) >> 4) | (a & 0x80008000u), 0x7B807B80u);
-    hi = bf16x2_mul(((b & 0x7f007f00u) >> 4) | (b & 0x80008000u), 0x7B807B80u);
+    lo = e4m3x2_to_bf16(__byte_perm(w, 0, 0x4140));
+    hi = e4m3x2_to_bf16(__byte_perm(w, 0, 0x4342));
 }
 // Four excess-128 bytes -> bf16, exactly: 0x4300 | (u & 127) is 128 + (u & 127);
 // less 256 where u < 128, less 128 (0x4380 with bit 7 cleared) elsewhere.
@@ -297,6 +307,12 @@ __device__ __forceinline__ int load_early(const int *p) {
     int v;
     asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
+}
+template <int kRegs> __device__ __forceinline__ void set_regs_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs> __device__ __forceinline__ void set_regs_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;
@@ -446,7 +462,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             mbar_init(&tail->pv_done[b], 1);
         }
         for (int b = 0; b < L::kStages; ++b) {
-            mbar_init(&tail->full[b], k8 ? 128 : 1);
+            mbar_init(&tail->full[b], k8 ? 32 * L::kConvWarps : 1);
             mbar_init(&tail->empty[b], 1);
         }
         mbar_init(&tail->epi_done, 256);
@@ -454,7 +470,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         for (int b = 0; b < L::kScaleRing; ++b) mbar_init(&tail->scale_full[b], 128);
         for (int b = 0; b < L::kRaw; ++b) {
             mbar_init(&tail->raw_full[b], 1);
-            mbar_init(&tail->raw_empty[b], 128);
+            mbar_init(&tail->raw_empty[b], 32 * L::kConvWarps);
         }
         tail->failed = 0;
         for (int b = 0; b < 5; ++b) tail->issued[b] = 0;
@@ -578,9 +594,13 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
 
     Walk walk;
     Segment s;
-    walk.start(p, from, x0, x1);
 
-    if (warp >= L::kLoadWarp) {
+    if (warp >= L::kMmaWarp) {
+    set_regs_down<L::kOtherRegs>();
+    walk.start(p, from, x0, x1);
+    if (warp == L::kWarps - 1) {
+        // idle: fills the warpgroup
+    } else if (warp >= L::kLoadWarp) {
         // ================= loads =================
         const int kv = warp - L::kLoadWarp;
         constexpr int kRing = k8 ? L::kRaw : L::kStages;
@@ -706,72 +726,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             u0 += 2 * n;
             ++seg;
         }
-    } else if (k8 && warp >= L::kConvWarp && warp < L::kConvWarp + 4) {
-        // ================= 8-bit codes -> bf16 tiles =================
-        const int t = tid - 32 * L::kConvWarp, c = t & 7;
-        uint32_t u = 0, tile_no = 0;
-        bool ok = true;
-        auto convert = [&](int kt, int kv, uint32_t tile) -> bool {
-            const uint32_t stage = u % L::kStages, slot = u % (k8 ? L::kRaw : 1);
-            if (!wait_bar(&tail->raw_full[slot], (u / (k8 ? L::kRaw : 1)) & 1u, failed) ||
-                !wait_bar(&tail->empty[stage], ((u / L::kStages) & 1u) ^ 1u, failed)) {
-                if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 20);
-                *failed = 1;
-                return false;
-            }
-            const uint8_t *const raw = smem + L::kRawOff + slot * (kTileBytes / 2) + t * 16;
-            uint8_t *const dst = smem + L::kStageOff + stage * kTileBytes;
-            uint4 in[8];   // all of it before the first store: the compiler cannot tell the tiles apart
-#pragma unroll
-            for (int m = 0; m < 8; ++m) in[m] = *reinterpret_cast<const uint4 *>(raw + m * 2048);
-            auto codes = [&](auto int8_t_) {
-                constexpr bool kInt8 = decltype(int8_t_)::value;
-                // lanes of the second block start with their odd chunk: no two of 8 lanes meet in a bank
-                const bool odd = c & 4;
-                uint8_t *const d0 = dst + (c >> 2) * kBlkBytes + swz(t >> 3, 2 * (c & 3) + (odd ? 1 : 0));
-                uint8_t *const d1 = dst + (c >> 2) * kBlkBytes + swz(t >> 3, 2 * (c & 3) + (odd ? 0 : 1));
-#pragma unroll
-                for (int m = 0; m < 8; ++m) {
-                    const uint4 w = in[m];
-                    uint32_t h[8];
-                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if constexpr (kInt8) u8x4_to_bf16(ws[k], h[2 * k], h[2 * k + 1]);
-                        else e4m3x4_to_bf16(ws[k], h[2 * k], h[2 * k + 1]);
-                    }
-                    const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-                    *reinterpret_cast<uint4 *>(d0 + m * 2048) = odd ? b : a;   // rows t / 8 + 16 m
-                    *reinterpret_cast<uint4 *>(d1 + m * 2048) = odd ? a : b;
-                }
-            };
-            if (kv == 1 && p.v_int8) codes(std::true_type{});
-            else codes(std::false_type{});
-            if (kv == 0) {   // a K tile brings both scales of its tokens; none behind the last one
-                const float *const rs = reinterpret_cast<const float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys +
-                                        (t >> 4) * (2 * kPageTokens) + (t & 15);
-                const bool live = kt * kKeys + t < s.len_end;
-                const uint32_t ring = tile % L::kScaleRing;
-                scale_ring[ring * 2 * kKeys + t] = live ? rs[0] * p.scale_log2 : 0.0f;
-                scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kPageTokens] : 0.0f;
-                mbar_arrive(&tail->scale_full[ring]);
-            }
-            fence_async_smem();
-            mbar_arrive(&tail->full[stage]);
-            mbar_arrive(&tail->raw_empty[slot]);
-            ++u;
-            return true;
-        };
-        while (ok && walk.next(p, s)) {
-            const int n = s.t1 - s.t0;
-            ok = convert(s.t0, 0, tile_no);
-            for (int i = 0; ok && i < n; ++i) {
-                if (i + 1 < n) ok = convert(s.t0 + i + 1, 0, tile_no + i + 1);
-                ok = ok && convert(s.t0 + i, 1, tile_no + i);
-            }
-            tile_no += n;
-        }
-    } else if (warp == kMmaWarp) {
+    } else {
         // ================= MMA issuer =================
         bool ok = true;
         const bool leader = elect_one();
@@ -900,7 +855,87 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             mbar_wait(&tail->mma_done, 0, kWaitLimitCycles);
         }
         __syncwarp();
+    }
+    } else if (k8 && warp >= L::kConvWarp) {
+        set_regs_down<L::kOtherRegs>();
+        walk.start(p, from, x0, x1);
+        // ================= 8-bit codes -> bf16 tiles =================
+        // Thread: 16 codes (piece c of 8) of rows t / 8 + 32 m.
+        constexpr int kRows = 128 * 8 / (32 * (k8 ? L::kConvWarps : 8));
+        const int t = tid - 32 * L::kConvWarp, c = t & 7;
+        // Pieces 4..7 (the second 64 dims) store their odd half first, so that no two of 8 lanes meet in a bank; they
+        // read their halves in that order, too.
+        const int odd = (c >> 2) & 1;
+        uint32_t u = 0, tile_no = 0;
+        bool ok = true;
+        auto convert = [&](int kt, int kv, uint32_t tile) -> bool {
+            const uint32_t stage = u % L::kStages, slot = u % (k8 ? L::kRaw : 1);
+            if (!wait_bar(&tail->raw_full[slot], (u / (k8 ? L::kRaw : 1)) & 1u, failed)) {
+                if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 20);
+                *failed = 1;
+                return false;
+            }
+            const uint8_t *const raw = smem + L::kRawOff + slot * (kTileBytes / 2) + t * 16;
+            uint2 in[kRows][2];   // all of it before the first store: the compiler cannot tell the tiles apart
+#pragma unroll
+            for (int m = 0; m < kRows; ++m) {
+                in[m][0] = *reinterpret_cast<const uint2 *>(raw + m * 4096 + odd * 8);
+                in[m][1] = *reinterpret_cast<const uint2 *>(raw + m * 4096 + (odd ^ 1) * 8);
+            }
+            if (kv == 0 && t < kKeys) {   // a K tile brings both scales of its tokens; none behind the last one
+                const float *const rs = reinterpret_cast<const float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys +
+                                        (t >> 4) * (2 * kPageTokens) + (t & 15);
+                const bool live = kt * kKeys + t < s.len_end;
+                const uint32_t ring = tile % L::kScaleRing;
+                scale_ring[ring * 2 * kKeys + t] = live ? rs[0] * p.scale_log2 : 0.0f;
+                scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kPageTokens] : 0.0f;
+                mbar_arrive(&tail->scale_full[ring]);
+            }
+            mbar_arrive(&tail->raw_empty[slot]);
+            if (!wait_bar(&tail->empty[stage], ((u / L::kStages) & 1u) ^ 1u, failed)) {
+                if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 19);
+                *failed = 1;
+                return false;
+            }
+            uint8_t *const blk = smem + L::kStageOff + stage * kTileBytes + (c >> 2) * kBlkBytes;
+            uint8_t *const d0 = blk + swz(t >> 3, 2 * (c & 3) + odd), *const d1 = blk + swz(t >> 3, 2 * (c & 3) + (odd ^ 1));
+            auto codes = [&](auto int8_t_) {
+                constexpr bool kInt8 = decltype(int8_t_)::value;
+#pragma unroll
+                for (int m = 0; m < kRows; ++m) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t h[4];
+                        if constexpr (kInt8) {
+                            u8x4_to_bf16(in[m][k].x, h[0], h[1]);
+                            u8x4_to_bf16(in[m][k].y, h[2], h[3]);
+                        } else {
+                            e4m3x4_to_bf16(in[m][k].x, h[0], h[1]);
+                            e4m3x4_to_bf16(in[m][k].y, h[2], h[3]);
+                        }
+                        *reinterpret_cast<uint4 *>((k ? d1 : d0) + m * 4096) = make_uint4(h[0], h[1], h[2], h[3]);
+                    }
+                }
+            };
+            if (kv == 1 && p.v_int8) codes(std::true_type{});
+            else codes(std::false_type{});
+            fence_async_smem();
+            mbar_arrive(&tail->full[stage]);
+            ++u;
+            return true;
+        };
+        while (ok && walk.next(p, s)) {
+            const int n = s.t1 - s.t0;
+            ok = convert(s.t0, 0, tile_no);
+            for (int i = 0; ok && i < n; ++i) {
+                if (i + 1 < n) ok = convert(s.t0 + i + 1, 0, tile_no + i + 1);
+                ok = ok && convert(s.t0 + i, 1, tile_no + i);
+            }
+            tile_no += n;
+        }
     } else {
+        set_regs_up<L::kSoftmaxRegs>();
+        walk.start(p, from, x0, x1);
         // ================= softmax and epilogue of lane l =================
         const int l = warp >> 2, quad = warp & 3, r = 32 * quad + lane;   // r: TMEM lane
         const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * quad) << 16);
@@ -910,6 +945,19 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             if (wait_bar(bar, par, failed)) return;
             if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 22);
             *failed = 1;
+        };
+
+        auto rescale_o = [&](float alpha) {
+            fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                float o[32];
+                tmem_ld32(tO + 32u * c, o);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] *= alpha;
+                tmem_st32(tO + 32u * c, o);
+            }
+            tmem_wait_st();
         };
 
         // Key tile kt (the ti-th of the segment) of pair and alternate mode; thread = query row.
@@ -931,7 +979,67 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 if (d < 0) return ((1u << -d) - 1u) | static_cast<uint32_t>(bits << -d);
                 return d < 64 ? static_cast<uint32_t>(bits >> d) : 0u;
             };
-            // pass 1: the row's largest score
+            if constexpr (!k8) {
+                // One reading: the row's 128 scores stay in registers between the maximum and P.
+                uint32_t sc[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32_issue(tS + 32u * c, sc[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_wait_ld32(sc[c]);
+                float t2[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if constexpr (kMasked) {
+                        const uint32_t w = seen(c);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sc[c][j] = (w >> j) & 1u ? sc[c][j] : 0xff800000u;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2)
+                        t2[c] = fmaxf(t2[c], fmaxf(__uint_as_float(sc[c][j]), __uint_as_float(sc[c][j + 1])));
+                }
+                const float top = fmaxf(fmaxf(t2[0], t2[1]), fmaxf(t2[2], t2[3])) * p.scale_log2;
+                float alpha = 1.0f;
+                bool rescale = false;
+                if (start) {
+                    m_ref = top;
+                } else if (top > m_ref + kRescaleLog2) {
+                    alpha = ex2_approx(m_ref - top);   // 0 where nothing was seen so far
+                    m_ref = top;
+                    l_run *= alpha;
+                    rescale = true;
+                }
+                // P V of the lane's previous tile has completed: O is at rest
+                if (!start) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
+                if (__any_sync(0xffffffffu, rescale)) rescale_o(alpha);
+                const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
+                const uint64_t nsub2 = f2(-sub, -sub), c2 = f2(p.scale_log2, p.scale_log2);
+                uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        float e[4];
+                        un_f2(fma_f2(f2(__uint_as_float(sc[c][j]), __uint_as_float(sc[c][j + 1])), c2, nsub2), e[0], e[1]);
+                        un_f2(fma_f2(f2(__uint_as_float(sc[c][j + 2]), __uint_as_float(sc[c][j + 3])), c2, nsub2), e[2], e[3]);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
+                        acc[0] = add_f2(acc[0], f2(e[0], e[1]));
+                        acc[1] = add_f2(acc[1], f2(e[2], e[3]));
+                        pk[j / 2] = pack_bf16x2(e[0], e[1]);
+                        pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                    }
+                    tmem_st16(tS + 16u * c, pk);
+                }
+                float s0, s1, s2, s3;
+                un_f2(acc[0], s0, s1);
+                un_f2(acc[1], s2, s3);
+                l_run += (s0 + s1) + (s2 + s3);
+                tmem_wait_st();
+                return;
+            }
+            // 8-bit caches have fewer registers to spare: two readings.  Pass 1: the row's largest score.
             float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             uint32_t sr[2][32];
             tmem_ld32_issue(tS, sr[0]);
@@ -974,16 +1082,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             if (!start) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
             if (__any_sync(0xffffffffu, rescale)) {
                 tmem_wait_ld32(sr[0]);
-                fence_after();
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float o[32];
-                    tmem_ld32(tO + 32u * c, o);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] *= alpha;
-                    tmem_st32(tO + 32u * c, o);
-                }
-                tmem_wait_st();
+                rescale_o(alpha);
                 tmem_ld32_issue(tS, sr[0]);
             }
             // pass 2: P into S's first 64 columns; chunk c's 16 columns lie in chunks already read
