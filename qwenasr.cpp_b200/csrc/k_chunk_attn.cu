@@ -102,7 +102,7 @@ struct Start {
 
 struct alignas(16) Tail {
     uint64_t q_full[2], seg_done[2];       // of a segment, by its parity
-    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], epi_done, mma_done;
+    uint64_t full[5], empty[5], s_full[2], p_full[2], o_full[2], epi_done, mma_done;
     uint64_t scale_full[4], raw_full[3], raw_empty[3];   // 8-bit
     float2 ml[2][128];                     // (reference, sum) of each lane's rows, at a segment's end
     float thin_ref[2][32];                 // thin mode: the lane's reference per column
@@ -319,7 +319,10 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r != 0;
 }
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+// A value that all lanes hold alike (and >= 0), by way of a warp reduction, whose result the compiler knows to be
+// uniform: what MMA and TMA instructions take from uniform registers then needs no transfer each time.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ int uniform(int v) { return static_cast<int>(uniform(static_cast<uint32_t>(v))); }
 
 // Packed pairs of f32 (two lanes of one instruction).
 __device__ __forceinline__ uint64_t f2(float a, float b) {
@@ -357,6 +360,11 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool pred) {
         : "r"(static_cast<int>(pred)), "r"(id), "r"(threads)
         : "memory");
     return r != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 constexpr int kBarLane = 1, kBarBoth = 3;   // ids kBarLane + lane, kBarBoth
 
@@ -458,14 +466,14 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             mbar_init(&tail->q_full[b], 1);
             mbar_init(&tail->seg_done[b], 1);
             mbar_init(&tail->s_full[b], 1);
-            mbar_init(&tail->p_full[b], 128);
-            mbar_init(&tail->pv_done[b], 1);
+            mbar_init(&tail->p_full[b], 4);      // warps
+            mbar_init(&tail->o_full[b], 1);
         }
         for (int b = 0; b < L::kStages; ++b) {
             mbar_init(&tail->full[b], k8 ? 32 * L::kConvWarps : 1);
             mbar_init(&tail->empty[b], 1);
         }
-        mbar_init(&tail->epi_done, 256);
+        mbar_init(&tail->epi_done, 8);      // warps
         mbar_init(&tail->mma_done, 1);
         for (int b = 0; b < L::kScaleRing; ++b) mbar_init(&tail->scale_full[b], 128);
         for (int b = 0; b < L::kRaw; ++b) {
@@ -615,10 +623,11 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             return false;
         };
         const bool leader = elect_one();
+        const uint32_t smem_u = uniform(smem_u32(smem));
         const int ps = lane & 7;   // this lane's page of a tile
         while (ok && walk.next(p, s) && !*failed) {
             const int *const pt = p.page_table + static_cast<size_t>(s.slot) * p.maxp;
-            const int key_pages = (s.len_end + kPageTokens - 1) / kPageTokens, n = s.t1 - s.t0;
+            const int key_pages = (s.len_end + kPageTokens - 1) / kPageTokens, n = uniform(s.t1 - s.t0);
             auto page_id = [&](int kt) { return kt * 8 + ps < key_pages ? load_early(pt + kt * 8 + ps) : p.n_pages; };
             // Outside the map's pages a box reads as zero: behind the last page, and for a bad id.
             auto checked = [&](int id, int kt) {
@@ -665,12 +674,12 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 const uint32_t slot = u % kRing;
                 int ids[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) ids[k] = __shfl_sync(0xffffffffu, id, k);
+                for (int k = 0; k < 8; ++k) ids[k] = uniform(ps == k ? id : 0);
                 const int y = kv * (kHkv * kPageTokens) + g2 * (kPageTokens / 2);
                 if (!wait(&ring_empty[slot], ((u / kRing) & 1u) ^ 1u)) return false;
                 uint64_t *const bar = &ring_full[slot];
                 if constexpr (!k8) {
-                    const uint32_t dst = smem_u32(smem) + L::kStageOff + slot * kTileBytes;
+                    const uint32_t dst = smem_u + static_cast<uint32_t>(L::kStageOff) + slot * kTileBytes;
                     // V rows behind the last token must be zero (their weight is zero, but not a NaN's product with
                     // it): the page the stream ends in comes by plain loads.
                     const int live = s.len_end - kt * kKeys, rows = live & (kPageTokens - 1), part = live >> 4;
@@ -702,8 +711,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         }
                     }
                 } else {
-                    const uint32_t dst = smem_u32(smem) + L::kRawOff + slot * (kTileBytes / 2);
-                    const uint32_t dst_s = smem_u32(smem) + L::kRawScaleOff + slot * (2 * kKeys * 4);
+                    const uint32_t dst = smem_u + static_cast<uint32_t>(L::kRawOff) + slot * (kTileBytes / 2);
+                    const uint32_t dst_s = smem_u + static_cast<uint32_t>(L::kRawScaleOff) + slot * (2 * kKeys * 4);
                     if (leader) {
                         // a K tile brings both scales of its tokens
                         mbar_arrive_expect_tx(bar, kTileBytes / 2 + (kv == 0 ? 2 * kKeys * 4 : 0));
@@ -731,6 +740,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         bool ok = true;
         const bool leader = elect_one();
         uint32_t u0 = 0, p_cnt0 = 0, p_cnt1 = 0, seg = 0, areas = 0;
+        const uint32_t tmem_u = uniform(tmem), smem_u = uniform(smem_u32(smem));
         auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, wait_bar(bar, par, failed)) != 0; };
         while (ok && walk.next(p, s)) {
             // warp-uniform copies: what the descriptors are made of
@@ -742,7 +752,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             auto wait_item = [&](uint32_t item) {
                 return wait(&tail->full[(u0 + item) % L::kStages], ((u0 + item) / L::kStages) & 1u);
             };
-            const uint32_t aQ0 = smem_u32(smem) + (thin ? kThinQ + (seg & 1u) * kThinQBytes : (pair ? 0u : (areas >> 1) * kTileBytes));
+            const uint32_t aQ0 = smem_u + (thin ? kThinQ + (seg & 1u) * kThinQBytes : (pair ? 0u : (areas >> 1) * kTileBytes));
             const uint32_t id_thin = idesc_thin(cols);
             auto free_stage = [&](uint32_t stage) {
                 if (leader) commit(&tail->empty[stage]);
@@ -750,34 +760,34 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             // S of the lane's tile from K stage `stage`
             auto issue_s = [&](int l, uint32_t stage) {
                 fence_after();
-                const Desc k(desc_kmajor(smem_u32(smem + L::kStageOff + stage * kTileBytes)));
+                const Desc k(desc_kmajor(smem_u + static_cast<uint32_t>(L::kStageOff) + stage * kTileBytes));
                 const Desc q(desc_kmajor(aQ0 + (pair ? l * kTileBytes : 0u)));
                 if (leader) {
                     if (thin) {
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma(tmem + l * 128u, k, (kk >> 2) * (kBlkBytes >> 4) + 2 * (kk & 3), q,
+                            mma(tmem_u + l * 128u, k, (kk >> 2) * (kBlkBytes >> 4) + 2 * (kk & 3), q,
                                 (kk >> 2) * (kThinQBlk >> 4) + 2 * (kk & 3), id_thin, kk > 0);
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk) {
                             const uint32_t off = (kk >> 2) * (kBlkBytes >> 4) + 2 * (kk & 3);
-                            mma(tmem + l * 128u, q, off, k, off, idesc_s<false>(), kk > 0);
+                            mma(tmem_u + l * 128u, q, off, k, off, idesc_s<false>(), kk > 0);
                         }
                     }
                     commit(&tail->s_full[l]);
                 }
                 __syncwarp();
             };
-            auto issue_pv = [&](int l, uint32_t stage, bool acc) -> bool {
+            auto issue_pv = [&](int l, uint32_t stage, bool acc, bool last) -> bool {
                 const uint32_t par = l ? p_cnt1++ : p_cnt0++;
                 if (!wait(&tail->p_full[l], par & 1u)) return false;
                 fence_after();
-                const Desc v(desc_mnmajor(smem_u32(smem + L::kStageOff + stage * kTileBytes)));   // 2 KB per 16 keys
-                const uint32_t tO = tmem + kTmemO + l * 128u;
+                const Desc v(desc_mnmajor(smem_u + static_cast<uint32_t>(L::kStageOff) + stage * kTileBytes));   // 2 KB per 16 keys
+                const uint32_t tO = tmem_u + kTmemO + l * 128u;
                 if (leader) {
                     if (thin) {
-                        const Desc pt(desc_thin_p(smem_u32(smem + kThinP + l * kThinPBytes), cols));
+                        const Desc pt(desc_thin_p(smem_u + kThinP + l * kThinPBytes, cols));
                         const uint32_t p16 = 2u * cols;   // 16 keys of P, in 16-byte units
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
@@ -785,9 +795,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_ta(tO, tmem + l * 128u + 8u * kk, v, kk * 128u, idesc_pv<false>(), (acc || kk > 0) ? 1 : 0);
+                            mma_ta(tO, tmem_u + l * 128u + 8u * kk, v, kk * 128u, idesc_pv<false>(), (acc || kk > 0) ? 1 : 0);
                     }
-                    commit(&tail->pv_done[l]);
+                    if (last) commit(&tail->o_full[l]);   // the lane's O of this segment is complete
                 }
                 __syncwarp();
                 return true;
@@ -815,13 +825,13 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 if (pair) {
                     const uint32_t ki = item_of_k(i + 1);
                     if (i < n0) {
-                        if (!(ok = issue_pv(0, stage_of(vi), i > 0))) break;
+                        if (!(ok = issue_pv(0, stage_of(vi), i > 0, i + 1 == n0))) break;
                         if (i + 1 < n0) {
                             if (!(ok = wait_item(ki))) break;
                             issue_s(0, stage_of(ki));
                         }
                     }
-                    if (!(ok = issue_pv(1, stage_of(vi), i > 0))) break;
+                    if (!(ok = issue_pv(1, stage_of(vi), i > 0, i + 1 == n))) break;
                     free_stage(stage_of(vi));
                     if (i + 1 < n) {
                         if (!(ok = wait_item(ki))) break;
@@ -830,7 +840,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     }
                 } else {
                     const int l = i & 1;
-                    if (!(ok = issue_pv(l, stage_of(vi), i > 1))) break;
+                    if (!(ok = issue_pv(l, stage_of(vi), i > 1, i + 2 >= n))) break;
                     free_stage(stage_of(vi));
                     if (i + 2 < n) {
                         const uint32_t ki = item_of_k(i + 2);
@@ -940,7 +950,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         const int l = warp >> 2, quad = warp & 3, r = 32 * quad + lane;   // r: TMEM lane
         const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * quad) << 16);
         const uint32_t tS = lane_addr + l * 128u, tO = lane_addr + kTmemO + l * 128u;
-        uint32_t cnt = 0, tile_no = 0;
+        uint32_t cnt = 0, tile_no = 0, seg_cnt = 0;   // tiles and segments of this lane
+        // S of a tile is issued behind P V of the lane's previous one by the same thread, so s_full also says that O is
+        // at rest and that the previous P has been read.
         auto wait = [&](uint64_t *bar, uint32_t par) {
             if (wait_bar(bar, par, failed)) return;
             if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 22);
@@ -996,7 +1008,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 2)
-                        t2[c] = fmaxf(t2[c], fmaxf(__uint_as_float(sc[c][j]), __uint_as_float(sc[c][j + 1])));
+                        t2[c] = max3(t2[c], __uint_as_float(sc[c][j]), __uint_as_float(sc[c][j + 1]));
                 }
                 const float top = fmaxf(fmaxf(t2[0], t2[1]), fmaxf(t2[2], t2[3])) * p.scale_log2;
                 float alpha = 1.0f;
@@ -1009,8 +1021,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     l_run *= alpha;
                     rescale = true;
                 }
-                // P V of the lane's previous tile has completed: O is at rest
-                if (!start) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
                 if (__any_sync(0xffffffffu, rescale)) rescale_o(alpha);
                 const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
                 const uint64_t nsub2 = f2(-sub, -sub), c2 = f2(p.scale_log2, p.scale_log2);
@@ -1062,8 +1072,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     for (int q = 0; q < 4; ++q) {
                         if (kMasked && !((w >> (j + q)) & 1u)) v[q] = -INFINITY;
                     }
-                    t4[0] = fmaxf(t4[0], fmaxf(v[0], v[1]));
-                    t4[1] = fmaxf(t4[1], fmaxf(v[2], v[3]));
+                    t4[0] = max3(t4[0], v[0], v[1]);
+                    t4[1] = max3(t4[1], v[2], v[3]);
                 }
             }
             float top = fmaxf(t4[0], t4[1]);
@@ -1078,8 +1088,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 l_run *= alpha;
                 rescale = true;
             }
-            // P V of the lane's previous tile has completed: O is at rest
-            if (!start) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
             if (__any_sync(0xffffffffu, rescale)) {
                 tmem_wait_ld32(sr[0]);
                 rescale_o(alpha);
@@ -1169,8 +1177,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         }
                     }
                 }
-                // P V of the lane's previous tile has completed: its P may go, O is at rest
-                if (k > 0) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
                 bool move = k == 0;
                 if (k > 0) {
                     float over = -INFINITY;
@@ -1243,11 +1249,12 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
                 fence_async_smem();
                 fence_before();
-                mbar_arrive(&tail->p_full[l]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tail->p_full[l]);
                 ++cnt;
             }
             if (mine > 0) {
-                wait(&tail->pv_done[l], (cnt - 1u) & 1u);
+                wait(&tail->o_full[l], seg_cnt++ & 1u);
                 // Column sums over the lane's 128 threads.  (Not by way of the P tile: with the last P V done, the
                 // loaders may already put a later segment's Q there.)
                 float *const wsum = reinterpret_cast<float *>(&tail->ml[l][64]);
@@ -1311,22 +1318,23 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     if (s.nq < 64) bits &= (1ull << s.nq) - 1ull;
                 }
                 float m_ref = -INFINITY, l_run = 0.0f;
-                for (int k = 0; k < mine; ++k) {
-                    const int ti = s.pair() ? k : 2 * k + l, kt = s.t0 + ti;
-                    wait(&tail->s_full[l], cnt & 1u);
-                    fence_after();
-                    if (!active) {
-                        if (k > 0) wait(&tail->pv_done[l], (cnt - 1u) & 1u);
-                    } else if (kt * kKeys + kKeys - 1 > (p.mask ? s.base - 1 : pos_min)) {
-                        row_tile(std::true_type{}, kt, ti, pos, bits, k == 0, m_ref, l_run);
-                    } else {
-                        row_tile(std::false_type{}, kt, ti, pos, bits, k == 0, m_ref, l_run);
+                // tiles that every row sees whole come first
+                const int step = s.pair() ? 1 : 2, ti0 = s.pair() ? 0 : l, clear = ((p.mask ? s.base : pos_min + 1) >> 7) - s.t0;
+                auto tiles = [&](auto masked_t, int ti, int end) {
+                    for (; ti < end; ti += step) {
+                        wait(&tail->s_full[l], cnt & 1u);
+                        ++cnt;
+                        fence_after();
+                        if (active) row_tile(masked_t, s.t0 + ti, ti, pos, bits, ti == ti0, m_ref, l_run);
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&tail->p_full[l]);
                     }
-                    fence_before();
-                    mbar_arrive(&tail->p_full[l]);
-                    ++cnt;
-                }
-                if (mine > 0) wait(&tail->pv_done[l], (cnt - 1u) & 1u);   // the lane's last P V
+                    return ti;
+                };
+                const int end = ti0 + step * mine;
+                tiles(std::true_type{}, tiles(std::false_type{}, ti0, min(clear, end)), end);
+                if (mine > 0) wait(&tail->o_full[l], seg_cnt++ & 1u);
                 const bool whole = s.first && s.last;
                 float a0 = 1.0f, a1 = 0.0f, m_tot = m_ref, l_tot = l_run;
                 if (!s.pair()) {
@@ -1390,7 +1398,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 }
             }
             fence_before();
-            mbar_arrive(&tail->epi_done);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tail->epi_done);
             if (s.first && !s.last && tid == 0) {
                 // the unit goes on in the CTAs up to the one that holds its last tile
                 const long long last = s.ustart + static_cast<long long>(s.pair() ? 2 : 1) * (s.tiles - 1);
