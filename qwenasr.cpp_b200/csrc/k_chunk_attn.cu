@@ -62,6 +62,7 @@ constexpr int kQueries = 64;               // queries of a query tile
 constexpr uint32_t kTmemCols = 512;        // S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512)
 constexpr uint32_t kTmemO = 256;
 constexpr float kRescaleLog2 = 30.0f;
+constexpr float kTileSumMax = 1099511627776.0f;   // 2^40: some term of a tile's sum is past 2^33, and none past 2^40 if not
 constexpr int kThinQueries = 16;           // most queries of thin mode
 enum Mode { kThin = 0, kAlternate = 1, kPair = 2 };
 // The two 32 KB areas before the stages: a query tile each, or area 1 split
@@ -973,8 +974,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         };
 
         // Key tile kt (the ti-th of the segment) of pair and alternate mode; thread = query row.
-        auto row_tile = [&](auto masked_t, int kt, int ti, int pos, unsigned long long bits, bool start, float &m_ref,
-                            float &l_run) {
+        // No maximum is taken as long as the row's reference will do: the tile's sum, which is needed anyway, tells
+        // when one of its terms has grown past 2^kRescaleLog2.  P is stored only then, since it lies over S.
+        auto row_tile = [&](auto masked_t, int kt, int ti, int pos, unsigned long long bits, float &m_ref, float &l_run) {
             constexpr bool kMasked = decltype(masked_t)::value;
             const uint32_t slot = (tile_no + ti) % L::kScaleRing;
             const float *ks = scale_ring + slot * 2 * kKeys, *vs = ks + kKeys;
@@ -991,150 +993,91 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 if (d < 0) return ((1u << -d) - 1u) | static_cast<uint32_t>(bits << -d);
                 return d < 64 ? static_cast<uint32_t>(bits >> d) : 0u;
             };
-            if constexpr (!k8) {
-                // One reading: the row's 128 scores stay in registers between the maximum and P.
-                uint32_t sc[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32_issue(tS + 32u * c, sc[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_wait_ld32(sc[c]);
-                float t2[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+            // the row's largest score of the tile (rare: rolled up)
+            auto largest = [&]() -> float {
+                float top = -INFINITY;
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
-                    if constexpr (kMasked) {
-                        const uint32_t w = seen(c);
+                    uint32_t v[32];
+                    tmem_ld32_issue(tS + 32u * c, v);
+                    tmem_wait_ld32(v);
+                    const uint32_t w = kMasked ? seen(c) : 0xffffffffu;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) sc[c][j] = (w >> j) & 1u ? sc[c][j] : 0xff800000u;
+                    for (int j = 0; j < 32; ++j) {
+                        float x = __uint_as_float(v[j]) * (k8 ? ks[32 * c + j] : p.scale_log2);
+                        if (kMasked && !((w >> j) & 1u)) x = -INFINITY;
+                        top = fmaxf(top, x);
                     }
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2)
-                        t2[c] = max3(t2[c], __uint_as_float(sc[c][j]), __uint_as_float(sc[c][j + 1]));
                 }
-                const float top = fmaxf(fmaxf(t2[0], t2[1]), fmaxf(t2[2], t2[3])) * p.scale_log2;
-                float alpha = 1.0f;
-                bool rescale = false;
-                if (start) {
-                    m_ref = top;
-                } else if (top > m_ref + kRescaleLog2) {
-                    alpha = ex2_approx(m_ref - top);   // 0 where nothing was seen so far
-                    m_ref = top;
-                    l_run *= alpha;
-                    rescale = true;
-                }
-                if (__any_sync(0xffffffffu, rescale)) rescale_o(alpha);
+                return top;
+            };
+            if (__any_sync(0xffffffffu, m_ref == -INFINITY)) {   // a row that has seen nothing yet
+                const float top = largest();
+                if (m_ref == -INFINITY) m_ref = top;
+            }
+            uint32_t pk[64];
+            float sum;
+#pragma unroll 1
+            for (int again = 0; again < 2; ++again) {
+                uint32_t sr[2][32];
+                tmem_ld32_issue(tS, sr[0]);
                 const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
                 const uint64_t nsub2 = f2(-sub, -sub), c2 = f2(p.scale_log2, p.scale_log2);
                 uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t pk[16];
+                    tmem_wait_ld32(sr[c & 1]);
+                    if (c < 3) tmem_ld32_issue(tS + 32u * (c + 1), sr[(c + 1) & 1]);
+                    const uint32_t w = kMasked ? seen(c) : 0u;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
+                        uint64_t fa = c2, fb = c2;
+                        if constexpr (k8) {
+                            const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                            fa = f2(f.x, f.y);
+                            fb = f2(f.z, f.w);
+                        }
                         float e[4];
-                        un_f2(fma_f2(f2(__uint_as_float(sc[c][j]), __uint_as_float(sc[c][j + 1])), c2, nsub2), e[0], e[1]);
-                        un_f2(fma_f2(f2(__uint_as_float(sc[c][j + 2]), __uint_as_float(sc[c][j + 3])), c2, nsub2), e[2], e[3]);
+                        un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j]), __uint_as_float(sr[c & 1][j + 1])), fa, nsub2), e[0], e[1]);
+                        un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j + 2]), __uint_as_float(sr[c & 1][j + 3])), fb, nsub2), e[2], e[3]);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
+                        for (int q = 0; q < 4; ++q) {
+                            if (kMasked && !((w >> (j + q)) & 1u)) e[q] = -INFINITY;
+                            e[q] = ex2_approx(e[q]);
+                        }
                         acc[0] = add_f2(acc[0], f2(e[0], e[1]));
                         acc[1] = add_f2(acc[1], f2(e[2], e[3]));
-                        pk[j / 2] = pack_bf16x2(e[0], e[1]);
-                        pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                        if constexpr (k8) {
+                            const float4 f = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
+                            un_f2(mul_f2(f2(e[0], e[1]), f2(f.x, f.y)), e[0], e[1]);
+                            un_f2(mul_f2(f2(e[2], e[3]), f2(f.z, f.w)), e[2], e[3]);
+                        }
+                        pk[16 * c + j / 2] = pack_bf16x2(e[0], e[1]);
+                        pk[16 * c + j / 2 + 1] = pack_bf16x2(e[2], e[3]);
                     }
-                    tmem_st16(tS + 16u * c, pk);
                 }
-                float s0, s1, s2, s3;
-                un_f2(acc[0], s0, s1);
-                un_f2(acc[1], s2, s3);
-                l_run += (s0 + s1) + (s2 + s3);
-                tmem_wait_st();
-                return;
-            }
-            // 8-bit caches have fewer registers to spare: two readings.  Pass 1: the row's largest score.
-            float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            uint32_t sr[2][32];
-            tmem_ld32_issue(tS, sr[0]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                tmem_wait_ld32(sr[c & 1]);
-                tmem_ld32_issue(tS + 32u * ((c + 1) & 3), sr[(c + 1) & 1]);   // after chunk 3: chunk 0 for pass 2
-                const uint32_t w = kMasked ? seen(c) : 0u;
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    float v[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = __uint_as_float(sr[c & 1][j + q]);
-                    if constexpr (k8) {
-                        const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
-                        un_f2(mul_f2(f2(v[0], v[1]), f2(f.x, f.y)), v[0], v[1]);
-                        un_f2(mul_f2(f2(v[2], v[3]), f2(f.z, f.w)), v[2], v[3]);
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (kMasked && !((w >> (j + q)) & 1u)) v[q] = -INFINITY;
-                    }
-                    t4[0] = max3(t4[0], v[0], v[1]);
-                    t4[1] = max3(t4[1], v[2], v[3]);
+                float s0, s1;
+                un_f2(add_f2(acc[0], acc[1]), s0, s1);
+                sum = s0 + s1;
+                const bool over = sum > kTileSumMax;
+                if (!__any_sync(0xffffffffu, over)) break;
+                // O is at rest (see s_full): to the new reference, and the tile once more
+                const float top = largest();
+                const float alpha = over ? ex2_approx(m_ref - top) : 1.0f;
+                if (over) {
+                    m_ref = top;
+                    l_run *= alpha;
                 }
-            }
-            float top = fmaxf(t4[0], t4[1]);
-            if constexpr (!k8) top *= p.scale_log2;
-            float alpha = 1.0f;
-            bool rescale = false;
-            if (start) {
-                m_ref = top;
-            } else if (top > m_ref + kRescaleLog2) {
-                alpha = ex2_approx(m_ref - top);   // 0 where nothing was seen so far
-                m_ref = top;
-                l_run *= alpha;
-                rescale = true;
-            }
-            if (__any_sync(0xffffffffu, rescale)) {
-                tmem_wait_ld32(sr[0]);
                 rescale_o(alpha);
-                tmem_ld32_issue(tS, sr[0]);
             }
-            // pass 2: P into S's first 64 columns; chunk c's 16 columns lie in chunks already read
-            const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
-            const uint64_t nsub2 = f2(-sub, -sub), c2 = f2(p.scale_log2, p.scale_log2);
-            uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+            l_run += sum;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                tmem_wait_ld32(sr[c & 1]);
-                if (c < 3) tmem_ld32_issue(tS + 32u * (c + 1), sr[(c + 1) & 1]);
-                const uint32_t w = kMasked ? seen(c) : 0u;
-                uint32_t pk[16];
+                uint32_t out16[16];
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    uint64_t fa = c2, fb = c2;
-                    if constexpr (k8) {
-                        const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
-                        fa = f2(f.x, f.y);
-                        fb = f2(f.z, f.w);
-                    }
-                    float e[4];
-                    un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j]), __uint_as_float(sr[c & 1][j + 1])), fa, nsub2), e[0], e[1]);
-                    un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j + 2]), __uint_as_float(sr[c & 1][j + 3])), fb, nsub2), e[2], e[3]);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (kMasked && !((w >> (j + q)) & 1u)) e[q] = -INFINITY;
-                        e[q] = ex2_approx(e[q]);
-                    }
-                    acc[0] = add_f2(acc[0], f2(e[0], e[1]));
-                    acc[1] = add_f2(acc[1], f2(e[2], e[3]));
-                    if constexpr (k8) {
-                        const float4 f = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
-                        un_f2(mul_f2(f2(e[0], e[1]), f2(f.x, f.y)), e[0], e[1]);
-                        un_f2(mul_f2(f2(e[2], e[3]), f2(f.z, f.w)), e[2], e[3]);
-                    }
-                    pk[j / 2] = pack_bf16x2(e[0], e[1]);
-                    pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
-                }
-                tmem_st16(tS + 16u * c, pk);
+                for (int j = 0; j < 16; ++j) out16[j] = pk[16 * c + j];
+                tmem_st16(tS + 16u * c, out16);
             }
-            float s0, s1, s2, s3;
-            un_f2(acc[0], s0, s1);
-            un_f2(acc[1], s2, s3);
-            l_run += (s0 + s1) + (s2 + s3);
             tmem_wait_st();
         };
 
@@ -1325,7 +1268,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         wait(&tail->s_full[l], cnt & 1u);
                         ++cnt;
                         fence_after();
-                        if (active) row_tile(masked_t, s.t0 + ti, ti, pos, bits, ti == ti0, m_ref, l_run);
+                        if (active) row_tile(masked_t, s.t0 + ti, ti, pos, bits, m_ref, l_run);
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&tail->p_full[l]);
