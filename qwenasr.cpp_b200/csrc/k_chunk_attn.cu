@@ -102,7 +102,7 @@ struct Start {
 };
 
 struct alignas(16) Tail {
-    uint64_t q_full[2], seg_done[2];       // of a segment, by its parity
+    uint64_t q_full[2], q_free[2];         // of a segment, by its parity; q_free: its areas
     uint64_t full[5], empty[5], s_full[2], p_full[2], o_full[2], epi_done, mma_done;
     uint64_t scale_full[4], raw_full[3], raw_empty[3];   // 8-bit
     float2 ml[2][128];                     // (reference, sum) of each lane's rows, at a segment's end
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tail->q_full[b], 1);
-            mbar_init(&tail->seg_done[b], 1);
+            mbar_init(&tail->q_free[b], 1);
             mbar_init(&tail->s_full[b], 1);
             mbar_init(&tail->p_full[b], 4);      // warps
             mbar_init(&tail->o_full[b], 1);
@@ -638,37 +638,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             };
             int id_next = page_id(s.t0);
             const int g2 = uniform(2 * s.g), row0 = uniform(s.row0);
-            if (kv == 0) {
-                // Q takes the areas of an earlier segment: the one before last has always ended (its Q barrier is
-                // reused), the last one if they meet.
-                const uint32_t prev = areas;
-                areas = q_areas(s.mode, prev);
-                const bool meets = (areas & prev) && !(s.mode == kThin && was_thin);
-                was_thin = s.mode == kThin;
-                if (seg >= 2) ok = wait(&tail->seg_done[seg & 1u], ((seg - 2) >> 1) & 1u);
-                if (ok && meets && seg >= 1) ok = wait(&tail->seg_done[(seg - 1) & 1u], ((seg - 1) >> 1) & 1u);
-                // Q rows: row 2 i + h.  Rows behind the unit's queries are some other row's or zero: rows (in thin mode
-                // columns) of S that no one reads.
-                if (ok && leader) {
-                    uint64_t *bar = &tail->q_full[seg & 1u];
-                    if (s.mode == kThin) {
-                        const uint32_t dst = smem_u32(smem) + kThinQ + (seg & 1u) * kThinQBytes;
-                        mbar_arrive_expect_tx(bar, 2 * kThinQBlk);
-                        tma_load_3d(dst, &maps.q_thin, 0, g2, row0, bar);
-                        tma_load_3d(dst + kThinQBlk, &maps.q_thin, 64, g2, row0, bar);
-                    } else {
-                        const int tiles = s.pair() ? 2 : 1;
-                        mbar_arrive_expect_tx(bar, tiles * kTileBytes);
-                        for (int j = 0; j < tiles; ++j) {
-                            const uint32_t dst = smem_u32(smem) + (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes);
-                            tma_load_3d(dst, &maps.q, 0, g2, row0 + j * kQueries, bar);
-                            tma_load_3d(dst + kBlkBytes, &maps.q, 64, g2, row0 + j * kQueries, bar);
-                        }
-                    }
-                }
-                if (!ok) break;
-                if (leader) tail->q_issued = seg + 1;
-            }
             // One thread issues a tile's boxes from warp-uniform page ids: as many lanes issuing one each took 90 cycles
             // a box.
             auto load = [&](int kt, uint32_t u, int id) -> bool {
@@ -728,10 +697,43 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 __syncwarp();
                 return true;
             };
+            auto load_q = [&]() -> bool {
+                // Q takes the areas of an earlier segment: the one before last has always ended (its Q barrier is
+                // reused), the last one if they meet.
+                const uint32_t prev = areas;
+                areas = q_areas(s.mode, prev);
+                const bool meets = (areas & prev) && !(s.mode == kThin && was_thin);
+                was_thin = s.mode == kThin;
+                if (seg >= 2) ok = wait(&tail->q_free[seg & 1u], ((seg - 2) >> 1) & 1u);
+                if (ok && meets && seg >= 1) ok = wait(&tail->q_free[(seg - 1) & 1u], ((seg - 1) >> 1) & 1u);
+                // Q rows: row 2 i + h.  Rows behind the unit's queries are some other row's or zero: rows (in thin mode
+                // columns) of S that no one reads.
+                if (!ok) return false;
+                if (leader) {
+                    uint64_t *bar = &tail->q_full[seg & 1u];
+                    if (s.mode == kThin) {
+                        const uint32_t dst = smem_u32(smem) + kThinQ + (seg & 1u) * kThinQBytes;
+                        mbar_arrive_expect_tx(bar, 2 * kThinQBlk);
+                        tma_load_3d(dst, &maps.q_thin, 0, g2, row0, bar);
+                        tma_load_3d(dst + kThinQBlk, &maps.q_thin, 64, g2, row0, bar);
+                    } else {
+                        const int tiles = s.pair() ? 2 : 1;
+                        mbar_arrive_expect_tx(bar, tiles * kTileBytes);
+                        for (int j = 0; j < tiles; ++j) {
+                            const uint32_t dst = smem_u32(smem) + (s.pair() ? j * kTileBytes : (areas >> 1) * kTileBytes);
+                            tma_load_3d(dst, &maps.q, 0, g2, row0 + j * kQueries, bar);
+                            tma_load_3d(dst + kBlkBytes, &maps.q, 64, g2, row0 + j * kQueries, bar);
+                        }
+                    }
+                }
+                if (leader) tail->q_issued = seg + 1;
+                return ok;
+            };
             for (int i = 0; ok && i < n; ++i) {
                 const int id = checked(id_next, s.t0 + i);
                 if (i + 1 < n) id_next = page_id(s.t0 + i + 1);
                 ok = load(s.t0 + i, u0 + (kv ? item_of_v(i, n) : item_of_k(i)), id);
+                if (i == 0 && kv == 0) ok = ok && load_q();   // its area may have to be waited for; the tile need not
             }
             u0 += 2 * n;
             ++seg;
@@ -740,7 +742,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         // ================= MMA issuer =================
         bool ok = true;
         const bool leader = elect_one();
-        uint32_t u0 = 0, p_cnt0 = 0, p_cnt1 = 0, seg = 0, areas = 0;
+        // Tiles are consumed in the order they are loaded: a running stage and its phase.
+        uint32_t st = 0, ph = 0, p_cnt0 = 0, p_cnt1 = 0, seg = 0, areas = 0;
         const uint32_t tmem_u = uniform(tmem), smem_u = uniform(smem_u32(smem));
         auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, wait_bar(bar, par, failed)) != 0; };
         while (ok && walk.next(p, s)) {
@@ -749,9 +752,18 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             const bool pair = mode == kPair, thin = mode == kThin;
             areas = uniform(q_areas(mode, areas));
             if (!(ok = wait(&tail->q_full[seg & 1u], (seg >> 1) & 1u))) break;
-            auto stage_of = [&](uint32_t item) { return (u0 + item) % L::kStages; };
-            auto wait_item = [&](uint32_t item) {
-                return wait(&tail->full[(u0 + item) % L::kStages], ((u0 + item) / L::kStages) & 1u);
+            // the next tile, once it is there
+            auto next_tile = [&](uint32_t &stage) -> bool {
+                stage = st;
+                const bool there = wait(&tail->full[st], ph);
+                if (++st == L::kStages) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+                return there;
+            };
+            auto q_done = [&]() {
+                if (leader) commit(&tail->q_free[seg & 1u]);
             };
             const uint32_t aQ0 = smem_u + (thin ? kThinQ + (seg & 1u) * kThinQBytes : (pair ? 0u : (areas >> 1) * kTileBytes));
             const uint32_t id_thin = idesc_thin(cols);
@@ -803,57 +815,53 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 __syncwarp();
                 return true;
             };
+            uint32_t kt = 0, vt = 0;
             // first tiles
-            if (!(ok = wait_item(0))) break;
-            if (pair) {
-                if (n0 > 0) issue_s(0, stage_of(0));
-                issue_s(1, stage_of(0));
-                free_stage(stage_of(0));
-            } else {
-                issue_s(0, stage_of(0));
-                free_stage(stage_of(0));
-                if (n > 1) {
-                    if (!(ok = wait_item(1))) break;
-                    issue_s(1, stage_of(1));
-                    free_stage(stage_of(1));
-                }
+            if (!(ok = next_tile(kt))) break;
+            if (n0 > 0) issue_s(0, kt);
+            if (pair) issue_s(1, kt);
+            free_stage(kt);
+            if (!pair && n > 1) {
+                if (!(ok = next_tile(kt))) break;
+                issue_s(1, kt);
+                free_stage(kt);
             }
+            if (!thin && n <= (pair ? 1 : 2)) q_done();   // Q is read by S alone; thin mode's area holds P, too
             // the previous segment's O has been read
             if (seg > 0 && !(ok = wait(&tail->epi_done, (seg - 1) & 1u))) break;
-            for (int i = 0; ok && i < n; ++i) {
-                const uint32_t vi = item_of_v(i, n);
-                if (!(ok = wait_item(vi))) break;
-                if (pair) {
-                    const uint32_t ki = item_of_k(i + 1);
+            if (pair) {
+                for (int i = 0; i < n; ++i) {
+                    const bool more = i + 1 < n;
+                    if (more && !(ok = next_tile(kt))) break;
+                    if (!(ok = next_tile(vt))) break;
                     if (i < n0) {
-                        if (!(ok = issue_pv(0, stage_of(vi), i > 0, i + 1 == n0))) break;
-                        if (i + 1 < n0) {
-                            if (!(ok = wait_item(ki))) break;
-                            issue_s(0, stage_of(ki));
-                        }
+                        if (!(ok = issue_pv(0, vt, i > 0, i + 1 == n0))) break;
+                        if (i + 1 < n0) issue_s(0, kt);
                     }
-                    if (!(ok = issue_pv(1, stage_of(vi), i > 0, i + 1 == n))) break;
-                    free_stage(stage_of(vi));
-                    if (i + 1 < n) {
-                        if (!(ok = wait_item(ki))) break;
-                        issue_s(1, stage_of(ki));
-                        free_stage(stage_of(ki));
+                    if (!(ok = issue_pv(1, vt, i > 0, i + 1 == n))) break;
+                    free_stage(vt);
+                    if (more) {
+                        issue_s(1, kt);
+                        free_stage(kt);
+                        if (i + 2 == n) q_done();
                     }
-                } else {
+                }
+            } else {
+                for (int i = 0; i < n; ++i) {
                     const int l = i & 1;
-                    if (!(ok = issue_pv(l, stage_of(vi), i > 1, i + 2 >= n))) break;
-                    free_stage(stage_of(vi));
+                    if (!(ok = next_tile(vt))) break;
+                    if (!(ok = issue_pv(l, vt, i > 1, i + 2 >= n))) break;
+                    free_stage(vt);
                     if (i + 2 < n) {
-                        const uint32_t ki = item_of_k(i + 2);
-                        if (!(ok = wait_item(ki))) break;
-                        issue_s(l, stage_of(ki));
-                        free_stage(stage_of(ki));
+                        if (!(ok = next_tile(kt))) break;
+                        issue_s(l, kt);
+                        free_stage(kt);
+                        if (!thin && i + 3 == n) q_done();
                     }
                 }
             }
             if (!ok) break;
-            if (leader) commit(&tail->seg_done[seg & 1u]);
-            u0 += 2 * n;
+            if (thin) q_done();
             ++seg;
         }
         if (!ok) {
@@ -1015,31 +1023,33 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 const float top = largest();
                 if (m_ref == -INFINITY) m_ref = top;
             }
+            constexpr int kWide = k8 ? 16 : 32;   // columns read at a time (8-bit caches have fewer registers)
             uint32_t pk[64];
             float sum;
 #pragma unroll 1
             for (int again = 0; again < 2; ++again) {
-                uint32_t sr[2][32];
-                tmem_ld32_issue(tS, sr[0]);
+                uint32_t sr[2][kWide];
+                tmem_ld_cols<kWide>(tS, sr[0]);
                 const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
                 const uint64_t nsub2 = f2(-sub, -sub), c2 = f2(p.scale_log2, p.scale_log2);
                 uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_wait_ld32(sr[c & 1]);
-                    if (c < 3) tmem_ld32_issue(tS + 32u * (c + 1), sr[(c + 1) & 1]);
-                    const uint32_t w = kMasked ? seen(c) : 0u;
+                for (int c = 0; c < kKeys / kWide; ++c) {
+                    uint32_t (&v)[kWide] = sr[c & 1];
+                    tmem_wait_ld_regs<kWide>(v);
+                    if (c + 1 < kKeys / kWide) tmem_ld_cols<kWide>(tS + kWide * (c + 1), sr[(c + 1) & 1]);
+                    const uint32_t w = kMasked ? seen(c * kWide / 32) >> (c * kWide % 32) : 0u;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
+                    for (int j = 0; j < kWide; j += 4) {
                         uint64_t fa = c2, fb = c2;
                         if constexpr (k8) {
-                            const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                            const float4 f = *reinterpret_cast<const float4 *>(ks + kWide * c + j);
                             fa = f2(f.x, f.y);
                             fb = f2(f.z, f.w);
                         }
                         float e[4];
-                        un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j]), __uint_as_float(sr[c & 1][j + 1])), fa, nsub2), e[0], e[1]);
-                        un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j + 2]), __uint_as_float(sr[c & 1][j + 3])), fb, nsub2), e[2], e[3]);
+                        un_f2(fma_f2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), fa, nsub2), e[0], e[1]);
+                        un_f2(fma_f2(f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), fb, nsub2), e[2], e[3]);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             if (kMasked && !((w >> (j + q)) & 1u)) e[q] = -INFINITY;
@@ -1048,12 +1058,12 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         acc[0] = add_f2(acc[0], f2(e[0], e[1]));
                         acc[1] = add_f2(acc[1], f2(e[2], e[3]));
                         if constexpr (k8) {
-                            const float4 f = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
+                            const float4 f = *reinterpret_cast<const float4 *>(vs + kWide * c + j);
                             un_f2(mul_f2(f2(e[0], e[1]), f2(f.x, f.y)), e[0], e[1]);
                             un_f2(mul_f2(f2(e[2], e[3]), f2(f.z, f.w)), e[2], e[3]);
                         }
-                        pk[16 * c + j / 2] = pack_bf16x2(e[0], e[1]);
-                        pk[16 * c + j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                        pk[kWide / 2 * c + j / 2] = pack_bf16x2(e[0], e[1]);
+                        pk[kWide / 2 * c + j / 2 + 1] = pack_bf16x2(e[2], e[3]);
                     }
                 }
                 float s0, s1;
