@@ -27,8 +27,8 @@
 // (one CTA per SM), wherever the cuts fall; a unit cut into pieces leaves (max,
 // sum, unnormalised O) per piece in the workspace, and a second kernel joins
 // them in order.  The cuts follow from the lengths in device memory alone, so a
-// captured call serves other lengths.  Every role walks its CTA's segments by
-// the same arithmetic.
+// captured call serves other lengths.  One warp walks a CTA's segments and
+// hands them to the others through a ring in shared memory.
 //
 // Softmax.  P is taken against a reference that moves only when a tile exceeds
 // it by more than 2^kRescaleLog2 (then O and the sum are rescaled); P, the sum
@@ -43,6 +43,8 @@
 // 2700 cycles per 32 KB and bounded every shape; the MMA warp runs its loop as
 // a whole and elects a thread only to issue, so that descriptors stay in
 // uniform registers.
+// What a segment's start and end cost was mostly code fetched afresh, so
+// those parts are kept short or rolled up.
 // All waits bounded; a softmax warp whose wait ran out goes on without waiting,
 // so that the named barriers stay matched.
 #include <cuda.h>
@@ -82,7 +84,8 @@ template <bool k8> struct Layout {
     static constexpr int kConvWarp = 8, kConvWarps = k8 ? 8 : 0;
     static constexpr int kMmaWarp = kConvWarp + kConvWarps;
     static constexpr int kLoadWarp = kMmaWarp + 1;   // K tiles and Q; the next one V tiles
-    static constexpr int kWarps = kMmaWarp + 4, kThreads = 32 * kWarps;   // whole warpgroups: one warp is idle
+    static constexpr int kPlanWarp = kMmaWarp + 3;
+    static constexpr int kWarps = kMmaWarp + 4, kThreads = 32 * kWarps;
     // Registers: the launch gives every thread kRegs (65536 over the threads, in eights); the warpgroups then trade
     // them.  bf16: 12 warps x 168 = 2 x 4 x 208 + 4 x 80 (and some left); 8-bit: 20 x 96 = 2 x 4 x 144 + 3 x 4 x 64.
     static constexpr int kSoftmaxRegs = k8 ? 144 : 208, kOtherRegs = k8 ? 64 : 80, kRegs = k8 ? 96 : 168;
@@ -94,28 +97,6 @@ template <bool k8> struct Layout {
     static constexpr size_t kTailOff = kRawScaleOff + kRaw * 2 * kKeys * sizeof(float);
 };
 constexpr int kMaxWarps = 20;
-
-// Where a CTA's part starts: the entry, the largest end before it, the work before it.
-struct Start {
-    int i, runmax;
-    long long pre;
-};
-
-struct alignas(16) Tail {
-    uint64_t q_full[2], q_free[2];         // of a segment, by its parity; q_free: its areas
-    uint64_t full[5], empty[5], s_full[2], p_full[2], o_full[2], epi_done, mma_done;
-    uint64_t scale_full[4], raw_full[3], raw_empty[3];   // 8-bit
-    float2 ml[2][128];                     // (reference, sum) of each lane's rows, at a segment's end
-    float thin_ref[2][32];                 // thin mode: the lane's reference per column
-    long long warp_sum[kMaxWarps];
-    int warp_max[kMaxWarps];
-    Start from;
-    uint32_t tmem;
-    int failed;
-    uint32_t issued[5], q_issued;          // last item of each ring slot and last Q, plus one
-};
-static_assert(Layout<false>::kTailOff + sizeof(Tail) <= 227 * 1024, "bf16 layout");
-static_assert(Layout<true>::kTailOff + sizeof(Tail) <= 227 * 1024, "8-bit layout");
 
 // ---- work split ----
 
@@ -163,13 +144,11 @@ __device__ __forceinline__ Entry load_entry(const ChunkAttendParams &p, int i, i
     return e;
 }
 
-struct Segment {
-    int slot, g, row0, nq, q0pos, base, len_end;   // query rows row0.., the first at position q0pos; keys [0, len_end)
-    int t0, t1;                                    // key tiles
-    int mode, cols;                                // cols: thin mode's columns (2 nq rounded up to 16)
-    bool first, last;                              // holds the unit's first / last tile
-    long long ustart;                              // position of the unit's first tile in the work
-    int tiles;                                     // of the unit
+struct alignas(16) Segment {
+    int slot, g, row0, nq;            // query rows row0 ..
+    int q0pos, base, len_end, mode;   // position of the first query, of the chunk's first token; keys [0, len_end)
+    int t0, t1, cols, first;          // key tiles; thin mode's columns (2 nq rounded up to 16); holds the first tile
+    int last, c_last, pad[2];         // holds the unit's last tile; the CTA that does, where this piece is the first
     __device__ __forceinline__ bool pair() const { return mode == kPair; }
 };
 
@@ -179,14 +158,43 @@ __device__ __forceinline__ uint32_t q_areas(int mode, uint32_t prev) {
     return mode == kPair ? 3u : (mode == kThin ? 2u : (prev & 1u ? 2u : 1u));
 }
 
+// Where a CTA's part starts: the entry, the largest end before it, the work before it.
+struct Start {
+    int i, runmax;
+    long long pre;
+};
+
+constexpr int kSegRing = 4;
+struct alignas(16) Tail {
+    Segment seg[kSegRing];
+    // (reference, sum) of each lane's rows or columns at a segment's end.  Thin mode uses 0..31 and, for its column
+    // sums by warp, 64..127; of lane 0, 32..63 for the columns' factors.  Before the first segment: the scan's scratch.
+    float2 ml[2][128];
+    float thin_ref[2][32];                 // thin mode: the lane's reference per column
+    uint64_t q_full[2], q_free[2];         // of a segment, by its parity; q_free: its areas
+    uint64_t full[5], empty[5], s_full[2], p_full[2], o_full[2], epi_done, mma_done;
+    uint64_t seg_full[kSegRing], seg_empty[kSegRing];
+    uint64_t scale_full[4], raw_full[3], raw_empty[3];   // 8-bit
+    Start from;
+    uint32_t tmem;
+    int failed;
+    uint32_t issued[5], q_issued;          // last item of each ring slot and last Q, plus one
+};
+static_assert(Layout<false>::kTailOff + sizeof(Tail) <= 227 * 1024, "bf16 layout");
+static_assert(Layout<true>::kTailOff + sizeof(Tail) <= 227 * 1024, "8-bit layout");
+
+// Goes through the segments of a CTA's part [x, x1) of the work.
 struct Walk {
     Entry e;
     int i, runmax, g, b;
-    long long x, x1, ustart;
+    long long x, x1, ustart, parts, total;
 
-    __device__ __forceinline__ void start(const ChunkAttendParams &p, const Start &f, long long from, long long to) {
+    __device__ __forceinline__ void start(const ChunkAttendParams &p, const Start &f, long long from, long long to,
+                                          long long n_parts, long long sum) {
         x = from;
         x1 = to;
+        parts = n_parts;
+        total = sum;
         if (x >= x1) return;
         i = f.i;
         runmax = f.runmax;
@@ -213,11 +221,11 @@ struct Walk {
                 ustart = x;
             }
             const int cnt = block_queries(e, b), w = cnt > kQueries ? 2 : 1;
-            s.tiles = block_tiles(e, b);
+            const int tiles = block_tiles(e, b);
             // tile t is the CTA's that holds position `at` + w t
-            const long long at = ustart + kUnitCost, uend = at + static_cast<long long>(w) * s.tiles;
+            const long long at = ustart + kUnitCost, uend = at + static_cast<long long>(w) * tiles;
             s.t0 = static_cast<int>(max(0ll, x - at + w - 1) >> (w - 1));
-            s.t1 = static_cast<int>(min(static_cast<long long>(s.tiles), max(0ll, x1 - at + w - 1) >> (w - 1)));
+            s.t1 = static_cast<int>(min(static_cast<long long>(tiles), max(0ll, x1 - at + w - 1) >> (w - 1)));
             s.slot = e.slot;
             s.g = g;
             s.row0 = e.first + b * 2 * kQueries;
@@ -229,8 +237,8 @@ struct Walk {
             s.mode = w == 2 ? kPair : (cnt > kThinQueries ? kAlternate : kThin);
             s.cols = cnt > 8 ? 32 : 16;
             s.first = s.t0 == 0;
-            s.last = s.t1 == s.tiles;
-            s.ustart = at;
+            s.last = s.t1 == tiles;
+            s.c_last = static_cast<int>(quot((at + static_cast<long long>(w) * (tiles - 1) + 1) * parts - 1, total));
             x = uend;
             ustart = uend;
             if (++b == e.nb) {
@@ -474,6 +482,10 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             mbar_init(&tail->full[b], k8 ? 32 * L::kConvWarps : 1);
             mbar_init(&tail->empty[b], 1);
         }
+        for (int b = 0; b < kSegRing; ++b) {
+            mbar_init(&tail->seg_full[b], 1);
+            mbar_init(&tail->seg_empty[b], L::kWarps - 1);   // the other warps
+        }
         mbar_init(&tail->epi_done, 8);      // warps
         mbar_init(&tail->mma_done, 1);
         for (int b = 0; b < L::kScaleRing; ++b) mbar_init(&tail->scale_full[b], 128);
@@ -555,11 +567,13 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             const int v = __shfl_up_sync(0xffffffffu, mx_inc, o);
             if (lane >= o) mx_inc = max(mx_inc, v);
         }
-        if (lane == 31) tail->warp_max[warp] = mx_inc;
+        long long *const warp_sum = reinterpret_cast<long long *>(tail->ml[0]);
+        int *const warp_max = reinterpret_cast<int *>(tail->ml[1]);
+        if (lane == 31) warp_max[warp] = mx_inc;
         __syncthreads();
         int runmax = __shfl_up_sync(0xffffffffu, mx_inc, 1);
         if (lane == 0) runmax = 0;
-        for (int w = 0; w < warp; ++w) runmax = max(runmax, tail->warp_max[w]);
+        for (int w = 0; w < warp; ++w) runmax = max(runmax, warp_max[w]);
         long long cost[kPer], sum = 0;
         int maxes[kPer];
 #pragma unroll
@@ -580,12 +594,12 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             const long long v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
-        if (lane == 31) tail->warp_sum[warp] = inc;
+        if (lane == 31) warp_sum[warp] = inc;
         __syncthreads();
         long long pre = inc - sum;
         for (int w = 0; w < L::kWarps; ++w) {
-            if (w < warp) pre += tail->warp_sum[w];
-            total += tail->warp_sum[w];
+            if (w < warp) pre += warp_sum[w];
+            total += warp_sum[w];
         }
         part_of();
 #pragma unroll
@@ -601,14 +615,47 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     fence_after();
     const uint32_t tmem = tail->tmem;
 
-    Walk walk;
     Segment s;
+    uint32_t seg_no = 0;
+    // The next segment (the same for every warp); false behind the last one.
+    auto next_segment = [&]() -> bool {
+        const uint32_t b = seg_no % kSegRing;
+        const bool there = __all_sync(0xffffffffu, wait_bar(&tail->seg_full[b], (seg_no / kSegRing) & 1u, failed));
+        if (!there) {
+            if (lane == 0 && !*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 18);
+            *failed = 1;
+            return false;
+        }
+        s = tail->seg[b];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tail->seg_empty[b]);
+        ++seg_no;
+        return s.slot >= 0;
+    };
 
     if (warp >= L::kMmaWarp) {
     set_regs_down<L::kOtherRegs>();
-    walk.start(p, from, x0, x1);
-    if (warp == L::kWarps - 1) {
-        // idle: fills the warpgroup
+    if (warp == L::kPlanWarp) {
+        // ================= plan: the segments, one after the other =================
+        if (lane == 0) {
+            Walk walk;
+            walk.start(p, from, x0, x1, parts, total);
+            bool more = true;
+            for (uint32_t k = 0; more; ++k) {
+                const uint32_t b = k % kSegRing;
+                Segment next;
+                more = walk.next(p, next);
+                if (!more) next.slot = -1;
+                if (!wait_bar(&tail->seg_empty[b], ((k / kSegRing) & 1u) ^ 1u, failed)) {
+                    if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 17);
+                    *failed = 1;
+                    break;
+                }
+                tail->seg[b] = next;
+                mbar_arrive(&tail->seg_full[b]);
+            }
+        }
+        __syncwarp();
     } else if (warp >= L::kLoadWarp) {
         // ================= loads =================
         const int kv = warp - L::kLoadWarp;
@@ -626,7 +673,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         const bool leader = elect_one();
         const uint32_t smem_u = uniform(smem_u32(smem));
         const int ps = lane & 7;   // this lane's page of a tile
-        while (ok && walk.next(p, s) && !*failed) {
+        while (ok && next_segment() && !*failed) {
             const int *const pt = p.page_table + static_cast<size_t>(s.slot) * p.maxp;
             const int key_pages = (s.len_end + kPageTokens - 1) / kPageTokens, n = uniform(s.t1 - s.t0);
             auto page_id = [&](int kt) { return kt * 8 + ps < key_pages ? load_early(pt + kt * 8 + ps) : p.n_pages; };
@@ -746,7 +793,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         uint32_t st = 0, ph = 0, p_cnt0 = 0, p_cnt1 = 0, seg = 0, areas = 0;
         const uint32_t tmem_u = uniform(tmem), smem_u = uniform(smem_u32(smem));
         auto wait = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, wait_bar(bar, par, failed)) != 0; };
-        while (ok && walk.next(p, s)) {
+        while (ok && next_segment()) {
             // warp-uniform copies: what the descriptors are made of
             const int n = uniform(s.t1 - s.t0), n0 = uniform(lane_tiles(s, 0)), mode = uniform(s.mode), cols = uniform(s.cols);
             const bool pair = mode == kPair, thin = mode == kThin;
@@ -877,7 +924,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     }
     } else if (k8 && warp >= L::kConvWarp) {
         set_regs_down<L::kOtherRegs>();
-        walk.start(p, from, x0, x1);
         // ================= 8-bit codes -> bf16 tiles =================
         // Thread: 16 codes (piece c of 8) of rows t / 8 + 32 m.
         constexpr int kRows = 128 * 8 / (32 * (k8 ? L::kConvWarps : 8));
@@ -943,7 +989,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             ++u;
             return true;
         };
-        while (ok && walk.next(p, s)) {
+        while (ok && next_segment()) {
             const int n = s.t1 - s.t0;
             ok = convert(s.t0, 0, tile_no);
             for (int i = 0; ok && i < n; ++i) {
@@ -954,7 +1000,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         }
     } else {
         set_regs_up<L::kSoftmaxRegs>();
-        walk.start(p, from, x0, x1);
         // ================= softmax and epilogue of lane l =================
         const int l = warp >> 2, quad = warp & 3, r = 32 * quad + lane;   // r: TMEM lane
         const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * quad) << 16);
@@ -984,7 +1029,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         // Key tile kt (the ti-th of the segment) of pair and alternate mode; thread = query row.
         // No maximum is taken as long as the row's reference will do: the tile's sum, which is needed anyway, tells
         // when one of its terms has grown past 2^kRescaleLog2.  P is stored only then, since it lies over S.
-        auto row_tile = [&](auto masked_t, int kt, int ti, int pos, unsigned long long bits, float &m_ref, float &l_run) {
+        auto row_tile = [&](auto masked_t, int kt, int ti, int pos, unsigned long long bits, bool start, float &m_ref,
+                            float &l_run) {
             constexpr bool kMasked = decltype(masked_t)::value;
             const uint32_t slot = (tile_no + ti) % L::kScaleRing;
             const float *ks = scale_ring + slot * 2 * kKeys, *vs = ks + kKeys;
@@ -1019,10 +1065,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 }
                 return top;
             };
-            if (__any_sync(0xffffffffu, m_ref == -INFINITY)) {   // a row that has seen nothing yet
-                const float top = largest();
-                if (m_ref == -INFINITY) m_ref = top;
-            }
             constexpr int kWide = k8 ? 16 : 32;   // columns read at a time (8-bit caches have fewer registers)
             uint32_t pk[64];
             float sum;
@@ -1069,16 +1111,19 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 float s0, s1;
                 un_f2(add_f2(acc[0], acc[1]), s0, s1);
                 sum = s0 + s1;
-                const bool over = sum > kTileSumMax;
+                // A row without a reference starts from 0 if that serves.
+                const bool unset = m_ref == -INFINITY;
+                const bool over = sum > kTileSumMax || (unset && sum < 1.0f / kTileSumMax);
+                if (unset && !over) m_ref = 0.0f;
                 if (!__any_sync(0xffffffffu, over)) break;
                 // O is at rest (see s_full): to the new reference, and the tile once more
                 const float top = largest();
-                const float alpha = over ? ex2_approx(m_ref - top) : 1.0f;
+                const float alpha = over && !unset ? ex2_approx(m_ref - top) : 1.0f;
                 if (over) {
                     m_ref = top;
                     l_run *= alpha;
                 }
-                rescale_o(alpha);
+                if (!start) rescale_o(alpha);   // the first P V of a segment writes O anew
             }
             l_run += sum;
 #pragma unroll
@@ -1130,8 +1175,29 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         }
                     }
                 }
-                bool move = k == 0;
-                if (k > 0) {
+                bool move;
+                if (k == 0) {
+                    // References start from 0 if that serves: no score past 2^kRescaleLog2, and every column has one
+                    // that is not far below.
+                    uint32_t fair = 0;
+                    float over = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) {
+                        fair |= x[j] > -kRescaleLog2 ? 1u << j : 0u;
+                        over = fmaxf(over, x[j]);
+                    }
+                    fair = __reduce_or_sync(0xffffffffu, fair);
+                    if (__any_sync(0xffffffffu, over > kRescaleLog2)) fair = 0x80000000u;   // the mark for it
+                    uint32_t *const words = reinterpret_cast<uint32_t *>(sP);
+                    if (lane == 0) words[quad] = fair;
+                    if (r < kCols) ref[r] = 0.0f;
+                    bar_sync(kBarLane + l, 128);
+                    const uint4 w = *reinterpret_cast<const uint4 *>(words);
+                    constexpr uint32_t kAll = kCols == 32 ? 0xffffffffu : (1u << kCols % 32) - 1u;
+                    const uint32_t every = w.x | w.y | w.z | w.w;
+                    move = every != kAll || w.x == 0x80000000u || w.y == 0x80000000u || w.z == 0x80000000u || w.w == 0x80000000u;
+                    bar_sync(kBarLane + l, 128);        // the scratch is read
+                } else {
                     float over = -INFINITY;
 #pragma unroll
                     for (int j = 0; j < kCols; ++j) over = fmaxf(over, x[j] - ref[j]);   // -inf - -inf: NaN, not the maximum
@@ -1220,40 +1286,47 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             fence_before();
             bar_sync(kBarBoth, 256);
             fence_after();
-            // dims as threads: lane l finishes columns [l kCols / 2, (l + 1) kCols / 2)
+            // A column's factors for the lanes' O, by one thread each; the piece's (reference, sum) where it is one.
             const bool whole = s.first && s.last;
-            constexpr int kHalf = kCols / 2;
-            uint32_t o0[kHalf], o1[kHalf];
-            tmem_ld_cols<kHalf>(lane_addr + kTmemO + l * kHalf, o0);
-            tmem_wait_ld_regs<kHalf>(o0);
-            if (n > 1) {
-                tmem_ld_cols<kHalf>(lane_addr + kTmemO + 128u + l * kHalf, o1);
-                tmem_wait_ld_regs<kHalf>(o1);
-            }
             const size_t piece = 2 * static_cast<size_t>(blockIdx.x) + (s.first ? 1 : 0);
             const int real = *failed ? 0 : 2 * s.nq;
-#pragma unroll
-            for (int j = 0; j < kHalf; ++j) {
-                const int col = l * kHalf + j;
-                if (col >= real) continue;
-                const float2 v0 = tail->ml[0][col], v1 = n > 1 ? tail->ml[1][col] : make_float2(-INFINITY, 0.0f);
+            float2 *const factor = &tail->ml[0][32];
+            if (l == 0 && r < kCols) {
+                const float2 v0 = tail->ml[0][r], v1 = n > 1 ? tail->ml[1][r] : make_float2(-INFINITY, 0.0f);
                 const float m = fmaxf(v0.x, v1.x);
                 const float a0 = v0.y > 0.0f ? ex2_approx(v0.x - m) : 0.0f, a1 = v1.y > 0.0f ? ex2_approx(v1.x - m) : 0.0f;
                 const float sum = a0 * v0.y + a1 * v1.y;
-                float o = a0 > 0.0f ? a0 * __uint_as_float(o0[j]) : 0.0f;
-                if (a1 > 0.0f) o += a1 * __uint_as_float(o1[j]);
-                if (whole) {
-                    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-                    reinterpret_cast<__nv_bfloat16 *>(p.out)[static_cast<size_t>(s.row0 + (col >> 1)) * kQDim +
-                                                             (2 * s.g + (col & 1)) * kHeadDim + r] = __float2bfloat16_rn(o * inv);
-                } else {
-                    p.part_o[piece * (kPieceRows * kHeadDim) + col * kHeadDim + r] = o;
-                    if (r == 0) p.part_ml[piece * kPieceRows + col] = make_float2(m, sum);
+                const float norm = whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+                factor[r] = make_float2(a0 * norm, a1 * norm);
+                if (!whole && r < real) p.part_ml[piece * kPieceRows + r] = make_float2(m, sum);
+            }
+            bar_sync(kBarBoth, 256);
+            // dims as threads: lane l finishes columns [l kCols / 2, (l + 1) kCols / 2), eight at a time
+#pragma unroll 1
+            for (int c = 0; c < kCols / 2; c += 8) {
+                const int col0 = l * (kCols / 2) + c;
+                uint32_t o0[8], o1[8];
+                tmem_ld_cols<8>(lane_addr + kTmemO + col0, o0);
+                tmem_ld_cols<8>(lane_addr + kTmemO + 128u + col0, o1);   // of a single tile's segment: not used
+                tmem_wait_ld_regs<8>(o0);
+                tmem_wait_ld_regs<8>(o1);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int col = col0 + j;
+                    const float2 f = factor[col];
+                    float o = f.x != 0.0f ? f.x * __uint_as_float(o0[j]) : 0.0f;
+                    if (f.y != 0.0f) o += f.y * __uint_as_float(o1[j]);
+                    if (col >= real) continue;
+                    if (whole)
+                        reinterpret_cast<__nv_bfloat16 *>(p.out)[static_cast<size_t>(s.row0 + (col >> 1)) * kQDim +
+                                                                 (2 * s.g + (col & 1)) * kHeadDim + r] = __float2bfloat16_rn(o);
+                    else
+                        p.part_o[piece * (kPieceRows * kHeadDim) + col * kHeadDim + r] = o;
                 }
             }
         };
 
-        while (walk.next(p, s)) {
+        while (next_segment()) {
             const int n = s.t1 - s.t0;
             if (s.mode == kThin) {
                 if (s.cols == 16) thin_segment(std::integral_constant<int, 16>{});
@@ -1278,7 +1351,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         wait(&tail->s_full[l], cnt & 1u);
                         ++cnt;
                         fence_after();
-                        if (active) row_tile(masked_t, s.t0 + ti, ti, pos, bits, m_ref, l_run);
+                        if (active) row_tile(masked_t, s.t0 + ti, ti, pos, bits, ti == ti0, m_ref, l_run);
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&tail->p_full[l]);
@@ -1354,9 +1427,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&tail->epi_done);
             if (s.first && !s.last && tid == 0) {
-                // the unit goes on in the CTAs up to the one that holds its last tile
-                const long long last = s.ustart + static_cast<long long>(s.pair() ? 2 : 1) * (s.tiles - 1);
-                p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.mode, static_cast<int>(quot((last + 1) * parts - 1, total))};
+                p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.mode, s.c_last};   // goes on elsewhere
             }
             tile_no += n;
         }
