@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                                         (t >> 4) * (2 * kPageTokens) + (t & 15);
                 const bool live = kt * kKeys + t < s.len_end;
                 const uint32_t ring = tile % L::kScaleRing;
-                scale_ring[ring * 2 * kKeys + t] = live ? rs[0] * p.scale_log2 : 0.0f;
+                scale_ring[ring * 2 * kKeys + t] = live ? rs[0] * p.scale_log2 : 1.0f;   // (masked: times -infinity)
                 scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kPageTokens] : 0.0f;
                 mbar_arrive(&tail->scale_full[ring]);
             }
@@ -1029,24 +1029,36 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         // Key tile kt (the ti-th of the segment) of pair and alternate mode; thread = query row.
         // No maximum is taken as long as the row's reference will do: the tile's sum, which is needed anyway, tells
         // when one of its terms has grown past 2^kRescaleLog2.  P is stored only then, since it lies over S.
-        auto row_tile = [&](auto masked_t, int kt, int ti, int pos, unsigned long long bits, bool start, float &m_ref,
-                            float &l_run) {
-            constexpr bool kMasked = decltype(masked_t)::value;
+        auto row_tile = [&](int kt, int ti, bool masked, int pos, unsigned long long bits, bool start, float &m_ref, float &l_run) {
             const uint32_t slot = (tile_no + ti) % L::kScaleRing;
             const float *ks = scale_ring + slot * 2 * kKeys, *vs = ks + kKeys;
             if constexpr (k8) wait(&tail->scale_full[slot], ((tile_no + ti) / L::kScaleRing) & 1u);
-            // keys of chunk c (32 keys) that the row sees
-            auto seen = [&](int c) -> uint32_t {
-                const int k0 = kt * kKeys + 32 * c;
-                if (!p.mask) {
-                    const int d = pos - k0;
-                    return d >= 31 ? 0xffffffffu : (d < 0 ? 0u : (2u << d) - 1u);
+            if (masked) {
+                // Scores of keys that the row does not see: -infinity, in place.  (The few tiles that need it share the
+                // code of the rest.)
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32_issue(tS + 32u * c, v);
+                    const int k0 = kt * kKeys + 32 * c;
+                    uint32_t seen;
+                    if (!p.mask) {
+                        const int d = pos - k0;
+                        seen = d >= 31 ? 0xffffffffu : (d < 0 ? 0u : (2u << d) - 1u);
+                    } else {
+                        const int d = k0 - s.base;   // chunk token of the first key
+                        seen = d <= -32 ? 0xffffffffu
+                                        : (d < 0 ? ((1u << -d) - 1u) | static_cast<uint32_t>(bits << -d)
+                                                 : (d < 64 ? static_cast<uint32_t>(bits >> d) : 0u));
+                    }
+                    tmem_wait_ld32(v);
+                    float x[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] = (seen >> j) & 1u ? __uint_as_float(v[j]) : -INFINITY;
+                    tmem_st32(tS + 32u * c, x);
                 }
-                const int d = k0 - s.base;   // chunk token of the first key
-                if (d <= -32) return 0xffffffffu;
-                if (d < 0) return ((1u << -d) - 1u) | static_cast<uint32_t>(bits << -d);
-                return d < 64 ? static_cast<uint32_t>(bits >> d) : 0u;
-            };
+                tmem_wait_st();
+            }
             // the row's largest score of the tile (rare: rolled up)
             auto largest = [&]() -> float {
                 float top = -INFINITY;
@@ -1055,13 +1067,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     uint32_t v[32];
                     tmem_ld32_issue(tS + 32u * c, v);
                     tmem_wait_ld32(v);
-                    const uint32_t w = kMasked ? seen(c) : 0xffffffffu;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float x = __uint_as_float(v[j]) * (k8 ? ks[32 * c + j] : p.scale_log2);
-                        if (kMasked && !((w >> j) & 1u)) x = -INFINITY;
-                        top = fmaxf(top, x);
-                    }
+                    for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]) * (k8 ? ks[32 * c + j] : p.scale_log2));
                 }
                 return top;
             };
@@ -1080,7 +1087,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     uint32_t (&v)[kWide] = sr[c & 1];
                     tmem_wait_ld_regs<kWide>(v);
                     if (c + 1 < kKeys / kWide) tmem_ld_cols<kWide>(tS + kWide * (c + 1), sr[(c + 1) & 1]);
-                    const uint32_t w = kMasked ? seen(c * kWide / 32) >> (c * kWide % 32) : 0u;
 #pragma unroll
                     for (int j = 0; j < kWide; j += 4) {
                         uint64_t fa = c2, fb = c2;
@@ -1093,10 +1099,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                         un_f2(fma_f2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), fa, nsub2), e[0], e[1]);
                         un_f2(fma_f2(f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), fb, nsub2), e[2], e[3]);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            if (kMasked && !((w >> (j + q)) & 1u)) e[q] = -INFINITY;
-                            e[q] = ex2_approx(e[q]);
-                        }
+                        for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
                         acc[0] = add_f2(acc[0], f2(e[0], e[1]));
                         acc[1] = add_f2(acc[1], f2(e[2], e[3]));
                         if constexpr (k8) {
@@ -1344,22 +1347,18 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     if (s.nq < 64) bits &= (1ull << s.nq) - 1ull;
                 }
                 float m_ref = -INFINITY, l_run = 0.0f;
-                // tiles that every row sees whole come first
+                // tiles below `clear` are seen whole by every row
                 const int step = s.pair() ? 1 : 2, ti0 = s.pair() ? 0 : l, clear = ((p.mask ? s.base : pos_min + 1) >> 7) - s.t0;
-                auto tiles = [&](auto masked_t, int ti, int end) {
-                    for (; ti < end; ti += step) {
-                        wait(&tail->s_full[l], cnt & 1u);
-                        ++cnt;
-                        fence_after();
-                        if (active) row_tile(masked_t, s.t0 + ti, ti, pos, bits, ti == ti0, m_ref, l_run);
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&tail->p_full[l]);
-                    }
-                    return ti;
-                };
-                const int end = ti0 + step * mine;
-                tiles(std::true_type{}, tiles(std::false_type{}, ti0, min(clear, end)), end);
+#pragma unroll 1
+                for (int k = 0, ti = ti0; k < mine; ++k, ti += step) {
+                    wait(&tail->s_full[l], cnt & 1u);
+                    ++cnt;
+                    fence_after();
+                    if (active) row_tile(s.t0 + ti, ti, ti >= clear, pos, bits, k == 0, m_ref, l_run);
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tail->p_full[l]);
+                }
                 if (mine > 0) wait(&tail->o_full[l], seg_cnt++ & 1u);
                 const bool whole = s.first && s.last;
                 float a0 = 1.0f, a1 = 0.0f, m_tot = m_ref, l_tot = l_run;
