@@ -72,7 +72,9 @@ enum Mode { kThin = 0, kAlternate = 1, kPair = 2 };
 constexpr uint32_t kThinQ = kTileBytes, kThinQBytes = 8192, kThinQBlk = 4096;
 constexpr uint32_t kThinP = kTileBytes + 16384, kThinPBytes = 8192;
 constexpr int kMinCost = 2;                // least work of a CTA (tiles of alternate mode)
-constexpr int kUnitCost = 2;               // work of a unit besides its tiles
+// Work of a unit besides its tiles.  Measured: 2640 cycles a tile and 9000 a unit in thin mode, 3260 a tile (counted
+// double) and 9200 a unit in pair mode.
+constexpr int kUnitCost = 3, kPairUnitCost = 6;
 constexpr int kPieceRows = 256;            // rows of a workspace piece (pair mode: both lanes)
 
 // K and V tiles in flight; 8-bit caches hold raw tiles besides (kRaw) and the
@@ -139,7 +141,7 @@ __device__ __forceinline__ Entry load_entry(const ChunkAttendParams &p, int i, i
         // full blocks end on a multiple of 128 queries: T_b = p0 + b + 1
         e.head_cost = 2 * (full * p0 + full * (full + 1) / 2) +
                       static_cast<long long>(block_queries(e, e.nb - 1) > kQueries ? 2 : 1) * block_tiles(e, e.nb - 1) +
-                      static_cast<long long>(kUnitCost) * e.nb;
+                      kPairUnitCost * full + (block_queries(e, e.nb - 1) > kQueries ? kPairUnitCost : kUnitCost);
     }
     return e;
 }
@@ -204,7 +206,7 @@ struct Walk {
         rem -= g * e.head_cost;
         b = 0;
         while (b < e.nb - 1) {
-            const long long c = 2ll * block_tiles(e, b) + kUnitCost;
+            const long long c = 2ll * block_tiles(e, b) + kPairUnitCost;
             if (rem < c) break;
             rem -= c;
             ++b;
@@ -223,7 +225,7 @@ struct Walk {
             const int cnt = block_queries(e, b), w = cnt > kQueries ? 2 : 1;
             const int tiles = block_tiles(e, b);
             // tile t is the CTA's that holds position `at` + w t
-            const long long at = ustart + kUnitCost, uend = at + static_cast<long long>(w) * tiles;
+            const long long at = ustart + (w == 2 ? kPairUnitCost : kUnitCost), uend = at + static_cast<long long>(w) * tiles;
             s.t0 = static_cast<int>(max(0ll, x - at + w - 1) >> (w - 1));
             s.t1 = static_cast<int>(min(static_cast<long long>(tiles), max(0ll, x1 - at + w - 1) >> (w - 1)));
             s.slot = e.slot;
