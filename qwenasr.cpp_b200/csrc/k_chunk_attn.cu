@@ -64,7 +64,9 @@ constexpr int kQueries = 64;               // queries of a query tile
 constexpr uint32_t kTmemCols = 512;        // S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512)
 constexpr uint32_t kTmemO = 256;
 constexpr float kRescaleLog2 = 30.0f;
-constexpr float kTileSumMax = 1099511627776.0f;   // 2^40: some term of a tile's sum is past 2^33, and none past 2^40 if not
+// Pair and alternate mode: bounds of a sum of 32 or 128 terms, 2^60 and 2^40.  Past kSumMove the reference moves before
+// the next tile; only past kSumMax it has to at once.  (O then stays finite for values below 2^67.)
+constexpr float kSumMax = 1152921504606846976.0f, kSumMove = 1099511627776.0f;
 constexpr int kThinQueries = 16;           // most queries of thin mode
 enum Mode { kThin = 0, kAlternate = 1, kPair = 2 };
 // The two 32 KB areas before the stages: a query tile each, or area 1 split
@@ -445,7 +447,7 @@ __device__ __forceinline__ uint32_t item_of_k(int i) { return i == 0 ? 0 : 2 * i
 __device__ __forceinline__ uint32_t item_of_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
 
 // Tensor maps: the layer's pool as [page][K|V x head x token][dim] with boxes of
-// 16 tokens (bf16: x 64 dims, 128-byte swizzle; 8-bit: x 128 bytes), and q as
+// 16 tokens x 128 bytes, swizzled, and q as
 // [row][head][dim] with boxes of 64 and 16 rows x 2 heads x 64 dims.
 struct Maps {
     CUtensorMap kv, q, q_thin;
@@ -927,28 +929,26 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     } else if (k8 && warp >= L::kConvWarp) {
         set_regs_down<L::kOtherRegs>();
         // ================= 8-bit codes -> bf16 tiles =================
-        // Thread: 16 codes (piece c of 8) of rows t / 8 + 32 m.
-        constexpr int kRows = 128 * 8 / (32 * (k8 ? L::kConvWarps : 8));
-        const int t = tid - 32 * L::kConvWarp, c = t & 7;
-        // Pieces 4..7 (the second 64 dims) store their odd half first, so that no two of 8 lanes meet in a bank; they
-        // read their halves in that order, too.
-        const int odd = (c >> 2) & 1;
+        // Thread: a 16-byte piece of rows row + 32 m.  Eight lanes take four pieces of rows r and r ^ 5, which differ in
+        // bits 0 and 2: swizzled, neither their 16-byte reads (pieces c ^ r) nor their writes (2 c ^ r, 2 c + 1 ^ r)
+        // meet in a bank.
+        constexpr int kRows = 4;
+        constexpr uint32_t kRing = k8 ? L::kRaw : 1;
+        const int t = tid - 32 * L::kConvWarp, c = (lane & 3) | ((lane >> 1) & 4), pair_no = (t >> 5) * 2 + (lane >> 4);
+        const int row0 = (pair_no >> 2) * 8 + (pair_no & 3), row = lane & 4 ? row0 ^ 5 : row0;
+        const uint32_t src0 = smem_u32(smem) + static_cast<uint32_t>(L::kRawOff) + swz(row, c);
+        const uint32_t dst0 = smem_u32(smem) + static_cast<uint32_t>(L::kStageOff) + (c >> 2) * kBlkBytes + swz(row, 2 * (c & 3));
+        const uint32_t dst1 = dst0 ^ 16u;
         uint32_t u = 0, tile_no = 0;
         bool ok = true;
-        auto convert = [&](int kt, int kv, uint32_t tile) -> bool {
-            const uint32_t stage = u % L::kStages, slot = u % (k8 ? L::kRaw : 1);
-            if (!wait_bar(&tail->raw_full[slot], (u / (k8 ? L::kRaw : 1)) & 1u, failed)) {
-                if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 20);
-                *failed = 1;
-                return false;
-            }
-            const uint8_t *const raw = smem + L::kRawOff + slot * (kTileBytes / 2) + t * 16;
-            uint2 in[kRows][2];   // all of it before the first store: the compiler cannot tell the tiles apart
-#pragma unroll
-            for (int m = 0; m < kRows; ++m) {
-                in[m][0] = *reinterpret_cast<const uint2 *>(raw + m * 4096 + odd * 8);
-                in[m][1] = *reinterpret_cast<const uint2 *>(raw + m * 4096 + (odd ^ 1) * 8);
-            }
+        auto give_up = [&](int where) {
+            if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, where);
+            *failed = 1;
+            return false;
+        };
+        auto item = [&](int kt, int kv, uint32_t tile) -> bool {
+            const uint32_t slot = u % kRing, stage = u % L::kStages;
+            if (!wait_bar(&tail->raw_full[slot], (u / kRing) & 1u, failed)) return give_up(1 << 20);
             if (kv == 0 && t < kKeys) {   // a K tile brings both scales of its tokens; none behind the last one
                 const float *const rs = reinterpret_cast<const float *>(smem + L::kRawScaleOff) + slot * 2 * kKeys +
                                         (t >> 4) * (2 * kPageTokens) + (t & 15);
@@ -958,34 +958,42 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kPageTokens] : 0.0f;
                 mbar_arrive(&tail->scale_full[ring]);
             }
-            mbar_arrive(&tail->raw_empty[slot]);
-            if (!wait_bar(&tail->empty[stage], ((u / L::kStages) & 1u) ^ 1u, failed)) {
-                if (!*failed) report_error(p.err, kErrWaitTimeout, kWhereChunkAttn, blockIdx.x, 1 << 19);
-                *failed = 1;
-                return false;
-            }
-            uint8_t *const blk = smem + L::kStageOff + stage * kTileBytes + (c >> 2) * kBlkBytes;
-            uint8_t *const d0 = blk + swz(t >> 3, 2 * (c & 3) + odd), *const d1 = blk + swz(t >> 3, 2 * (c & 3) + (odd ^ 1));
+            if (!wait_bar(&tail->empty[stage], ((u / L::kStages) & 1u) ^ 1u, failed)) return give_up(1 << 19);
             auto codes = [&](auto int8_t_) {
                 constexpr bool kInt8 = decltype(int8_t_)::value;
+                uint32_t src = src0 + slot * (kTileBytes / 2), to0 = dst0 + stage * kTileBytes, to1 = dst1 + stage * kTileBytes;
+#pragma unroll 1
+                for (int m = 0; m < kRows; m += 2) {
+                    uint4 in[2];
 #pragma unroll
-                for (int m = 0; m < kRows; ++m) {
+                    for (int k = 0; k < 2; ++k)
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(in[k].x), "=r"(in[k].y), "=r"(in[k].z), "=r"(in[k].w)
+                                     : "r"(src + k * 4096));
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        uint32_t h[4];
-                        if constexpr (kInt8) {
-                            u8x4_to_bf16(in[m][k].x, h[0], h[1]);
-                            u8x4_to_bf16(in[m][k].y, h[2], h[3]);
-                        } else {
-                            e4m3x4_to_bf16(in[m][k].x, h[0], h[1]);
-                            e4m3x4_to_bf16(in[m][k].y, h[2], h[3]);
+                        const uint32_t ws[4] = {in[k].x, in[k].y, in[k].z, in[k].w};
+                        uint32_t h[8];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            if constexpr (kInt8) u8x4_to_bf16(ws[w], h[2 * w], h[2 * w + 1]);
+                            else e4m3x4_to_bf16(ws[w], h[2 * w], h[2 * w + 1]);
                         }
-                        *reinterpret_cast<uint4 *>((k ? d1 : d0) + m * 4096) = make_uint4(h[0], h[1], h[2], h[3]);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to0 + k * 4096), "r"(h[0]), "r"(h[1]), "r"(h[2]),
+                                     "r"(h[3])
+                                     : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to1 + k * 4096), "r"(h[4]), "r"(h[5]), "r"(h[6]),
+                                     "r"(h[7])
+                                     : "memory");
                     }
+                    src += 8192;
+                    to0 += 8192;
+                    to1 += 8192;
                 }
             };
             if (kv == 1 && p.v_int8) codes(std::true_type{});
             else codes(std::false_type{});
+            mbar_arrive(&tail->raw_empty[slot]);
             fence_async_smem();
             mbar_arrive(&tail->full[stage]);
             ++u;
@@ -993,10 +1001,10 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         };
         while (ok && next_segment()) {
             const int n = s.t1 - s.t0;
-            ok = convert(s.t0, 0, tile_no);
+            ok = item(s.t0, 0, tile_no);
             for (int i = 0; ok && i < n; ++i) {
-                if (i + 1 < n) ok = convert(s.t0 + i + 1, 0, tile_no + i + 1);
-                ok = ok && convert(s.t0 + i, 1, tile_no + i);
+                if (i + 1 < n) ok = item(s.t0 + i + 1, 0, tile_no + i + 1);
+                ok = ok && item(s.t0 + i, 1, tile_no + i);
             }
             tile_no += n;
         }
@@ -1028,13 +1036,48 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             tmem_wait_st();
         };
 
+        // Rare: at chunk c (32 keys) of a tile, rows with `bad` take the largest score of the chunks from c on for their
+        // reference; what they have so far, P of the earlier chunks included, is rescaled.
+        auto outgrown = [&](int c, bool bad, bool unset, bool start, const float *ks, float &m_ref, float &l_run, float &tile_sum) {
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int k = c; k < 4; ++k) {
+                uint32_t v[32];
+                tmem_ld32_issue(tS + 32u * k, v);
+                tmem_wait_ld32(v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]) * (k8 ? ks[32 * k + j] : p.scale_log2));
+            }
+            const float alpha = bad && !unset ? ex2_approx(m_ref - top) : 1.0f;
+            if (bad) m_ref = top;
+            l_run *= alpha;
+            tile_sum *= alpha;
+#pragma unroll 1
+            for (int k = 0; k < c; ++k) {
+                uint32_t v[16];
+                tmem_ld_cols<16>(tS + 16u * k, v);
+                tmem_wait_ld_regs<16>(v);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = pack_bf16x2(bf16lo(v[j]) * alpha, bf16hi(v[j]) * alpha);
+                tmem_st16(tS + 16u * k, v);
+            }
+            tmem_wait_st();
+            if (!start) rescale_o(alpha);   // the first P V of a segment writes O anew
+        };
+
         // Key tile kt (the ti-th of the segment) of pair and alternate mode; thread = query row.
-        // No maximum is taken as long as the row's reference will do: the tile's sum, which is needed anyway, tells
-        // when one of its terms has grown past 2^kRescaleLog2.  P is stored only then, since it lies over S.
-        auto row_tile = [&](int kt, int ti, bool masked, int pos, unsigned long long bits, bool start, float &m_ref, float &l_run) {
+        // No maximum is taken: the sums, which are needed anyway, tell when the reference will not do any more.
+        auto row_tile = [&](int kt, int ti, bool masked, int pos, unsigned long long bits, bool start, float &m_ref, float &l_run,
+                            float &want) {
             const uint32_t slot = (tile_no + ti) % L::kScaleRing;
             const float *ks = scale_ring + slot * 2 * kKeys, *vs = ks + kKeys;
             if constexpr (k8) wait(&tail->scale_full[slot], ((tile_no + ti) / L::kScaleRing) & 1u);
+            if (__any_sync(0xffffffffu, want != m_ref)) {   // O is at rest (see s_full)
+                const float alpha = want != m_ref ? ex2_approx(m_ref - want) : 1.0f;
+                m_ref = want;
+                l_run *= alpha;
+                rescale_o(alpha);
+            }
             if (masked) {
                 // Scores of keys that the row does not see: -infinity, in place.  (The few tiles that need it share the
                 // code of the rest.)
@@ -1061,83 +1104,115 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 }
                 tmem_wait_st();
             }
-            // the row's largest score of the tile (rare: rolled up)
-            auto largest = [&]() -> float {
-                float top = -INFINITY;
+            const uint64_t c2 = f2(p.scale_log2, p.scale_log2);
+            float tile_sum = 0.0f;
+            uint32_t sr[2][32];
+            tmem_ld32_issue(tS, sr[0]);
+            if constexpr (!k8) {
+                // The whole tile unrolled and P stored at its end, over S that is intact until then (rolled up, as
+                // below, a 2048-row piece took 336 us instead of 297; with the converting warps beside it, the short
+                // code wins: 102 us against 106 for 8-bit contexts, 188 against 202 for ragged segments).
+                uint32_t pk[4][16];
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32_issue(tS + 32u * c, v);
-                    tmem_wait_ld32(v);
+                for (int again = 0; again < 2; ++again) {
+                    const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
+                    const uint64_t nsub2 = f2(-sub, -sub);
+                    uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]) * (k8 ? ks[32 * c + j] : p.scale_log2));
-                }
-                return top;
-            };
-            constexpr int kWide = k8 ? 16 : 32;   // columns read at a time (8-bit caches have fewer registers)
-            uint32_t pk[64];
-            float sum;
-#pragma unroll 1
-            for (int again = 0; again < 2; ++again) {
-                uint32_t sr[2][kWide];
-                tmem_ld_cols<kWide>(tS, sr[0]);
-                const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
-                const uint64_t nsub2 = f2(-sub, -sub), c2 = f2(p.scale_log2, p.scale_log2);
-                uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_wait_ld32(sr[c & 1]);
+                        if (c < 3) tmem_ld32_issue(tS + 32u * (c + 1), sr[(c + 1) & 1]);
 #pragma unroll
-                for (int c = 0; c < kKeys / kWide; ++c) {
-                    uint32_t (&v)[kWide] = sr[c & 1];
-                    tmem_wait_ld_regs<kWide>(v);
-                    if (c + 1 < kKeys / kWide) tmem_ld_cols<kWide>(tS + kWide * (c + 1), sr[(c + 1) & 1]);
+                        for (int j = 0; j < 32; j += 4) {
+                            float e[4];
+                            un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j]), __uint_as_float(sr[c & 1][j + 1])), c2, nsub2), e[0], e[1]);
+                            un_f2(fma_f2(f2(__uint_as_float(sr[c & 1][j + 2]), __uint_as_float(sr[c & 1][j + 3])), c2, nsub2), e[2], e[3]);
 #pragma unroll
-                    for (int j = 0; j < kWide; j += 4) {
-                        uint64_t fa = c2, fb = c2;
-                        if constexpr (k8) {
-                            const float4 f = *reinterpret_cast<const float4 *>(ks + kWide * c + j);
-                            fa = f2(f.x, f.y);
-                            fb = f2(f.z, f.w);
+                            for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
+                            acc[0] = add_f2(acc[0], f2(e[0], e[1]));
+                            acc[1] = add_f2(acc[1], f2(e[2], e[3]));
+                            pk[c][j / 2] = pack_bf16x2(e[0], e[1]);
+                            pk[c][j / 2 + 1] = pack_bf16x2(e[2], e[3]);
                         }
-                        float e[4];
-                        un_f2(fma_f2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), fa, nsub2), e[0], e[1]);
-                        un_f2(fma_f2(f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), fb, nsub2), e[2], e[3]);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
-                        acc[0] = add_f2(acc[0], f2(e[0], e[1]));
-                        acc[1] = add_f2(acc[1], f2(e[2], e[3]));
-                        if constexpr (k8) {
-                            const float4 f = *reinterpret_cast<const float4 *>(vs + kWide * c + j);
-                            un_f2(mul_f2(f2(e[0], e[1]), f2(f.x, f.y)), e[0], e[1]);
-                            un_f2(mul_f2(f2(e[2], e[3]), f2(f.z, f.w)), e[2], e[3]);
-                        }
-                        pk[kWide / 2 * c + j / 2] = pack_bf16x2(e[0], e[1]);
-                        pk[kWide / 2 * c + j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                    }
+                    float s0, s1;
+                    un_f2(add_f2(acc[0], acc[1]), s0, s1);
+                    tile_sum = s0 + s1;
+                    const bool unset = m_ref == -INFINITY, bad = tile_sum > kSumMove || (unset && tile_sum < 1.0f / kSumMove);
+                    if (!__any_sync(0xffffffffu, bad)) break;
+                    if (again == 0) {
+                        outgrown(0, bad, unset, start, ks, m_ref, l_run, tile_sum);
+                        tmem_ld32_issue(tS, sr[0]);
                     }
                 }
-                float s0, s1;
-                un_f2(add_f2(acc[0], acc[1]), s0, s1);
-                sum = s0 + s1;
-                // A row without a reference starts from 0 if that serves.
-                const bool unset = m_ref == -INFINITY;
-                const bool over = sum > kTileSumMax || (unset && sum < 1.0f / kTileSumMax);
-                if (unset && !over) m_ref = 0.0f;
-                if (!__any_sync(0xffffffffu, over)) break;
-                // O is at rest (see s_full): to the new reference, and the tile once more
-                const float top = largest();
-                const float alpha = over && !unset ? ex2_approx(m_ref - top) : 1.0f;
-                if (over) {
-                    m_ref = top;
-                    l_run *= alpha;
+                if (m_ref == -INFINITY && tile_sum > 0.0f) m_ref = 0.0f;
+                l_run += tile_sum;
+                want = m_ref;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_st16(tS + 16u * c, pk[c]);
+                tmem_wait_st();
+                return;
+            }
+#pragma unroll 1
+            for (int cc = 0; cc < 4; cc += 2) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = cc + h;   // 32 keys
+                    tmem_wait_ld32(sr[h]);
+                    if (h == 0 || cc == 0) tmem_ld32_issue(tS + 32u * (c + 1), sr[h ^ 1]);
+                    uint32_t pk[16];
+                    float sum;
+#pragma unroll 1
+                    for (int again = 0; again < 2; ++again) {
+                        const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
+                        const uint64_t nsub2 = f2(-sub, -sub);
+                        uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            uint64_t fa = c2, fb = c2;
+                            if constexpr (k8) {
+                                const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                                fa = f2(f.x, f.y);
+                                fb = f2(f.z, f.w);
+                            }
+                            float e[4];
+                            un_f2(fma_f2(f2(__uint_as_float(sr[h][j]), __uint_as_float(sr[h][j + 1])), fa, nsub2), e[0], e[1]);
+                            un_f2(fma_f2(f2(__uint_as_float(sr[h][j + 2]), __uint_as_float(sr[h][j + 3])), fb, nsub2), e[2], e[3]);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
+                            acc[0] = add_f2(acc[0], f2(e[0], e[1]));
+                            acc[1] = add_f2(acc[1], f2(e[2], e[3]));
+                            if constexpr (k8) {
+                                const float4 f = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
+                                un_f2(mul_f2(f2(e[0], e[1]), f2(f.x, f.y)), e[0], e[1]);
+                                un_f2(mul_f2(f2(e[2], e[3]), f2(f.z, f.w)), e[2], e[3]);
+                            }
+                            pk[j / 2] = pack_bf16x2(e[0], e[1]);
+                            pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                        }
+                        float s0, s1;
+                        un_f2(add_f2(acc[0], acc[1]), s0, s1);
+                        sum = s0 + s1;
+                        // Before P goes over S: has a term outgrown the range, or is a row's first sum too small to tell
+                        // its terms from zero (or has it none)?
+                        const bool unset = m_ref == -INFINITY, bad = sum > kSumMax || (unset && c == 0 && sum < 1.0f / kSumMax);
+                        if (!__any_sync(0xffffffffu, bad)) break;
+                        if (again == 0) {
+                            tmem_wait_ld32(sr[h ^ 1]);
+                            outgrown(c, bad, unset, start, ks, m_ref, l_run, tile_sum);
+                            if (h == 0 || cc == 0) tmem_ld32_issue(tS + 32u * (c + 1), sr[h ^ 1]);
+                        }
+                    }
+                    if (m_ref == -INFINITY && sum > 0.0f) m_ref = 0.0f;
+                    tile_sum += sum;
+                    tmem_st16(tS + 16u * c, pk);
                 }
-                if (!start) rescale_o(alpha);   // the first P V of a segment writes O anew
             }
-            l_run += sum;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t out16[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) out16[j] = pk[16 * c + j];
-                tmem_st16(tS + 16u * c, out16);
-            }
+            l_run += tile_sum;
+            // The range is wide; a row that leaves its middle moves its reference before the next tile.
+            want = m_ref;
+            if (tile_sum > kSumMove || (tile_sum < 1.0f / kSumMove && tile_sum > 0.0f && l_run == tile_sum))
+                want += static_cast<float>((__float_as_int(tile_sum) >> 23) - 127);
             tmem_wait_st();
         };
 
@@ -1348,7 +1423,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     bits = p.mask[s.row0 + qoff + i];
                     if (s.nq < 64) bits &= (1ull << s.nq) - 1ull;
                 }
-                float m_ref = -INFINITY, l_run = 0.0f;
+                float m_ref = -INFINITY, l_run = 0.0f, want = -INFINITY;   // want: m_ref from the next tile on
                 // tiles below `clear` are seen whole by every row
                 const int step = s.pair() ? 1 : 2, ti0 = s.pair() ? 0 : l, clear = ((p.mask ? s.base : pos_min + 1) >> 7) - s.t0;
 #pragma unroll 1
@@ -1356,7 +1431,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     wait(&tail->s_full[l], cnt & 1u);
                     ++cnt;
                     fence_after();
-                    if (active) row_tile(s.t0 + ti, ti, ti >= clear, pos, bits, k == 0, m_ref, l_run);
+                    if (active) row_tile(s.t0 + ti, ti, ti >= clear, pos, bits, k == 0, m_ref, l_run, want);
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&tail->p_full[l]);
@@ -1530,7 +1605,7 @@ bool encode_maps(Maps *m, const ChunkAttendParams &p, bool k8) {
             return false;
     }
     return encode_3d(&m->kv, k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.pool, kv_dims, kv_strides,
-                     kv_box, k8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B) &&
+                     kv_box, CU_TENSOR_MAP_SWIZZLE_128B) &&
            encode_3d(&m->q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.q, q_dims, q_strides, q_box, CU_TENSOR_MAP_SWIZZLE_128B) &&
            encode_3d(&m->q_thin, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.q, q_dims, q_strides, thin_box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
