@@ -480,10 +480,9 @@ class Decoder:
     def chunk_append(self, layer, n, slots_ptr, pos_ptr, axes_ptr, sections, interleaved, qkv_ptr, q_out_ptr, q_dtype,
                      stream=None):
         """kv_append with a rotary position per axis (axes_ptr: [3][n]); q out as q_dtype (F32 or BF16)."""
-        sec = _i32(sections)
-        if sec.shape != (3,):
+        if len(sections) != 3:
             raise ValueError("sections: three counts of rotation pairs")
-        self._check(lib.qkv_chunk_append(self.h, layer, n, slots_ptr, pos_ptr, axes_ptr, _ptr(sec, C.c_int32),
+        self._check(lib.qkv_chunk_append(self.h, layer, n, slots_ptr, pos_ptr, axes_ptr, (C.c_int32 * 3)(*sections),
                                          int(interleaved), qkv_ptr, q_out_ptr, q_dtype, stream))
 
     def chunk_attend(self, layer, n, slots_ptr, starts_ptr, lens_ptr, rows, mask_ptr, q_ptr, out_ptr, stream=None):
