@@ -1855,7 +1855,7 @@ int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
         else axis = i < sections[0] ? 0 : (i < sections[0] + sections[1] ? 1 : 2);
         p.axis_of[i] = static_cast<unsigned char>(axis);
     }
-    CK(launch_chunk_append(p, h->rt.kv_dtype, static_cast<cudaStream_t>(stream)));
+    CK(launch_chunk_append(p, h->rt.kv_dtype, h->num_sms, static_cast<cudaStream_t>(stream)));
     h->launches += 1;
     return QKV_OK;
 }
