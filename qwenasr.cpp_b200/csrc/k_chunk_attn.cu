@@ -75,8 +75,9 @@ constexpr uint32_t kThinQ = kTileBytes, kThinQBytes = 8192, kThinQBlk = 4096;
 constexpr uint32_t kThinP = kTileBytes + 16384, kThinPBytes = 8192;
 constexpr int kMinCost = 2;                // least work of a CTA (tiles of alternate mode)
 // Work of a unit besides its tiles.  Measured: 2640 cycles a tile and 9000 a unit in thin mode, 3260 a tile (counted
-// double) and 9200 a unit in pair mode.
-constexpr int kUnitCost = 3, kPairUnitCost = 6;
+// double) and 9200 a unit in pair mode.  Of (2, 3), (3, 6) and (5, 9), the last gave 64 draft trees 95 us against 99 and
+// 97, ragged segments 187 against 194 and 196, and a 2048-row piece 269 against 267 and 267.
+constexpr int kUnitCost = 5, kPairUnitCost = 9;
 constexpr int kPieceRows = 256;            // rows of a workspace piece (pair mode: both lanes)
 
 // K and V tiles in flight; 8-bit caches hold raw tiles besides (kRaw) and the
