@@ -1066,6 +1066,32 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             if (!start) rescale_o(alpha);   // the first P V of a segment writes O anew
         };
 
+        // Then P of the chunks [c, c1) by the new reference, over their S; their sums.  (Apart from the usual path: a
+        // loop around that one, to go through it again, took 16 of 186 us of ragged 8-bit segments.)
+        auto redo = [&](int c, int c1, const float *ks, const float *vs, float m_ref) -> float {
+            const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
+            float sum = 0.0f;
+#pragma unroll 1
+            for (; c < c1; ++c) {
+                uint32_t v[32], pk[16];
+                tmem_ld32_issue(tS + 32u * c, v);
+                tmem_wait_ld32(v);
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    float e[2];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        e[q] = ex2_approx(fmaf(__uint_as_float(v[j + q]), k8 ? ks[32 * c + j + q] : p.scale_log2, -sub));
+                        sum += e[q];
+                        if constexpr (k8) e[q] *= vs[32 * c + j + q];
+                    }
+                    pk[j / 2] = pack_bf16x2(e[0], e[1]);
+                }
+                tmem_st16(tS + 16u * c, pk);
+            }
+            return sum;
+        };
+
         // Key tile kt (the ti-th of the segment) of pair and alternate mode; thread = query row.
         // No maximum is taken: the sums, which are needed anyway, tell when the reference will not do any more.
         auto row_tile = [&](int kt, int ti, bool masked, int pos, unsigned long long bits, bool start, float &m_ref, float &l_run,
@@ -1107,12 +1133,11 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             }
             const uint64_t c2 = f2(p.scale_log2, p.scale_log2);
             float tile_sum = 0.0f;
-            uint32_t sr[2][32];
-            tmem_ld32_issue(tS, sr[0]);
             if constexpr (!k8) {
-                // The whole tile unrolled and P stored at its end, over S that is intact until then (rolled up, as
-                // below, a 2048-row piece took 336 us instead of 297; with the converting warps beside it, the short
-                // code wins: 102 us against 106 for 8-bit contexts, 188 against 202 for ragged segments).
+                uint32_t sr[2][32];
+                tmem_ld32_issue(tS, sr[0]);
+                // The whole tile unrolled, two chunks of S in registers, and P stored at its end, over S that is intact
+                // until then: a 2048-row piece takes 265 us, 320 with the short loop below.
                 uint32_t pk[4][16];
 #pragma unroll 1
                 for (int again = 0; again < 2; ++again) {
@@ -1154,60 +1179,46 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 tmem_wait_st();
                 return;
             }
+            // The shortest code wins where the converting warps fetch theirs, too: ragged segments take 162 us, 170 with two
+            // chunks unrolled and 195 with the whole tile.
 #pragma unroll 1
-            for (int cc = 0; cc < 4; cc += 2) {
+            for (int c = 0; c < 4; ++c) {
+                uint32_t sv[32], pk[16];
+                tmem_ld32_issue(tS + 32u * c, sv);
+                tmem_wait_ld32(sv);
+                const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
+                const uint64_t nsub2 = f2(-sub, -sub);
+                uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c = cc + h;   // 32 keys
-                    tmem_wait_ld32(sr[h]);
-                    if (h == 0 || cc == 0) tmem_ld32_issue(tS + 32u * (c + 1), sr[h ^ 1]);
-                    uint32_t pk[16];
-                    float sum;
-#pragma unroll 1
-                    for (int again = 0; again < 2; ++again) {
-                        const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
-                        const uint64_t nsub2 = f2(-sub, -sub);
-                        uint64_t acc[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 fk = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                    float e[4];
+                    un_f2(fma_f2(f2(__uint_as_float(sv[j]), __uint_as_float(sv[j + 1])), f2(fk.x, fk.y), nsub2), e[0], e[1]);
+                    un_f2(fma_f2(f2(__uint_as_float(sv[j + 2]), __uint_as_float(sv[j + 3])), f2(fk.z, fk.w), nsub2), e[2], e[3]);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            uint64_t fa = c2, fb = c2;
-                            if constexpr (k8) {
-                                const float4 f = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
-                                fa = f2(f.x, f.y);
-                                fb = f2(f.z, f.w);
-                            }
-                            float e[4];
-                            un_f2(fma_f2(f2(__uint_as_float(sr[h][j]), __uint_as_float(sr[h][j + 1])), fa, nsub2), e[0], e[1]);
-                            un_f2(fma_f2(f2(__uint_as_float(sr[h][j + 2]), __uint_as_float(sr[h][j + 3])), fb, nsub2), e[2], e[3]);
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
-                            acc[0] = add_f2(acc[0], f2(e[0], e[1]));
-                            acc[1] = add_f2(acc[1], f2(e[2], e[3]));
-                            if constexpr (k8) {
-                                const float4 f = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
-                                un_f2(mul_f2(f2(e[0], e[1]), f2(f.x, f.y)), e[0], e[1]);
-                                un_f2(mul_f2(f2(e[2], e[3]), f2(f.z, f.w)), e[2], e[3]);
-                            }
-                            pk[j / 2] = pack_bf16x2(e[0], e[1]);
-                            pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
-                        }
-                        float s0, s1;
-                        un_f2(add_f2(acc[0], acc[1]), s0, s1);
-                        sum = s0 + s1;
-                        // Before P goes over S: has a term outgrown the range, or is a row's first sum too small to tell
-                        // its terms from zero (or has it none)?
-                        const bool unset = m_ref == -INFINITY, bad = sum > kSumMax || (unset && c == 0 && sum < 1.0f / kSumMax);
-                        if (!__any_sync(0xffffffffu, bad)) break;
-                        if (again == 0) {
-                            tmem_wait_ld32(sr[h ^ 1]);
-                            outgrown(c, bad, unset, start, ks, m_ref, l_run, tile_sum);
-                            if (h == 0 || cc == 0) tmem_ld32_issue(tS + 32u * (c + 1), sr[h ^ 1]);
-                        }
-                    }
-                    if (m_ref == -INFINITY && sum > 0.0f) m_ref = 0.0f;
-                    tile_sum += sum;
+                    for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
+                    acc[0] = add_f2(acc[0], f2(e[0], e[1]));
+                    acc[1] = add_f2(acc[1], f2(e[2], e[3]));
+                    const float4 fv = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
+                    un_f2(mul_f2(f2(e[0], e[1]), f2(fv.x, fv.y)), e[0], e[1]);
+                    un_f2(mul_f2(f2(e[2], e[3]), f2(fv.z, fv.w)), e[2], e[3]);
+                    pk[j / 2] = pack_bf16x2(e[0], e[1]);
+                    pk[j / 2 + 1] = pack_bf16x2(e[2], e[3]);
+                }
+                float s0, s1;
+                un_f2(add_f2(acc[0], acc[1]), s0, s1);
+                float sum = s0 + s1;
+                // Before P goes over S: has a term outgrown the range, or is a row's first sum too small to tell its
+                // terms from zero (or has it none)?
+                const bool unset = m_ref == -INFINITY, bad = sum > kSumMax || (unset && c == 0 && sum < 1.0f / kSumMax);
+                if (__any_sync(0xffffffffu, bad)) {
+                    outgrown(c, bad, unset, start, ks, m_ref, l_run, tile_sum);
+                    sum = redo(c, c + 1, ks, vs, m_ref);
+                } else {
                     tmem_st16(tS + 16u * c, pk);
                 }
+                if (m_ref == -INFINITY && sum > 0.0f) m_ref = 0.0f;
+                tile_sum += sum;
             }
             l_run += tile_sum;
             // The range is wide; a row that leaves its middle moves its reference before the next tile.
