@@ -849,3 +849,209 @@ def test_chunk_calls_in_a_captured_graph(pkg):
             c.dec.sync()
             chunks = [(ln[j] - m[j], m[j]) for j in range(2)]
             check_attend(c, chunks, q, [0, m[0]], out)
+
+
+# ---- many entries, wide ranges, large pools ----
+
+def check_entry(c, stream, length, rows, q, out, seen, extra=0.0):
+    m = rows.stop - rows.start
+    k, v = c.values(0, stream, length)
+    want, mag = attend_oracle(q[rows].double().view(m, HQ, D), k, v, seen)
+    err = (out[rows].double().view(m, HQ, D) - want).abs()
+    over = err > attend_tolerance(want, mag) + extra * mag
+    assert not over.any(), (c.kind, stream, length, m, err.max().item(), int(over.sum()))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "e4i8"])
+@pytest.mark.parametrize("n,bad", [(32, -1), (33, -1), (200, 77), (1024, -1)])
+def test_attend_many_entries(pkg, kv, n, bad):
+    """Entries by the hundred: padding between them, empty chunks, prefixes of a stream, a bad one; twice, the same bits."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(1, 400, 24)]
+    sizes = [0, 1, 1, 2, 5, 9, 17, 40] + ([70, 130] if n <= 200 else [])
+    slots, starts, ends, chunks = [], [0], [], []
+    for i in range(n):
+        j = int(rng.integers(0, len(lens)))
+        m = min(int(rng.choice(sizes)), lens[j])
+        end = int(rng.integers(max(m, 1), lens[j] + 1))
+        pad = rng.random() < 0.1
+        slots.append(-1 if pad else j)
+        chunks.append(None if pad or i == bad else (j, end, m))
+        ends.append(end)
+        starts.append(starts[-1] + m)
+    with Cache(pkg, kv, lens) as c:
+        c.fill()
+        c.poison_behind(lens)
+        gen = torch.Generator(device="cuda").manual_seed(2)
+        q = (1.3 * torch.randn((starts[-1] + 2, HQ * D), device="cuda", generator=gen)).to(torch.bfloat16)
+        ids = i32([999 if i == bad else (-1 if j < 0 else c.streams[j]) for i, j in enumerate(slots)])
+        d_starts, d_lens = i32(starts), i32(ends)
+        side = torch.cuda.Stream()
+        outs = [torch.full_like(q, -77.0) for _ in range(2)]
+        torch.cuda.synchronize()
+        for out in outs:
+            c.dec.chunk_attend(0, n, ids.data_ptr(), d_starts.data_ptr(), d_lens.data_ptr(), q.shape[0], None, q.data_ptr(),
+                               out.data_ptr(), side.cuda_stream)
+        torch.cuda.synchronize()
+        if bad >= 0:
+            with pytest.raises(pkg.QkvError) as ei:
+                c.dec.sync()
+            assert ei.value.code == 5
+        else:
+            c.dec.sync()
+        assert torch.equal(outs[0], outs[1])
+        for i, chunk in enumerate(chunks):
+            rows = slice(starts[i], starts[i + 1])
+            if chunk is None:
+                assert (outs[0][rows] == -77).all()
+            elif chunk[2]:
+                j, end, m = chunk
+                check_entry(c, c.streams[j], end, rows, q, outs[0], visible(end - m, m))
+        assert (outs[0][starts[-1]:] == -77).all()
+
+
+def profile(name, n):
+    """Size of token t's key along a direction: the scores, in powers of two, are about 16 times as large."""
+    t = np.arange(n)
+    return {"rising": 80.0 * t / n - 40.0, "falling": 40.0 - 80.0 * t / n, "low": -30.0 + 0.1 * np.sin(t),
+            "high": 45.0 + 0.1 * np.sin(t), "steps": np.array([-60.0, -20.0, 20.0, 0.0, 60.0, -5.0])[(t + 64) // 128 % 6],
+            "spike": np.where(t == n // 2, 50.0, 0.01 * np.cos(t)), "first": np.where(t == 0, 50.0, -0.3)}[name]
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "e4i8"])
+@pytest.mark.parametrize("name", ["rising", "falling", "low", "high", "steps", "spike", "first"])
+def test_attend_score_profiles(pkg, kv, name):
+    """Scores that run through hundreds of powers of two along the keys, for every number of rows at a time."""
+    chunks = [(660, 5), (663, 14), (650, 40), (600, 130), (0, 200), (3, 12)]
+    lens = [b + m for b, m in chunks]
+    starts = [sum(m for _, m in chunks[:j]) for j in range(len(chunks) + 1)]
+    with Cache(pkg, kv, lens) as c:
+        c.fill()
+        gen = torch.Generator(device="cuda").manual_seed(8)
+        u = torch.randint(0, 2, (HKV, D), device="cuda", generator=gen).float() * 2 - 1
+        for s, n in zip(c.streams, lens):
+            coef = torch.tensor(profile(name, n), dtype=torch.float32, device="cuda")
+            t = torch.arange(n, device="cuda")
+            page = torch.tensor(c.dec.pages(s).astype(np.int64), device="cuda")[t // PT]
+            if kv == "bf16":
+                c.pool[0, page, 0, :, t % PT] = (coef[:, None, None] * u).to(torch.bfloat16)
+            else:
+                code = torch.where(coef[:, None, None] * u >= 0, 0x38, 0xB8).to(torch.uint8)   # +-1
+                c.pool[0, page, 0, :, t % PT] = code
+                c.scales[0, page, 0, :, t % PT] = coef.abs()[:, None].clamp_min(1e-30).expand(-1, HKV).contiguous()
+        c.poison_behind(lens)
+        size = torch.ones((starts[-1], 1, 1), device="cuda")
+        size[1::4] = -1.0                     # these rows go through the profile upside down
+        size[2::4] = 0.01
+        q = size * u.repeat_interleave(2, 0) + 0.02 * torch.randn((starts[-1], HQ, D), device="cuda", generator=gen)
+        q = q.reshape(-1, HQ * D).to(torch.bfloat16)
+        out = run_attend(c, chunks, q, starts)
+        # the f32 rounding of scores in the hundreds reaches the weights: 128 2^-24 sum |q k| / sqrt(128) each way
+        for j, (base, m) in enumerate(chunks):
+            k, _ = c.values(0, c.streams[j], base + m)
+            rows = slice(starts[j], starts[j + 1])
+            qs = q[rows].double().view(m, HQ, D)
+            top = (torch.einsum("mhd,nhd->mhn", qs.abs(), k.abs().repeat_interleave(2, 1)) / math.sqrt(D)).max().item()
+            check_entry(c, c.streams[j], base + m, rows, q, out, visible(base, m), 2 * (128 * U * top + 2.0 ** -12))
+
+
+def test_attend_reports_missing_pages(pkg):
+    """A length that reaches pages the stream does not have: reported; the other entries' rows are right."""
+    with Cache(pkg, "bf16", [100, 230], max_context=600) as c:
+        c.fill()
+        gen = torch.Generator(device="cuda").manual_seed(2)
+        q = torch.randn((84, HQ * D), device="cuda", generator=gen).to(torch.bfloat16)
+        for m in (4, 40, 80):
+            starts = [0, m, m + 4]
+            with pytest.raises(pkg.QkvError) as ei:
+                run_attend(c, [None] * 2, q, starts, slots=c.streams, lens=[500, 230])
+            assert ei.value.code == 5
+            out = torch.full_like(q, -77.0)
+            d = [i32(c.streams), i32(starts), i32([500, 230])]
+            c.dec.chunk_attend(0, 2, d[0].data_ptr(), d[1].data_ptr(), d[2].data_ptr(), 84, None, q.data_ptr(), out.data_ptr())
+            torch.cuda.synchronize()
+            with pytest.raises(pkg.QkvError):
+                c.dec.sync()
+            check_entry(c, c.streams[1], 230, slice(m, m + 4), q, out, visible(226, 4))
+            assert (out[m + 4:] == -77).all()
+
+
+@pytest.mark.parametrize("kv", KINDS)
+def test_append_many_rows(pkg, kv):
+    """More rows than the SMs take at once, one at a time and together: the same bits; bad and padding rows between."""
+    n, lens = 3001, [3001, 3001]
+    with Cache(pkg, kv, lens) as c:
+        gen = torch.Generator(device="cuda").manual_seed(7)
+        qkv = torch.randn((n, QKV), device="cuda", generator=gen)
+        axes = torch.randint(-4000, 4000, (3, n), device="cuda", dtype=torch.int32, generator=gen)
+        pos = i32(range(n))
+        q = torch.full((n, HQ * D), -77.0, device="cuda")
+        slots = [c.streams[0]] * n
+        slots[1500] = -1
+        c.pool.zero_()
+        d = i32(slots)
+        c.dec.chunk_append(0, n, d.data_ptr(), pos.data_ptr(), axes.data_ptr(), (24, 20, 20), True, qkv.data_ptr(),
+                           q.data_ptr(), pkg.F32)
+        c.dec.sync()
+        one = torch.full((n, HQ * D), -77.0, device="cuda")
+        d1 = i32([c.streams[1]] * n)
+        picked = [0, 1, 591, 592, 593, 1499, 1501, 2999, 3000]
+        for r in picked:
+            ax = axes[:, r].contiguous()
+            c.dec.chunk_append(0, 1, d1[r:].data_ptr(), pos[r:].data_ptr(), ax.data_ptr(), (24, 20, 20), True,
+                               qkv[r].data_ptr(), one[r].data_ptr(), pkg.F32)
+        c.dec.sync()
+        assert torch.equal(q[picked], one[picked]) and (q[1500] == -77).all() and not (q == -77).all(1)[:1500].any()
+        (k0, v0), (k1, v1) = [c.values(0, s, n) for s in c.streams]
+        assert torch.equal(k0[picked], k1[picked]) and torch.equal(v0[picked], v1[picked]) and (k0[1500] == 0).all()
+        want, mag = append_oracle(qkv.double()[:, :HQ * D].view(n, HQ, D), torch.tensor(c.qn[0], device="cuda").double(), axes,
+                                  axis_of_pairs((24, 20, 20), True))
+        rows = torch.arange(n, device="cuda") != 1500
+        assert not ((q.double().view(n, HQ, D) - want).abs() > 2.0 ** -19 * mag + 1e-30)[rows].any()
+
+
+@pytest.mark.parametrize("kv,pages", [("bf16", 70000), ("fp8", 135000)])
+def test_pools_past_4_gib(pkg, kv, pages):
+    """Pages whose bytes lie past 2^32: append, attention, moves, and copies of more pages than a grid has rows."""
+    page_bytes = 65536 if kv == "bf16" else 32768
+    with Cache(pkg, kv, [], max_streams=2, spare=pages, max_context=8192) as c, Cache(pkg, kv, [3000, 3000]) as small:
+        gen = torch.Generator(device="cuda").manual_seed(7)
+        qkv = torch.randn((3000, QKV), device="cuda", generator=gen)
+        pos, got = i32(range(3000)), []
+        for dec in (c.dec, small.dec):
+            if dec is c.dec:
+                c.streams = [dec.open() for _ in range(2)]
+                for s in c.streams:
+                    dec.extend(s, 3000)
+                assert (dec.pages(c.streams[0]).astype(np.int64) * page_bytes > 1 << 32).any()
+            cache = c if dec is c.dec else small
+            slots = i32([cache.streams[0]] * 3000)
+            axes = torch.stack([pos] * 3).contiguous()
+            q = torch.empty((3000, HQ * D), device="cuda", dtype=torch.bfloat16)
+            dec.chunk_append(0, 3000, slots.data_ptr(), pos.data_ptr(), axes.data_ptr(), (24, 20, 20), True, qkv.data_ptr(),
+                             q.data_ptr(), pkg.BF16)
+            dec.sync()
+            chunk = q[-70:].contiguous()
+            out = run_attend(cache, [(2930, 70)], chunk, [0, 70])
+            run_move(cache, [(cache.streams[0], 5, cache.streams[1], 100, list(range(0, 2800, 7)))])
+            got.append((q, out, cache.values(0, cache.streams[0], 3000), [t[100:500] for t in cache.values(0, cache.streams[1], 500)]))
+        assert torch.equal(got[0][0], got[1][0])
+        for x, y in zip(got[0][2] + got[0][3], got[1][2] + got[1][3]):
+            assert torch.equal(x, y)
+        check_entry(c, c.streams[0], 3000, slice(0, 70), got[0][0][-70:], got[0][1], visible(2930, 70))
+        n = pages // 2 - 1000
+        perm = np.random.default_rng(1).permutation(pages)
+        src, dst = i32(perm[:n]), i32(perm[n:2 * n])
+        # a few bytes of each source page tell it from the others
+        raw_pool = c.pool.view(torch.uint8).view(pages, page_bytes)
+        mark = torch.randint(0, 256, (n, 64), device="cuda", dtype=torch.uint8, generator=gen)
+        raw_pool[src.long(), :32] = mark[:, :32]
+        raw_pool[src.long(), -32:] = mark[:, 32:]
+        c.dec.pages_copy(n, src.data_ptr(), dst.data_ptr())
+        c.dec.sync()
+        assert torch.equal(raw_pool[dst.long(), :32], mark[:, :32]) and torch.equal(raw_pool[dst.long(), -32:], mark[:, 32:])
+        probe = torch.randperm(n, device="cuda", generator=gen)[:500]
+        assert torch.equal(raw_pool[dst.long()[probe]], raw_pool[src.long()[probe]])
+        if c.scales is not None:
+            sc = c.scales.view(torch.int32)[0]
+            assert torch.equal(sc[dst.long()], sc[src.long()])
