@@ -339,11 +339,14 @@ int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
  * chunks of at most 64 rows), bit b says whether it sees the chunk's token b.
  * A row that sees nothing gives zeros.  q and out: [rows][Hq*D] bf16, 16-byte
  * aligned, q post-RoPE and unscaled; rows outside every chunk are left as they
- * are.  K and V of the lens[i] tokens must be finite; what lies behind them is
- * not read.  A slot may be listed more than once.  QKV_ERR_STATE for an f32
- * cache (qkv_prefill_attend serves it).  Uses the handle's workspace: calls on
- * one handle, captured ones too, must not overlap.  The prompt half of
- * text-decoder.cpp:322-334 for any number of rows at any context. */
+ * are.  K and V of the lens[i] tokens must be finite; what lies behind them does
+ * not matter.  A slot may be listed more than once.  An entry that breaks these
+ * rules is reported (qkv_sync) and skipped; one whose lens[i] reaches pages that
+ * the stream does not have is reported, and its rows are not defined.
+ * QKV_ERR_STATE for an f32 cache (qkv_prefill_attend serves it).  Uses the
+ * handle's workspace: calls on one handle, captured ones too, must not overlap.
+ * The prompt half of text-decoder.cpp:322-334 for any number of rows at any
+ * context. */
 int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slots_dev, const int32_t *starts_dev,
                      const int32_t *lens_dev, int32_t rows, const uint64_t *mask_dev, const void *q_dev, void *out_dev,
                      void *stream);
@@ -358,7 +361,8 @@ int qkv_pages_copy(qkv_handle *h, int32_t n, const int32_t *src_dev, const int32
  * dst_slots[i].  keep[rows] ascends within a group.  The two streams may be the
  * same with dst_bases[i] <= src_bases[i]: the accepted path of a draft tree
  * moves together before qkv_stream_truncate drops the rest.  Groups must not
- * touch each other's tokens.  A group outside these rules is reported and not
+ * touch each other's tokens, and pages that streams share after a fork are
+ * written for all of them.  A group outside these rules is reported and not
  * moved. */
 int qkv_tokens_move(qkv_handle *h, int32_t n, const int32_t *src_slots_dev, const int32_t *src_bases_dev,
                     const int32_t *dst_slots_dev, const int32_t *dst_bases_dev, const int32_t *starts_dev, int32_t rows,

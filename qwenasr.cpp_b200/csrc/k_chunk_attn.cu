@@ -19,8 +19,9 @@
 // In pair and alternate mode S = Q K', thread = query row; P goes back over S as
 // bf16 and is the A operand of P V in TMEM.  That costs a thread 128
 // exponentials a tile however few rows are real, which a short chunk, bound by
-// reading its context, cannot hide (186 us where 53 us are read: 64 draft trees
-// of 3 to 12 rows); in thin mode a thread has one key and computes 16 or 32.
+// reading its context, cannot hide (64 draft trees of 3 to 12 rows on contexts
+// of 150 to 2100 tokens: 186 us, 78 us in thin mode, 53 us to read them); in
+// thin mode a thread has one key and computes 16 or 32.
 //
 // Work split.  A unit's work is w T: T key tiles, w = 2 in pair mode and 1
 // elsewhere.  All units laid end to end are cut into equal parts, one per CTA
@@ -38,13 +39,24 @@
 // scale multiplies its scores, a value's scale its P.
 //
 // Roles: warps 0..3 lane 0, 4..7 lane 1, one MMA warp, two load warps (TMA: a
-// page's 16 keys of a head are a box; one warp K and Q, one V), and for 8-bit caches four warps that
-// convert the raw tiles.  Staging the tiles by cp.async from four warps took
-// 2700 cycles per 32 KB and bounded every shape; the MMA warp runs its loop as
-// a whole and elects a thread only to issue, so that descriptors stay in
-// uniform registers.
-// What a segment's start and end cost was mostly code fetched afresh, so
-// those parts are kept short or rolled up.
+// page's 16 keys of a head are a box; one warp K and Q, one V), one that plans
+// the segments, and for 8-bit caches eight that convert the raw tiles.  Staging
+// the tiles by cp.async from four warps took 2700 cycles per 32 KB and bounded
+// every shape; the MMA warp runs its loop as a whole and elects a thread only to
+// issue, so that descriptors stay in uniform registers.  What a segment's start
+// and end cost was mostly code fetched afresh, so those parts are kept short or
+// rolled up.
+//
+// What bounds it.  2048 bf16 rows on 16000 tokens: 265 to 300 us (by the card's
+// clock), 0.95 to 1.07 PFLOP/s; of a pair step's 3220 cycles the tensor cores
+// work 2100 and each softmax warp 2060, which is its 128 exponentials a row at
+// the pipe's rate, and the rest is one lane waiting where neither covers the
+// other.  The draft trees above: 4.5 TB/s, the rest their segments' starts and
+// ends.  Six 8-bit contexts of 9000 to 33000 tokens: 101 us, 3.1 TB/s, of 125
+// tiles of a CTA 864 cycles each in the converting warps (88 us without them).
+// Ragged e4m3 segments of 17 to 390 rows: 155 us; a pair step takes 6300 cycles,
+// as each softmax warp reads two scales a key besides and shares its scheduler
+// with the converting warps.
 // All waits bounded; a softmax warp whose wait ran out goes on without waiting,
 // so that the named barriers stay matched.
 #include <cuda.h>
@@ -105,13 +117,13 @@ constexpr int kMaxWarps = 20;
 
 // ---- work split ----
 
-// One listed chunk: its rows, and the work of one kv head.
 // Unsigned quotient; by 32 bits where that does (a 64-bit one takes hundreds of cycles).
 __device__ __forceinline__ long long quot(long long a, long long b) {
     if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
     return a / b;
 }
 
+// One listed chunk: its rows, and the work of one kv head.
 struct Entry {
     int slot, first, m, base, nb;
     long long head_cost;
@@ -374,11 +386,6 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool pred) {
         : "r"(static_cast<int>(pred)), "r"(id), "r"(threads)
         : "memory");
     return r != 0;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
 }
 constexpr int kBarLane = 1, kBarBoth = 3;   // ids kBarLane + lane, kBarBoth
 
