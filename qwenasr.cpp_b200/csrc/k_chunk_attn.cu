@@ -86,6 +86,7 @@ enum Mode { kThin = 0, kAlternate = 1, kPair = 2 };
 constexpr uint32_t kThinQ = kTileBytes, kThinQBytes = 8192, kThinQBlk = 4096;
 constexpr uint32_t kThinP = kTileBytes + 16384, kThinPBytes = 8192;
 constexpr int kMinCost = 2;                // least work of a CTA (tiles of alternate mode)
+static_assert(kMinCost >= 2, "every CTA between a unit's first and last holds one of its tiles");
 // Work of a unit besides its tiles.  Measured: 2640 cycles a tile and 9000 a unit in thin mode, 3260 a tile (counted
 // double) and 9200 a unit in pair mode.  Of (2, 3), (3, 6) and (5, 9), the last gave 64 draft trees 95 us against 99 and
 // 97, ragged segments 187 against 194 and 196, and a 2048-row piece 269 against 267 and 267.
@@ -135,13 +136,20 @@ __device__ __forceinline__ int block_tiles(const Entry &e, int b) {
     return static_cast<int>((static_cast<long long>(e.base) + min(e.m, (b + 1) * 2 * kQueries) + kKeys - 1) / kKeys);
 }
 
-// runmax: the largest end of the entries before i; rows that overlap an
+struct RawEntry {
+    int slot, first, next, len;
+};
+__device__ __forceinline__ RawEntry load_raw(const ChunkAttendParams &p, int i) {
+    return {__ldg(p.slots + i), __ldg(p.starts + i), __ldg(p.starts + i + 1), __ldg(p.lens + i)};
+}
+
+// runmax: the largest end of the entries before it; rows that overlap an
 // earlier entry's make the later one bad.
-__device__ __forceinline__ Entry load_entry(const ChunkAttendParams &p, int i, int runmax) {
+__device__ __forceinline__ Entry make_entry(const ChunkAttendParams &p, const RawEntry &r, int runmax) {
     Entry e;
-    e.slot = __ldg(p.slots + i);
-    e.first = __ldg(p.starts + i);
-    const int next = __ldg(p.starts + i + 1), len = __ldg(p.lens + i);
+    e.slot = r.slot;
+    e.first = r.first;
+    const int next = r.next, len = r.len;
     const bool in = e.first >= 0 && next >= e.first && next <= p.rows && e.first >= runmax;
     e.m = in ? next - e.first : 0;
     e.bad = e.slot != -1 && (!in || e.slot < 0 || e.slot >= p.max_streams || len < e.m ||
@@ -165,7 +173,7 @@ struct alignas(16) Segment {
     int slot, g, row0, nq;            // query rows row0 ..
     int q0pos, base, len_end, mode;   // position of the first query, of the chunk's first token; keys [0, len_end)
     int t0, t1, cols, first;          // key tiles; thin mode's columns (2 nq rounded up to 16); holds the first tile
-    int last, c_last, pad[2];         // holds the unit's last tile; the CTA that does, where this piece is the first
+    int last, c_first, c_last, pad;   // holds the unit's last tile; the CTAs that hold its first and its last
     __device__ __forceinline__ bool pair() const { return mode == kPair; }
 };
 
@@ -206,8 +214,8 @@ struct Walk {
     int i, runmax, g, b;
     long long x, x1, ustart, parts, total;
 
-    __device__ __forceinline__ void start(const ChunkAttendParams &p, const Start &f, long long from, long long to,
-                                          long long n_parts, long long sum) {
+    __device__ __forceinline__ void start(const Entry &first, const Start &f, long long from, long long to, long long n_parts,
+                                          long long sum) {
         x = from;
         x1 = to;
         parts = n_parts;
@@ -215,7 +223,7 @@ struct Walk {
         if (x >= x1) return;
         i = f.i;
         runmax = f.runmax;
-        e = load_entry(p, i, runmax);
+        e = first;
         long long rem = x - f.pre;
         g = static_cast<int>(quot(rem, e.head_cost));
         rem -= g * e.head_cost;
@@ -233,7 +241,7 @@ struct Walk {
             while (g == kHkv || e.m == 0) {        // the next entry with work
                 runmax = max(runmax, __ldg(p.starts + i + 1));
                 if (++i >= p.n) return false;
-                e = load_entry(p, i, runmax);
+                e = make_entry(p, load_raw(p, i), runmax);
                 g = b = 0;
                 ustart = x;
             }
@@ -255,7 +263,9 @@ struct Walk {
             s.cols = cnt > 8 ? 32 : 16;
             s.first = s.t0 == 0;
             s.last = s.t1 == tiles;
-            s.c_last = static_cast<int>(quot((at + static_cast<long long>(w) * (tiles - 1) + 1) * parts - 1, total));
+            auto holder = [&](long long pos) { return static_cast<int>(quot((pos + 1) * parts - 1, total)); };
+            s.c_first = holder(at);
+            s.c_last = holder(at + static_cast<long long>(w) * (tiles - 1));
             x = uend;
             ustart = uend;
             if (++b == e.nb) {
@@ -527,8 +537,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     pdl_wait();   // the entries, q rows and pages come from earlier kernels and copies
 
     // ---- this CTA's part [x0, x1) of the work ----
-    // Running maximum of the ends and running sum of the costs over the entries, four to a thread (n <= 1024); one
-    // warp alone holds up to 32 entries, and every warp then does the same without a barrier.
+    // Running maximum of the ends and running sum of the costs over the entries: up to 32 by the plan warp itself, more
+    // by all threads, four to a thread (n <= 1024).
     long long x0 = 0, x1 = 0, parts = 1, total = 0;
     auto part_of = [&]() {
         parts = max(1ll, min(static_cast<long long>(gridDim.x), total / kMinCost));
@@ -538,34 +548,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         }
     };
     Start from{0, 0, 0};
-    if (p.n <= 32) {
-        const int end = lane < p.n ? __ldg(p.starts + lane + 1) : 0;
-        int mx = end;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, mx, o);
-            if (lane >= o) mx = max(mx, v);
-        }
-        mx = __shfl_up_sync(0xffffffffu, mx, 1);
-        const int runmax = lane == 0 ? 0 : max(mx, 0);
-        long long c = 0;
-        if (lane < p.n) {
-            const Entry e = load_entry(p, lane, runmax);
-            if (e.bad && blockIdx.x == 0 && warp == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, lane, e.first);
-            c = kHkv * e.head_cost;
-        }
-        long long inc = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        total = __shfl_sync(0xffffffffu, inc, 31);
-        part_of();
-        const unsigned mine = __ballot_sync(0xffffffffu, inc - c <= x0 && x0 < inc);
-        const int i0 = mine ? __ffs(mine) - 1 : 0;
-        from = Start{i0, __shfl_sync(0xffffffffu, runmax, i0), __shfl_sync(0xffffffffu, inc - c, i0)};
-    } else {
+    if (p.n > 32) {
         constexpr int kPer = (kAttnMaxRows + kThreads - 1) / kThreads;
         const int e0 = tid * kPer;
         int ends[kPer], mx = 0;
@@ -593,7 +576,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             cost[k] = 0;
             maxes[k] = runmax;
             if (e0 + k < p.n) {
-                const Entry e = load_entry(p, e0 + k, runmax);
+                const Entry e = make_entry(p, load_raw(p, e0 + k), runmax);
                 if (e.bad && blockIdx.x == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, e0 + k, e.first);
                 cost[k] = kHkv * e.head_cost;
             }
@@ -622,7 +605,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         __syncthreads();
         from = tail->from;
     }
-    if (tid == 0) p.splits[blockIdx.x].c_last = -1;   // no unit starts here and goes on elsewhere (so far)
+    if (tid < 2) p.splits[2 * blockIdx.x + tid].n = 0;   // no unit cut here (so far)
     __syncthreads();
     fence_after();
     const uint32_t tmem = tail->tmem;
@@ -649,9 +632,44 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     set_regs_down<L::kOtherRegs>();
     if (warp == L::kPlanWarp) {
         // ================= plan: the segments, one after the other =================
+        Entry mine;
+        if (p.n <= 32) {
+            RawEntry raw{-1, 0, 0, 0};
+            if (lane < p.n) raw = load_raw(p, lane);
+            int mx = raw.next;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, mx, o);
+                if (lane >= o) mx = max(mx, v);
+            }
+            mx = __shfl_up_sync(0xffffffffu, mx, 1);
+            const int runmax = lane == 0 ? 0 : max(mx, 0);
+            mine = make_entry(p, raw, runmax);
+            if (mine.bad && blockIdx.x == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, lane, mine.first);
+            const long long c = kHkv * mine.head_cost;
+            long long inc = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            total = __shfl_sync(0xffffffffu, inc, 31);
+            part_of();
+            const unsigned has = __ballot_sync(0xffffffffu, inc - c <= x0 && x0 < inc);
+            const int i0 = has ? __ffs(has) - 1 : 0;
+            from = Start{i0, __shfl_sync(0xffffffffu, runmax, i0), __shfl_sync(0xffffffffu, inc - c, i0)};
+            mine.slot = __shfl_sync(0xffffffffu, mine.slot, i0);
+            mine.first = __shfl_sync(0xffffffffu, mine.first, i0);
+            mine.m = __shfl_sync(0xffffffffu, mine.m, i0);
+            mine.base = __shfl_sync(0xffffffffu, mine.base, i0);
+            mine.nb = __shfl_sync(0xffffffffu, mine.nb, i0);
+            mine.head_cost = __shfl_sync(0xffffffffu, mine.head_cost, i0);
+        } else if (x0 < x1) {
+            mine = make_entry(p, load_raw(p, from.i), from.runmax);
+        }
         if (lane == 0) {
             Walk walk;
-            walk.start(p, from, x0, x1, parts, total);
+            walk.start(mine, from, x0, x1, parts, total);
             bool more = true;
             for (uint32_t k = 0; more; ++k) {
                 const uint32_t b = k % kSegRing;
@@ -1521,9 +1539,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tail->epi_done);
-            if (s.first && !s.last && tid == 0) {
-                p.splits[blockIdx.x] = ChunkSplit{s.row0, s.nq, s.g, s.mode, s.c_last};   // goes on elsewhere
-            }
+            if (!(s.first && s.last) && tid == 0)
+                p.splits[2 * blockIdx.x + (s.first ? 1 : 0)] =
+                    ChunkSplit{s.row0, s.nq, s.g, s.mode, s.c_first, s.c_last - s.c_first + 1};
             tile_no += n;
         }
     }
@@ -1545,41 +1563,66 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     }
 }
 
-// Joins the pieces of the unit that starts in CTA blockIdx.x and goes on
-// elsewhere: o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, pieces in order.
-// Thread = (row, four dims), in the order the pieces lie in memory: thin mode's
-// row by row, the others' four dims of all rows together.
-constexpr int kJoinThreads = 256;
+// Joins the pieces of the units that are cut: o = sum_p 2^(m_p - M) o_p /
+// sum_p 2^(m_p - M) l_p, pieces in order.  As many blocks (times gridDim.y) share
+// a unit as it has pieces: those of the CTAs that held one, which are two units'
+// at most.  Thread = (row, four dims), in the order the pieces lie in memory:
+// thin mode's row by row, the others' four dims of all rows together.  Bound by
+// the latency of a launch and its dependent loads; kJoinBatch pieces' are in
+// flight together (one at a time, by the first CTA's blocks alone, 100 rows on
+// 3000 tokens took 47 us).
+constexpr int kJoinThreads = 256, kJoinBatch = 8, kJoinRows = 4;
 
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkAttendParams p) {
     pdl_trigger();
     pdl_wait();
-    const ChunkSplit d = p.splits[blockIdx.x];
-    const int c0 = blockIdx.x;
-    if (d.c_last <= c0) return;
-    const int rows = 2 * d.nq;   // pair: lane 0's 128 rows, then lane 1's
-    for (int w = blockIdx.y * kJoinThreads + threadIdx.x; w < rows * (kHeadDim / 4); w += gridDim.y * kJoinThreads) {
-        const bool thin = d.mode == kThin;
-        const int r = thin ? w / (kHeadDim / 4) : w % rows, c = thin ? w % (kHeadDim / 4) : w / rows;
-        const size_t off = thin ? static_cast<size_t>(w) * 4 : static_cast<size_t>(c) * (kPieceRows * 4) + r * 4;
-        float m = -INFINITY;
-        for (int k = c0; k <= d.c_last; ++k) m = fmaxf(m, p.part_ml[(2 * k + (k == c0 ? 1 : 0)) * kPieceRows + r].x);
-        float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = c0; k <= d.c_last; ++k) {
-            const size_t piece = 2 * k + (k == c0 ? 1 : 0);
-            const float2 ml = p.part_ml[piece * kPieceRows + r];
-            if (!(ml.y > 0.0f)) continue;
-            const float a = exp2f(ml.x - m);
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + piece * (kPieceRows * kHeadDim) + off);
-            l += a * ml.y;
-            o[0] += a * v.x;
-            o[1] += a * v.y;
-            o[2] += a * v.z;
-            o[3] += a * v.w;
+    const ChunkSplit both[2] = {p.splits[2 * blockIdx.x], p.splits[2 * blockIdx.x + 1]};
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+        const ChunkSplit d = side ? both[1] : both[0];
+        const int c0 = d.c_first, c_last = c0 + d.n - 1, rows = 2 * d.nq;   // pair: lane 0's 128 rows, then lane 1's
+        if (d.n < 2) continue;
+        for (int w = ((blockIdx.x - c0) * gridDim.y + blockIdx.y) * kJoinThreads + threadIdx.x; w < rows * (kHeadDim / 4);
+             w += d.n * gridDim.y * kJoinThreads) {
+            const bool thin = d.mode == kThin;
+            const int r = thin ? w / (kHeadDim / 4) : w % rows, c = thin ? w % (kHeadDim / 4) : w / rows;
+            const size_t off = thin ? static_cast<size_t>(w) * 4 : static_cast<size_t>(c) * (kPieceRows * 4) + r * 4;
+            float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k = c0; k <= c_last; k += kJoinBatch) {
+                float2 ml[kJoinBatch];
+                float4 v[kJoinBatch];
+#pragma unroll
+                for (int b = 0; b < kJoinBatch; ++b) {
+                    ml[b] = make_float2(-INFINITY, 0.0f);
+                    v[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (k + b > c_last) continue;
+                    const size_t piece = 2 * (k + b) + (k + b == c0 ? 1 : 0);
+                    ml[b] = p.part_ml[piece * kPieceRows + r];
+                    v[b] = *reinterpret_cast<const float4 *>(p.part_o + piece * (kPieceRows * kHeadDim) + off);
+                }
+                float top = m;
+#pragma unroll
+                for (int b = 0; b < kJoinBatch; ++b) top = ml[b].y > 0.0f ? fmaxf(top, ml[b].x) : top;
+                const float keep = l > 0.0f ? exp2f(m - top) : 0.0f;
+                m = top;
+                l *= keep;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o[q] *= keep;
+#pragma unroll
+                for (int b = 0; b < kJoinBatch; ++b) {
+                    if (!(ml[b].y > 0.0f)) continue;   // (a piece that saw nothing of the row)
+                    const float a = exp2f(ml[b].x - m);
+                    l += a * ml[b].y;
+                    o[0] += a * v[b].x;
+                    o[1] += a * v[b].y;
+                    o[2] += a * v[b].z;
+                    o[3] += a * v[b].w;
+                }
+            }
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            uint16_t *out = p.out + static_cast<size_t>(d.row0 + (r >> 1)) * kQDim + (2 * d.g + (r & 1)) * kHeadDim + 4 * c;
+            *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
         }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        uint16_t *out = p.out + static_cast<size_t>(d.row0 + (r >> 1)) * kQDim + (2 * d.g + (r & 1)) * kHeadDim + 4 * c;
-        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
     }
 }
 
@@ -1643,7 +1686,7 @@ template <bool k8> cudaError_t launch_main(const ChunkAttendParams &p, int num_s
 
 ChunkWorkspace chunk_workspace(int num_sms) {
     const size_t pieces = 2 * static_cast<size_t>(num_sms);
-    return ChunkWorkspace{pieces * kPieceRows * kHeadDim, pieces * kPieceRows, static_cast<size_t>(num_sms)};
+    return ChunkWorkspace{pieces * kPieceRows * kHeadDim, pieces * kPieceRows, pieces};
 }
 
 cudaError_t prepare_chunk_attn() {
@@ -1663,7 +1706,7 @@ cudaError_t launch_chunk_attn(const ChunkAttendParams &p, int kv_dtype, int num_
     if (kv_dtype == kKvBF16) e = launch_main<false>(p, num_sms, st);
     else if (kv_is_8bit(kv_dtype)) e = launch_main<true>(p, num_sms, st);
     if (e != cudaSuccess) return e;
-    return launch_pdl(chunk_join_kernel, dim3(num_sms, 8), dim3(kJoinThreads), 0, st, p);
+    return launch_pdl(chunk_join_kernel, dim3(num_sms, kJoinRows), dim3(kJoinThreads), 0, st, p);
 }
 
 }  // namespace qkv

@@ -137,10 +137,10 @@ struct ChunkAppendParams {
     int q_bf16;
 };
 
-// A unit of the chunk attention that starts in one CTA and ends in CTA c_last
-// (-1: none): its query rows, kv head and mode.
+// A unit of the chunk attention that n CTAs from c_first on hold a piece of
+// (n < 2: none): its query rows, kv head and mode.
 struct ChunkSplit {
-    int row0, nq, g, mode, c_last;
+    int row0, nq, g, mode, c_first, n;
 };
 
 // Chunk attention: stream i of n has queries starts[i] .. starts[i + 1] - 1 of
@@ -166,7 +166,7 @@ struct ChunkAttendParams {
     // workspace (chunk_workspace): two pieces per CTA of rows cut between CTAs
     float *part_o;
     float2 *part_ml;           // (reference maximum in log2, sum)
-    ChunkSplit *splits;        // [CTAs]
+    ChunkSplit *splits;        // [CTAs][unit that began before, unit that goes on]
 };
 
 struct ChunkWorkspace {
