@@ -1569,9 +1569,11 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
 // at most.  Thread = (row, four dims), in the order the pieces lie in memory:
 // thin mode's row by row, the others' four dims of all rows together.  Bound by
 // the latency of a launch and its dependent loads; kJoinBatch pieces' are in
-// flight together (one at a time, by the first CTA's blocks alone, 100 rows on
-// 3000 tokens took 47 us).
-constexpr int kJoinThreads = 256, kJoinBatch = 8, kJoinRows = 4;
+// flight together.  Operator time of 100 rows on 3000 tokens (some 20 pieces a
+// unit): 20 us, 47 us with one piece at a time by the first CTA's blocks alone;
+// of 5 rows on 512 tokens: 10.1 us, 11.2 us so.  More or larger blocks cost the
+// small launch what they give the large one.
+constexpr int kJoinThreads = 128, kJoinBatch = 6, kJoinRows = 8;
 
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkAttendParams p) {
     pdl_trigger();
