@@ -1872,6 +1872,8 @@ int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
     if (rows > kChunkMaxRows) return fail(h, QKV_ERR_CAPACITY, "chunk_attend: more than 2^20 rows");
     if (!aligned16(q_dev) || !aligned16(out_dev))
         return fail(h, QKV_ERR_INVALID_ARG, "chunk_attend: q and out must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(mask_dev) % sizeof(uint64_t) != 0)
+        return fail(h, QKV_ERR_INVALID_ARG, "chunk_attend: mask must be 8-byte aligned");
     if (n == 0 || rows == 0) return QKV_OK;
     CK(cudaSetDevice(h->device));
     ChunkAttendParams p{};

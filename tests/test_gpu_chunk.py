@@ -955,6 +955,21 @@ def test_attend_score_profiles(pkg, kv, name):
             check_entry(c, c.streams[j], base + m, rows, q, out, visible(base, m), 2 * (128 * U * top + 2.0 ** -12))
 
 
+def test_attend_mask_alignment_and_large_values(pkg):
+    with Cache(pkg, "bf16", [300, 300]) as c:
+        c.fill()
+        buf = torch.zeros(4096, dtype=torch.int64, device="cuda")
+        a = buf.data_ptr()
+        with pytest.raises(pkg.QkvError) as ei:
+            c.dec.chunk_attend(0, 1, a, a, a, 1, a + 4, a, a)
+        assert ei.value.code == 1
+        c.pool[:, :, 1] *= 2.0 ** 61           # exact; largest magnitude below 2^64
+        gen = torch.Generator(device="cuda").manual_seed(2)
+        q = torch.randn((80, HQ * D), device="cuda", generator=gen).to(torch.bfloat16)
+        chunks, starts = [(290, 10), (230, 70)], [0, 10, 80]
+        check_attend(c, chunks, q, starts, run_attend(c, chunks, q, starts))
+
+
 def test_attend_reports_missing_pages(pkg):
     """A length that reaches pages the stream does not have: reported; the other entries' rows are right."""
     with Cache(pkg, "bf16", [100, 230], max_context=600) as c:
