@@ -52,8 +52,8 @@
 // work 2100 and each softmax warp 2060, which is its 128 exponentials a row at
 // the pipe's rate, and the rest is one lane waiting where neither covers the
 // other.  The draft trees above: 4.5 TB/s, the rest their segments' starts and
-// ends.  Six 8-bit contexts of 9000 to 33000 tokens: 101 us, 3.1 TB/s, of 125
-// tiles of a CTA 864 cycles each in the converting warps (88 us without them).
+// ends.  Six 8-bit contexts of 9000 to 33000 tokens: 101 us, 3.1 TB/s, of
+// a CTA's 125 K and V tiles 864 cycles each in the converting warps (88 us without them).
 // Ragged e4m3 segments of 17 to 390 rows: 155 us; a pair step takes 6300 cycles,
 // as each softmax warp reads two scales a key besides and shares its scheduler
 // with the converting warps.
@@ -1135,8 +1135,6 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 // code of the rest.)
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32_issue(tS + 32u * c, v);
                     const int k0 = kt * kKeys + 32 * c;
                     uint32_t seen;
                     if (!p.mask) {
@@ -1148,6 +1146,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                                         : (d < 0 ? ((1u << -d) - 1u) | static_cast<uint32_t>(bits << -d)
                                                  : (d < 64 ? static_cast<uint32_t>(bits >> d) : 0u));
                     }
+                    if (__all_sync(0xffffffffu, seen == 0xffffffffu)) continue;
+                    uint32_t v[32];
+                    tmem_ld32_issue(tS + 32u * c, v);
                     tmem_wait_ld32(v);
                     float x[32];
 #pragma unroll
