@@ -339,14 +339,16 @@ int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
  * chunks of at most 64 rows), bit b says whether it sees the chunk's token b.
  * A row that sees nothing gives zeros.  q and out: [rows][Hq*D] bf16, 16-byte
  * aligned, q post-RoPE and unscaled; rows outside every chunk are left as they
- * are.  K and V of the lens[i] tokens must be finite, V below 2^64 in magnitude;
- * what lies behind them does not matter.  A slot may be listed more than once.  An entry that breaks these
- * rules is reported (qkv_sync) and skipped; one whose lens[i] reaches pages that
- * the stream does not have is reported, and its rows are not defined.
- * QKV_ERR_STATE for an f32 cache (qkv_prefill_attend serves it).  Uses the
- * handle's workspace: calls on one handle, captured ones too, must not overlap.
- * The prompt half of text-decoder.cpp:322-334 for any number of rows at any
- * context. */
+ * are.  K and V of the lens[i] tokens must be finite, V below 2^64 in
+ * magnitude; what lies behind them does not matter.  A slot may be listed more
+ * than once.  An entry that breaks these rules is reported (qkv_sync) and
+ * skipped; one whose lens[i] reaches pages that the stream does not have is
+ * reported, and its rows are not defined.  QKV_ERR_STATE for an f32 cache
+ * (qkv_prefill_attend serves it), QKV_ERR_CAPACITY for more than 2^20 rows, or
+ * so many with a max_context past 2^20 that their work passes 2^31 tiles.  Uses
+ * the handle's workspace: calls on one handle, captured ones too, must not
+ * overlap.  The prompt half of text-decoder.cpp:322-334 for any number of rows
+ * at any context. */
 int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slots_dev, const int32_t *starts_dev,
                      const int32_t *lens_dev, int32_t rows, const uint64_t *mask_dev, const void *q_dev, void *out_dev,
                      void *stream);

@@ -118,22 +118,16 @@ constexpr int kMaxWarps = 20;
 
 // ---- work split ----
 
-// Unsigned quotient; by 32 bits where that does (a 64-bit one takes hundreds of cycles).
-__device__ __forceinline__ long long quot(long long a, long long b) {
-    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-    return a / b;
-}
-
 // One listed chunk: its rows, and the work of one kv head.
 struct Entry {
     int slot, first, m, base, nb;
-    long long head_cost;
+    int head_cost;            // (all work of a call together stays below 2^31: chunk_work_fits)
     bool bad;
 };
 
 __device__ __forceinline__ int block_queries(const Entry &e, int b) { return min(2 * kQueries, e.m - b * 2 * kQueries); }
 __device__ __forceinline__ int block_tiles(const Entry &e, int b) {
-    return static_cast<int>((static_cast<long long>(e.base) + min(e.m, (b + 1) * 2 * kQueries) + kKeys - 1) / kKeys);
+    return static_cast<int>((static_cast<unsigned>(e.base) + min(e.m, (b + 1) * 2 * kQueries) + kKeys - 1) / kKeys);
 }
 
 struct RawEntry {
@@ -160,10 +154,10 @@ __device__ __forceinline__ Entry make_entry(const ChunkAttendParams &p, const Ra
     e.nb = (e.m + 2 * kQueries - 1) / (2 * kQueries);
     e.head_cost = 0;
     if (e.nb > 0) {
-        const long long full = e.nb - 1, p0 = (static_cast<long long>(e.base) + kKeys - 1) / kKeys;
+        const int full = e.nb - 1, p0 = static_cast<int>((static_cast<unsigned>(e.base) + kKeys - 1) / kKeys);
         // full blocks end on a multiple of 128 queries: T_b = p0 + b + 1
         e.head_cost = 2 * (full * p0 + full * (full + 1) / 2) +
-                      static_cast<long long>(block_queries(e, e.nb - 1) > kQueries ? 2 : 1) * block_tiles(e, e.nb - 1) +
+                      (block_queries(e, e.nb - 1) > kQueries ? 2 : 1) * block_tiles(e, e.nb - 1) +
                       kPairUnitCost * full + (block_queries(e, e.nb - 1) > kQueries ? kPairUnitCost : kUnitCost);
     }
     return e;
@@ -185,9 +179,23 @@ __device__ __forceinline__ uint32_t q_areas(int mode, uint32_t prev) {
 
 // Where a CTA's part starts: the entry, the largest end before it, the work before it.
 struct Start {
-    int i, runmax;
-    long long pre;
+    int i, runmax, pre;
 };
+
+// The work cut into equal parts, the first r of them one larger.
+struct Cuts {
+    int parts, q, r;
+    __device__ __forceinline__ int at(int c) const { return c * q + min(c, r); }   // where part c starts
+    __device__ __forceinline__ int holder(int pos) const {
+        const int lim = r * (q + 1);
+        return pos < lim ? static_cast<int>(static_cast<unsigned>(pos) / static_cast<unsigned>(q + 1))
+                         : r + static_cast<int>(static_cast<unsigned>(pos - lim) / static_cast<unsigned>(q));
+    }
+};
+__device__ __forceinline__ Cuts cut_work(int total) {
+    const int parts = max(1, min(static_cast<int>(gridDim.x), total / kMinCost)), q = total / parts;
+    return {parts, q, total - q * parts};
+}
 
 constexpr int kSegRing = 4;
 struct alignas(16) Tail {
@@ -212,24 +220,26 @@ static_assert(Layout<true>::kTailOff + sizeof(Tail) <= 227 * 1024, "8-bit layout
 struct Walk {
     Entry e;
     int i, runmax, g, b;
-    long long x, x1, ustart, parts, total;
+    int x, x1, ustart;
+    Cuts cuts;
 
-    __device__ __forceinline__ void start(const Entry &first, const Start &f, long long from, long long to, long long n_parts,
-                                          long long sum) {
-        x = from;
-        x1 = to;
-        parts = n_parts;
-        total = sum;
+    __device__ __forceinline__ void start(const Entry &first, const Start &f, const Cuts &c) {
+        cuts = c;
+        x = x1 = 0;
+        if (static_cast<int>(blockIdx.x) < c.parts) {
+            x = c.at(blockIdx.x);
+            x1 = c.at(blockIdx.x + 1);
+        }
         if (x >= x1) return;
         i = f.i;
         runmax = f.runmax;
         e = first;
-        long long rem = x - f.pre;
-        g = static_cast<int>(quot(rem, e.head_cost));
+        int rem = x - f.pre;
+        g = rem / e.head_cost;
         rem -= g * e.head_cost;
         b = 0;
         while (b < e.nb - 1) {
-            const long long c = 2ll * block_tiles(e, b) + kPairUnitCost;
+            const int c = 2 * block_tiles(e, b) + kPairUnitCost;
             if (rem < c) break;
             rem -= c;
             ++b;
@@ -248,9 +258,9 @@ struct Walk {
             const int cnt = block_queries(e, b), w = cnt > kQueries ? 2 : 1;
             const int tiles = block_tiles(e, b);
             // tile t is the CTA's that holds position `at` + w t
-            const long long at = ustart + (w == 2 ? kPairUnitCost : kUnitCost), uend = at + static_cast<long long>(w) * tiles;
-            s.t0 = static_cast<int>(max(0ll, x - at + w - 1) >> (w - 1));
-            s.t1 = static_cast<int>(min(static_cast<long long>(tiles), max(0ll, x1 - at + w - 1) >> (w - 1)));
+            const int at = ustart + (w == 2 ? kPairUnitCost : kUnitCost), uend = at + w * tiles;
+            s.t0 = max(0, x - at + w - 1) >> (w - 1);
+            s.t1 = min(tiles, max(0, x1 - at + w - 1) >> (w - 1));
             s.slot = e.slot;
             s.g = g;
             s.row0 = e.first + b * 2 * kQueries;
@@ -263,9 +273,8 @@ struct Walk {
             s.cols = cnt > 8 ? 32 : 16;
             s.first = s.t0 == 0;
             s.last = s.t1 == tiles;
-            auto holder = [&](long long pos) { return static_cast<int>(quot((pos + 1) * parts - 1, total)); };
-            s.c_first = holder(at);
-            s.c_last = holder(at + static_cast<long long>(w) * (tiles - 1));
+            s.c_first = cuts.holder(at);
+            s.c_last = cuts.holder(at + w * (tiles - 1));
             x = uend;
             ustart = uend;
             if (++b == e.nb) {
@@ -534,20 +543,15 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tail->tmem;
     pdl_wait();   // the entries, q rows and pages come from earlier kernels and copies
 
-    // ---- this CTA's part [x0, x1) of the work ----
-    // Running maximum of the ends and running sum of the costs over the entries: up to 32 by the plan warp itself, more
-    // by all threads, four to a thread (n <= 1024).
-    long long x0 = 0, x1 = 0, parts = 1, total = 0;
-    auto part_of = [&]() {
-        parts = max(1ll, min(static_cast<long long>(gridDim.x), total / kMinCost));
-        if (blockIdx.x < parts) {
-            x0 = quot(blockIdx.x * total, parts);
-            x1 = quot((blockIdx.x + 1) * total, parts);
-        }
-    };
-    Start from{0, 0, 0};
+    // ---- this CTA's part of the work ----
+    // Running maximum of the ends and running sum of the costs over the entries: up to 32 by the plan warp itself (its
+    // part of a small call is a chain of latencies, and begins here), more by all threads, four to a thread (n <= 1024).
+    int total = 0;
     if (p.n > 32) {
         constexpr int kPer = (kAttnMaxRows + kThreads - 1) / kThreads;
         const int e0 = tid * kPer;
@@ -562,14 +566,14 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             const int v = __shfl_up_sync(0xffffffffu, mx_inc, o);
             if (lane >= o) mx_inc = max(mx_inc, v);
         }
-        long long *const warp_sum = reinterpret_cast<long long *>(tail->ml[0]);
+        int *const warp_sum = reinterpret_cast<int *>(tail->ml[0]);
         int *const warp_max = reinterpret_cast<int *>(tail->ml[1]);
         if (lane == 31) warp_max[warp] = mx_inc;
         __syncthreads();
         int runmax = __shfl_up_sync(0xffffffffu, mx_inc, 1);
         if (lane == 0) runmax = 0;
         for (int w = 0; w < warp; ++w) runmax = max(runmax, warp_max[w]);
-        long long cost[kPer], sum = 0;
+        int cost[kPer], sum = 0;
         int maxes[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
@@ -583,32 +587,29 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             sum += cost[k];
             runmax = max(runmax, ends[k]);
         }
-        long long inc = sum;
+        int inc = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
         if (lane == 31) warp_sum[warp] = inc;
         __syncthreads();
-        long long pre = inc - sum;
+        int pre = inc - sum;
         for (int w = 0; w < L::kWarps; ++w) {
             if (w < warp) pre += warp_sum[w];
             total += warp_sum[w];
         }
-        part_of();
+        const Cuts cuts = cut_work(total);
+        const int x0 = cuts.at(blockIdx.x);
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             if (pre <= x0 && x0 < pre + cost[k]) tail->from = Start{e0 + k, maxes[k], pre};
             pre += cost[k];
         }
         __syncthreads();
-        from = tail->from;
     }
-    if (tid < 2) p.splits[2 * blockIdx.x + tid].n = 0;   // no unit cut here (so far)
-    __syncthreads();
-    fence_after();
-    const uint32_t tmem = tail->tmem;
+    if (tid == 0) p.splits[2 * blockIdx.x].n = p.splits[2 * blockIdx.x + 1].n = 0;   // no unit cut here (so far)
 
     Segment s;
     uint32_t seg_no = 0;
@@ -633,6 +634,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     if (warp == L::kPlanWarp) {
         // ================= plan: the segments, one after the other =================
         Entry mine;
+        Start from;
+        Cuts cuts;
         if (p.n <= 32) {
             RawEntry raw{-1, 0, 0, 0};
             if (lane < p.n) raw = load_raw(p, lane);
@@ -646,15 +649,15 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             const int runmax = lane == 0 ? 0 : max(mx, 0);
             mine = make_entry(p, raw, runmax);
             if (mine.bad && blockIdx.x == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, lane, mine.first);
-            const long long c = kHkv * mine.head_cost;
-            long long inc = c;
+            const int c = kHkv * mine.head_cost;
+            int inc = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                const int v = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += v;
             }
-            total = __shfl_sync(0xffffffffu, inc, 31);
-            part_of();
+            cuts = cut_work(__shfl_sync(0xffffffffu, inc, 31));
+            const int x0 = cuts.at(blockIdx.x);
             const unsigned has = __ballot_sync(0xffffffffu, inc - c <= x0 && x0 < inc);
             const int i0 = has ? __ffs(has) - 1 : 0;
             from = Start{i0, __shfl_sync(0xffffffffu, runmax, i0), __shfl_sync(0xffffffffu, inc - c, i0)};
@@ -664,12 +667,14 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             mine.base = __shfl_sync(0xffffffffu, mine.base, i0);
             mine.nb = __shfl_sync(0xffffffffu, mine.nb, i0);
             mine.head_cost = __shfl_sync(0xffffffffu, mine.head_cost, i0);
-        } else if (x0 < x1) {
+        } else {
+            cuts = cut_work(total);
+            from = tail->from;
             mine = make_entry(p, load_raw(p, from.i), from.runmax);
         }
         if (lane == 0) {
             Walk walk;
-            walk.start(mine, from, x0, x1, parts, total);
+            walk.start(mine, from, cuts);
             bool more = true;
             for (uint32_t k = 0; more; ++k) {
                 const uint32_t b = k % kSegRing;
@@ -1686,6 +1691,13 @@ template <bool k8> cudaError_t launch_main(const ChunkAttendParams &p, int num_s
 }
 
 }  // namespace
+
+// Whether the work of a call, counted as the kernel does, stays below 2^31 whatever its lists say.
+bool chunk_work_fits(int n, int rows, int maxp) {
+    const long long blocks = rows / (2 * kQueries) + static_cast<long long>(n);
+    const long long tiles = (static_cast<long long>(maxp) * kPageTokens + kKeys - 1) / kKeys;
+    return blocks * (2 * tiles + kPairUnitCost) * kHkv < 1ll << 31;
+}
 
 ChunkWorkspace chunk_workspace(int num_sms) {
     const size_t pieces = 2 * static_cast<size_t>(num_sms);

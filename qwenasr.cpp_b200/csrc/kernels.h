@@ -205,6 +205,7 @@ struct TokensMoveParams {
 cudaError_t launch_kv_append(const AppendParams &p, int kv_dtype, cudaStream_t st);
 cudaError_t launch_chunk_append(const ChunkAppendParams &p, int kv_dtype, int num_sms, cudaStream_t st);
 // bf16 and 8-bit caches.
+bool chunk_work_fits(int n, int rows, int maxp);
 ChunkWorkspace chunk_workspace(int num_sms);
 cudaError_t prepare_chunk_attn();
 cudaError_t launch_chunk_attn(const ChunkAttendParams &p, int kv_dtype, int num_sms, cudaStream_t st);

@@ -793,8 +793,7 @@ int check_streams(qkv_handle *h, int n, const int32_t *streams) {
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// Rows one chunk attention takes: its work arithmetic stays inside 32 bits
-// well past it.
+// Rows one chunk attention takes at most.
 constexpr int kChunkMaxRows = 1 << 20;
 
 // Softmax scale folded into q: 1 / sqrt(head dim) in the log2 domain.
@@ -1870,6 +1869,8 @@ int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
     if (h->rt.kv_dtype == QKV_F32) return fail(h, QKV_ERR_STATE, "chunk_attend: needs a bf16 or 8-bit cache");
     if (n > kAttnMaxRows) return fail(h, QKV_ERR_CAPACITY, "chunk_attend: more than 1024 streams");
     if (rows > kChunkMaxRows) return fail(h, QKV_ERR_CAPACITY, "chunk_attend: more than 2^20 rows");
+    if (!chunk_work_fits(n, rows, h->maxp))
+        return fail(h, QKV_ERR_CAPACITY, "chunk_attend: too many rows for contexts this long in one call");
     if (!aligned16(q_dev) || !aligned16(out_dev))
         return fail(h, QKV_ERR_INVALID_ARG, "chunk_attend: q and out must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(mask_dev) % sizeof(uint64_t) != 0)

@@ -970,6 +970,18 @@ def test_attend_mask_alignment_and_large_values(pkg):
         check_attend(c, chunks, q, starts, run_attend(c, chunks, q, starts))
 
 
+def test_attend_refuses_more_work_than_it_counts(pkg):
+    """2^20 rows where each could see 2^21 tokens: past 2^31 units of work; a few rows there are served."""
+    with Cache(pkg, "bf16", [300], max_context=1 << 21) as c:
+        c.fill()
+        gen = torch.Generator(device="cuda").manual_seed(2)
+        q = torch.randn((300, HQ * D), device="cuda", generator=gen).to(torch.bfloat16)
+        with pytest.raises(pkg.QkvError) as ei:
+            run_attend(c, [(0, 300)], q, [0, 300], rows=1 << 20)
+        assert ei.value.code == 3
+        check_attend(c, [(0, 300)], q, [0, 300], run_attend(c, [(0, 300)], q, [0, 300]))
+
+
 def test_attend_reports_missing_pages(pkg):
     """A length that reaches pages the stream does not have: reported; the other entries' rows are right."""
     with Cache(pkg, "bf16", [100, 230], max_context=600) as c:
