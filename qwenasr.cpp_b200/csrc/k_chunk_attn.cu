@@ -20,7 +20,7 @@
 // bf16 and is the A operand of P V in TMEM.  That costs a thread 128
 // exponentials a tile however few rows are real, which a short chunk, bound by
 // reading its context, cannot hide (64 draft trees of 3 to 12 rows on contexts
-// of 150 to 2100 tokens: 186 us, 78 us in thin mode, 53 us to read them); in
+// of 150 to 2100 tokens: 186 us, 77 us in thin mode, 53 us to read them); in
 // thin mode a thread has one key and computes 16 or 32.
 //
 // Work split.  A unit's work is w T: T key tiles, w = 2 in pair mode and 1
@@ -47,16 +47,18 @@
 // and end cost was mostly code fetched afresh, so those parts are kept short or
 // rolled up.
 //
-// What bounds it.  2048 bf16 rows on 16000 tokens: 265 to 300 us (by the card's
-// clock), 0.95 to 1.07 PFLOP/s; of a pair step's 3220 cycles the tensor cores
+// What bounds it.  2048 bf16 rows on 16000 tokens: 250 to 295 us (by the card's
+// clock), 0.97 to 1.14 PFLOP/s; of a pair step's 3220 cycles the tensor cores
 // work 2100 and each softmax warp 2060, which is its 128 exponentials a row at
 // the pipe's rate, and the rest is one lane waiting where neither covers the
 // other.  The draft trees above: 4.5 TB/s, the rest their segments' starts and
 // ends.  Six 8-bit contexts of 9000 to 33000 tokens: 101 us, 3.1 TB/s, of
 // a CTA's 125 K and V tiles 864 cycles each in the converting warps (88 us without them).
-// Ragged e4m3 segments of 17 to 390 rows: 155 us; a pair step takes 6300 cycles,
+// Ragged e4m3 segments of 17 to 390 rows: 156 us; a pair step takes 6300 cycles,
 // as each softmax warp reads two scales a key besides and shares its scheduler
-// with the converting warps.
+// with the converting warps.  Five rows on 512 tokens: 9.4 us, a chain of
+// latencies (plan 3300 cycles, K tile in place at 7100, P V done at 9200,
+// epilogue 2100, then the join).
 // All waits bounded; a softmax warp whose wait ran out goes on without waiting,
 // so that the named barriers stay matched.
 #include <cuda.h>
@@ -1575,10 +1577,10 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
 // at most.  Thread = (row, four dims), in the order the pieces lie in memory:
 // thin mode's row by row, the others' four dims of all rows together.  Bound by
 // the latency of a launch and its dependent loads; kJoinBatch pieces' are in
-// flight together.  Operator time of 100 rows on 3000 tokens (some 20 pieces a
-// unit): 20 us, 47 us with one piece at a time by the first CTA's blocks alone;
-// of 5 rows on 512 tokens: 10.1 us, 11.2 us so.  More or larger blocks cost the
-// small launch what they give the large one.
+// flight together.  With one piece at a time by the first CTA's blocks alone, 100
+// rows on 3000 tokens (some 20 pieces a unit) took 47 us instead of 20, 5 rows on
+// 512 tokens 11.2 us instead of 10.1.  More or larger blocks cost the small
+// launch what they give the large one.
 constexpr int kJoinThreads = 128, kJoinBatch = 6, kJoinRows = 8;
 
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkAttendParams p) {
