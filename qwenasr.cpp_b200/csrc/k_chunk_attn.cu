@@ -116,7 +116,6 @@ template <bool k8> struct Layout {
     static constexpr size_t kRawScaleOff = kScaleOff + (k8 ? kScaleRing * 2 * kKeys * sizeof(float) : 0);
     static constexpr size_t kTailOff = kRawScaleOff + kRaw * 2 * kKeys * sizeof(float);
 };
-constexpr int kMaxWarps = 20;
 
 // ---- work split ----
 
