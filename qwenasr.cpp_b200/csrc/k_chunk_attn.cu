@@ -556,11 +556,12 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
     if (p.n > 32) {
         constexpr int kPer = (kAttnMaxRows + kThreads - 1) / kThreads;
         const int e0 = tid * kPer;
-        int ends[kPer], mx = 0;
+        RawEntry raw[kPer];
+        int mx = 0;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) ends[k] = e0 + k < p.n ? __ldg(p.starts + e0 + k + 1) : 0;
+        for (int k = 0; k < kPer; ++k) raw[k] = e0 + k < p.n ? load_raw(p, e0 + k) : RawEntry{-1, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) mx = max(mx, ends[k]);
+        for (int k = 0; k < kPer; ++k) mx = max(mx, raw[k].next);
         int mx_inc = mx;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -578,15 +579,12 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         int maxes[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            cost[k] = 0;
             maxes[k] = runmax;
-            if (e0 + k < p.n) {
-                const Entry e = make_entry(p, load_raw(p, e0 + k), runmax);
-                if (e.bad && blockIdx.x == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, e0 + k, e.first);
-                cost[k] = kHkv * e.head_cost;
-            }
+            const Entry e = make_entry(p, raw[k], runmax);
+            if (e.bad && blockIdx.x == 0) report_error(p.err, kErrRowBounds, kWhereChunkAttn, e0 + k, e.first);
+            cost[k] = kHkv * e.head_cost;
             sum += cost[k];
-            runmax = max(runmax, ends[k]);
+            runmax = max(runmax, raw[k].next);
         }
         int inc = sum;
 #pragma unroll
