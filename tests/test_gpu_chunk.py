@@ -1082,3 +1082,28 @@ def test_pools_past_4_gib(pkg, kv, pages):
         if c.scales is not None:
             sc = c.scales.view(torch.int32)[0]
             assert torch.equal(sc[dst.long()], sc[src.long()])
+
+
+def test_two_handles_at_once(pkg):
+    """Calls of two handles on two streams, in flight together, give what they give alone."""
+    chunks = [[(900, 9), (40, 130)], [(1500, 30), (10, 2), (333, 70)]]
+    with Cache(pkg, "bf16", [b + m for b, m in chunks[0]]) as a, Cache(pkg, "fp8", [b + m for b, m in chunks[1]]) as b:
+        caches, work = (a, b), []
+        for c, ch in zip(caches, chunks):
+            c.fill()
+            starts = [sum(m for _, m in ch[:j]) for j in range(len(ch) + 1)]
+            gen = torch.Generator(device="cuda").manual_seed(2)
+            q = torch.randn((starts[-1], HQ * D), device="cuda", generator=gen).to(torch.bfloat16)
+            alone = run_attend(c, ch, q, starts)
+            check_attend(c, ch, q, starts, alone)
+            lists = [i32(c.streams), i32(starts), i32([base + m for base, m in ch])]
+            work.append((c, len(ch), lists, q, alone, [torch.full_like(q, -77.0) for _ in range(20)], torch.cuda.Stream()))
+        torch.cuda.synchronize()
+        for k in range(20):
+            for c, n, lists, q, _, outs, st in work:
+                c.dec.chunk_attend(0, n, *[t.data_ptr() for t in lists], q.shape[0], None, q.data_ptr(), outs[k].data_ptr(),
+                                   st.cuda_stream)
+        torch.cuda.synchronize()
+        for c, _, _, _, alone, outs, _ in work:
+            c.dec.sync()
+            assert all(torch.equal(o, alone) for o in outs)
