@@ -201,14 +201,12 @@ def _pool(case, layers, pages, seed):
     return codes, scale[..., 0].contiguous()
 
 
-SECTIONS = (24, 20, 20)
-
-
 def _axis_of_pair(case):
-    """Axis of each of the 64 rotation pairs: the sections in blocks, or interleaved."""
+    """Axis of each of the 64 rotation pairs; sections of 24, 20 and 20 pairs, in blocks or interleaved."""
+    sections = (24, 20, 20)
     if case["interleaved"]:
-        return [i % 3 if i < 3 * SECTIONS[i % 3] else 0 for i in range(D // 2)]
-    return [0] * SECTIONS[0] + [1] * SECTIONS[1] + [2] * SECTIONS[2]
+        return [i % 3 if i < 3 * sections[i % 3] else 0 for i in range(D // 2)], sections
+    return [0] * sections[0] + [1] * sections[1] + [2] * sections[2], sections
 
 
 def _inputs(case, seed):
@@ -343,7 +341,7 @@ def _run_own(st):
         return st["out"]
     if case["op"] == "append":
         dec.chunk_append(0, case["rows"], st["slots_dev"].data_ptr(), st["pos_dev"].data_ptr(), st["axes"].data_ptr(),
-                         SECTIONS, case["interleaved"], st["qkv"].data_ptr(), st["q_out"].data_ptr(),
+                         _axis_of_pair(case)[1], case["interleaved"], st["qkv"].data_ptr(), st["q_out"].data_ptr(),
                          st["pkg"].F32 if case["kv"] == "f32" else st["pkg"].BF16, stream)
         return {"q": st["q_out"], "pool": st["pool"]}
     if case["op"] == "copy":
@@ -397,7 +395,7 @@ def _run_plain(st):
         return out
     if case["op"] == "append":
         n = case["rows"]
-        axis = torch.tensor(_axis_of_pair(case), device="cuda")
+        axis = torch.tensor(_axis_of_pair(case)[0], device="cuda")
         freq = THETA ** (-2.0 * torch.arange(D // 2, device="cuda", dtype=torch.float64) / D)
         angle = st["axes"].T[:, axis].double() * freq
         cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
@@ -456,7 +454,7 @@ def exact(case, seed):
                 out[first:first + m, dims] = torch.einsum("rt,td->rd", torch.softmax(logit, 1), v[:, h // GROUP].double())
         return out
     n = case["rows"]
-    axis = _axis_of_pair(case)
+    axis, _ = _axis_of_pair(case)
     turn = torch.empty((n, D // 2), dtype=torch.complex128, device="cuda")
     for i in range(D // 2):
         turn[:, i] = torch.exp(1j * (st["axes"][axis[i]].double() * THETA ** (-i / (D / 2))))
