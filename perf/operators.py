@@ -277,6 +277,18 @@ def _wrap(owner, ptr, shape, dtype):
     return torch.as_tensor(_Memory(owner, ptr, nbytes), device="cuda").view(dtype).view(shape)
 
 
+def _host_lists(*lists):
+    """A call's lists, which change from call to call, in pinned host memory; the call uploads them."""
+    return [len(x) for x in lists], torch.tensor([v for x in lists for v in x], dtype=torch.int32).pin_memory()
+
+
+def _upload(lists):
+    """One copy to the device: (what keeps it alive, the address of each list)."""
+    sizes, host = lists
+    dev = host.to("cuda", non_blocking=True)
+    return dev, [dev.data_ptr() + 4 * sum(sizes[:i]) for i in range(len(sizes))]
+
+
 def _own_state(case, st):
     """The same inputs in a decoder handle: its streams, and its pool filled."""
     import __graft_entry__
@@ -304,10 +316,10 @@ def _own_state(case, st):
         _wrap(dec, info["scales"], tuple(st["scales"].shape), torch.float32).copy_(st["scales"])
     st["dec"], st["pkg"] = dec, pkg
     if case["op"] == "attend":
-        st["slots_dev"], st["starts_dev"], st["lens_dev"] = _i32(streams), _i32(st["starts"]), _i32(lens)
+        st["lists"] = _host_lists(streams, st["starts"], lens)
         st["out"] = torch.empty_like(st["q"])
     elif case["op"] == "append":
-        st["slots_dev"], st["pos_dev"] = _i32([streams[s] for s in st["slot_of"]]), _i32(st["pos_of"])
+        st["lists"] = _host_lists([streams[s] for s in st["slot_of"]], st["pos_of"])
         st["q_out"] = torch.empty((case["rows"], HQ * D), dtype=DTYPES[case["kv"]], device="cuda")
     elif case["op"] == "move":
         n, shape = len(st["shape"]), st["shape"]
@@ -336,11 +348,13 @@ def _run_own(st):
     stream = torch.cuda.current_stream().cuda_stream or None
     if case["op"] == "attend":
         mask = st["mask"].data_ptr() if case["tree"] else None
-        dec.chunk_attend(0, len(st["lens"]), st["slots_dev"].data_ptr(), st["starts_dev"].data_ptr(),
-                         st["lens_dev"].data_ptr(), st["rows"], mask, st["q"].data_ptr(), st["out"].data_ptr(), stream)
+        keep, (slots, starts, lens) = _upload(st["lists"])
+        dec.chunk_attend(0, len(st["lens"]), slots, starts, lens, st["rows"], mask, st["q"].data_ptr(),
+                         st["out"].data_ptr(), stream)
         return st["out"]
     if case["op"] == "append":
-        dec.chunk_append(0, case["rows"], st["slots_dev"].data_ptr(), st["pos_dev"].data_ptr(), st["axes"].data_ptr(),
+        keep, (slots, pos) = _upload(st["lists"])
+        dec.chunk_append(0, case["rows"], slots, pos, st["axes"].data_ptr(),
                          _axis_of_pair(case)[1], case["interleaved"], st["qkv"].data_ptr(), st["q_out"].data_ptr(),
                          st["pkg"].F32 if case["kv"] == "f32" else st["pkg"].BF16, stream)
         return {"q": st["q_out"], "pool": st["pool"]}
