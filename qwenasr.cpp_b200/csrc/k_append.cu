@@ -48,6 +48,15 @@ __global__ void page_gather_kernel(const TC *pool, const int *pages, int n_pages
     }
 }
 
+// Page-table entries -> their places: a block per run.  The entries come as
+// arguments, so that they are those of the launch however late it runs.
+__global__ void page_table_patch_kernel(const __grid_constant__ PageTablePatch p) {
+    const PageTableRun r = p.runs[blockIdx.x];
+    int *row = p.table + static_cast<size_t>(r.slot) * p.maxp + r.first;
+    for (int k = threadIdx.x; k < r.count; k += blockDim.x) row[k] = p.pages[r.start + k];
+}
+static_assert(sizeof(PageTablePatch) <= 4096, "kernel arguments");
+
 __device__ __forceinline__ uint64_t mix64(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
@@ -121,6 +130,13 @@ cudaError_t launch_page_gather(const void *pool, int kv_dtype, const int *pages,
             break;
         default: return cudaErrorInvalidValue;
     }
+    return cudaGetLastError();
+}
+
+// Launched without the programmatic attribute: kernels before it still read the entries that it replaces.
+cudaError_t launch_page_table_patch(const PageTablePatch &p, cudaStream_t st) {
+    if (p.n_runs <= 0) return cudaSuccess;
+    page_table_patch_kernel<<<p.n_runs, 128, 0, st>>>(p);
     return cudaGetLastError();
 }
 

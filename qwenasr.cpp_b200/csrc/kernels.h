@@ -185,6 +185,20 @@ struct PagesCopyParams {
     DevError *err;
 };
 
+// Page-table entries by value, at most 4 KB of kernel arguments: run i puts
+// pages[start .. start + count) at entries first .. of stream slot's row.
+struct PageTableRun {
+    int slot, first, count, start;
+};
+struct PageTablePatch {
+    static constexpr int kRuns = 64, kPages = 760;
+    int *table;                // [max_streams][maxp]
+    int maxp;
+    int n_runs;
+    PageTableRun runs[kRuns];
+    int pages[kPages];
+};
+
 struct TokensMoveParams {
     int n;                     // groups
     int rows;                  // entries of keep
@@ -232,6 +246,7 @@ cudaError_t launch_prefill_attn_tc(const PrefillAttnParams &p, int kv_dtype, con
 cudaError_t launch_q_to16(const float *q, int n, float scale, bool f16, void *out, cudaStream_t st);
 cudaError_t launch_page_gather(const void *pool, int kv_dtype, const int *pages, int n_pages_row, int len,
                                int n_pages, void *k_out, void *v_out, DevError *err, cudaStream_t st);
+cudaError_t launch_page_table_patch(const PageTablePatch &p, cudaStream_t st);
 cudaError_t launch_page_fill(void *pool_layer, float *scales_layer, int kv_dtype, const int *pages, int n,
                              uint64_t seed, cudaStream_t st);
 

@@ -633,6 +633,58 @@ int upload_items(qkv_handle *h, int n, const int32_t *lens, const int *base, int
     return QKV_OK;
 }
 
+// Page-table entries on their way to the device.  They travel as kernel
+// arguments: a copy from the host mirror would read it when it runs, behind
+// whatever the stream still has to do, and calls made in the meantime change it.
+class PageTableWriter {
+public:
+    PageTableWriter(qkv_handle *h, cudaStream_t st) : h_(h), st_(st) {
+        p_.table = h->d_page_table;
+        p_.maxp = h->maxp;
+        p_.n_runs = 0;
+    }
+    // Entries [first, last) of stream s, as the mirror has them now.
+    int put(int32_t s, size_t first, size_t last) {
+        const int *row = h_->h_page_table + static_cast<size_t>(s) * h_->maxp;
+        while (first < last) {
+            if (p_.n_runs == PageTablePatch::kRuns || used_ == PageTablePatch::kPages) {
+                const int rc = flush();
+                if (rc) return rc;
+            }
+            const int count = static_cast<int>(std::min<size_t>(last - first, static_cast<size_t>(PageTablePatch::kPages - used_)));
+            p_.runs[p_.n_runs++] = {s, static_cast<int>(first), count, used_};
+            std::copy(row + first, row + first + count, p_.pages + used_);
+            used_ += count;
+            first += static_cast<size_t>(count);
+        }
+        return QKV_OK;
+    }
+    int flush() {
+        if (p_.n_runs == 0) return QKV_OK;
+        qkv_handle *h = h_;
+        CK(launch_page_table_patch(p_, st_));
+        h->launches += 1;
+        p_.n_runs = used_ = 0;
+        return QKV_OK;
+    }
+
+private:
+    qkv_handle *h_;
+    cudaStream_t st_;
+    PageTablePatch p_;
+    int used_ = 0;
+};
+
+// The handle's own stream waits for what `st` holds so far.  So close, compact
+// and extend, which work on it, never overtake page-table entries of a caller's
+// stream.
+int follow(qkv_handle *h, cudaStream_t st) {
+    if (st == h->stream) return QKV_OK;
+    CK(cudaEventRecord(h->order_ev, st));
+    CK(cudaStreamWaitEvent(h->stream, h->order_ev, 0));
+    return QKV_OK;
+}
+
 // Grow each row's stream by `tokens` (pages from the pager) and push changed
 // page-table rows to the device.
 int grow_streams(qkv_handle *h, int n, const int32_t *streams, const int32_t *tokens, cudaStream_t st) {
@@ -651,6 +703,7 @@ int grow_streams(qkv_handle *h, int n, const int32_t *streams, const int32_t *to
                                                  std::to_string(h->pager->free_pages()) + ")");
     }
     std::vector<int32_t> added;
+    PageTableWriter table(h, st);
     for (int i = 0; i < n; ++i) {
         added.clear();
         std::string e;
@@ -661,11 +714,13 @@ int grow_streams(qkv_handle *h, int n, const int32_t *streams, const int32_t *to
             const size_t first = pg->size() - added.size();
             int *row = h->h_page_table + static_cast<size_t>(streams[i]) * h->maxp;
             for (size_t k = first; k < pg->size(); ++k) row[k] = (*pg)[k];
-            CK(cudaMemcpyAsync(h->d_page_table + static_cast<size_t>(streams[i]) * h->maxp + first, row + first,
-                               added.size() * sizeof(int), cudaMemcpyHostToDevice, st));
+            const int put = table.put(streams[i], first, pg->size());
+            if (put != QKV_OK) return put;
         }
     }
-    return QKV_OK;
+    if (need == 0) return QKV_OK;
+    const int rc = table.flush();
+    return rc ? rc : follow(h, st);
 }
 
 // Pinned staging for the per-call row arrays.  A slot is reused only after the
@@ -876,14 +931,10 @@ int apply_pages(qkv_handle *h, int32_t s, size_t first, size_t last, int copy_sr
     const std::vector<int32_t> *pg = h->pager->pages(s);
     int *row = h->h_page_table + static_cast<size_t>(s) * h->maxp;
     for (size_t k = first; k < last; ++k) row[k] = k < pg->size() ? (*pg)[k] : -1;
-    if (last > first)
-        CK(cudaMemcpyAsync(h->d_page_table + static_cast<size_t>(s) * h->maxp + first, row + first,
-                           (last - first) * sizeof(int), cudaMemcpyHostToDevice, st));
-    if (st != h->stream) {
-        CK(cudaEventRecord(h->order_ev, st));
-        CK(cudaStreamWaitEvent(h->stream, h->order_ev, 0));
-    }
-    return QKV_OK;
+    PageTableWriter table(h, st);
+    int rc = table.put(s, first, last);
+    if (rc == QKV_OK) rc = table.flush();
+    return rc ? rc : follow(h, st);
 }
 
 // Calls that change the page lists on the host cannot be part of a captured graph.

@@ -58,11 +58,13 @@ struct qkv_handle {
     int n_pages = 0;
     int maxp = 0;               // pages per stream
     int *d_page_table = nullptr;
-    int *h_page_table = nullptr;    // pinned mirror [max_streams][maxp]
+    // Mirror [max_streams][maxp].  Pinned: close and compact copy from it, and wait for their copy; entries that
+    // nothing waits for go as kernel arguments.
+    int *h_page_table = nullptr;
     float2 *d_rope = nullptr;
     int rope_len = 0;
     double *d_turns = nullptr;  // [kHeadDim/2] rotary frequencies in turns per position
-    cudaEvent_t order_ev = nullptr;   // orders the handle's stream behind a caller's (fork, truncate)
+    cudaEvent_t order_ev = nullptr;   // orders the handle's stream behind a caller's (page-table changes)
     qkv::Pager *pager = nullptr;
 
     // scratch (rows = max(max_batch_tokens, max_streams))
