@@ -124,8 +124,9 @@ int qkv_pool_stats(const qkv_handle *h, int64_t *free_pages, int64_t *total_page
  * prompt, a beam, a draft): full pages are shared, each freed with its last
  * holder, and a partly filled last page is copied.  src keeps everything.  The
  * copy and the page-table entries are ordered on `stream` (NULL = the legacy
- * default stream), which must be the one that wrote src's tokens, and before
- * every later model-level call; nothing is synchronised.  A shared page is
+ * default stream), which must be the one that wrote src's tokens, behind the
+ * handle's earlier forks and truncates (on whatever streams) and before every
+ * later model-level call; nothing is synchronised.  A shared page is
  * read-only: do not append at a position below `tokens` of either stream.
  * After a fork at src's full length a decode step may continue from src's
  * last greedy id.  QKV_ERR_CAPACITY / QKV_ERR_OUT_OF_PAGES without a free

@@ -685,6 +685,15 @@ int follow(qkv_handle *h, cudaStream_t st) {
     return QKV_OK;
 }
 
+// `st` waits for the last page-table change on any stream: pages that a
+// truncate gave back may still be read by calls enqueued before it, on its
+// stream.  Before every change on `st` (and `follow` behind it), so that the
+// changes stand one behind the other.
+int wait_for_pages(qkv_handle *h, cudaStream_t st) {
+    if (st != h->stream) CK(cudaStreamWaitEvent(st, h->order_ev, 0));
+    return QKV_OK;
+}
+
 // Grow each row's stream by `tokens` (pages from the pager) and push changed
 // page-table rows to the device.
 int grow_streams(qkv_handle *h, int n, const int32_t *streams, const int32_t *tokens, cudaStream_t st) {
@@ -701,6 +710,10 @@ int grow_streams(qkv_handle *h, int n, const int32_t *streams, const int32_t *to
     if (need > h->pager->free_pages()) {
         return fail(h, QKV_ERR_OUT_OF_PAGES, "KV pool out of pages (need " + std::to_string(need) + ", free " +
                                                  std::to_string(h->pager->free_pages()) + ")");
+    }
+    if (need > 0) {
+        const int rc = wait_for_pages(h, st);
+        if (rc) return rc;
     }
     std::vector<int32_t> added;
     PageTableWriter table(h, st);
@@ -920,6 +933,8 @@ PagesCopyParams pages_copy_params(qkv_handle *h) {
 // The page copy and page-table entries [first, last) of a stream that fork or
 // truncate left to do, on the caller's stream; the handle's own stream follows.
 int apply_pages(qkv_handle *h, int32_t s, size_t first, size_t last, int copy_src, int copy_dst, cudaStream_t st) {
+    int rc = wait_for_pages(h, st);
+    if (rc) return rc;
     if (copy_src >= 0) {
         PagesCopyParams pc = pages_copy_params(h);
         pc.n = 1;
@@ -932,7 +947,7 @@ int apply_pages(qkv_handle *h, int32_t s, size_t first, size_t last, int copy_sr
     int *row = h->h_page_table + static_cast<size_t>(s) * h->maxp;
     for (size_t k = first; k < last; ++k) row[k] = k < pg->size() ? (*pg)[k] : -1;
     PageTableWriter table(h, st);
-    int rc = table.put(s, first, last);
+    rc = table.put(s, first, last);
     if (rc == QKV_OK) rc = table.flush();
     return rc ? rc : follow(h, st);
 }

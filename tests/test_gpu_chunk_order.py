@@ -149,3 +149,30 @@ def test_step_that_grows_then_truncate_and_close_without_waiting(pkg):
         dec.sync()
         assert torch.equal(outs[0], outs[1]) and not (outs[1] == -77).all(-1).any()
         assert dec.length(a) == 96 and len(dec.pages(a)) == 96 // PT
+
+
+@pytest.mark.parametrize("taker", ["fork", "step"])
+def test_pages_given_back_on_one_stream_and_taken_on_another(pkg, taker):
+    """The taker's stream is idle, and its copy or token goes into a page that a waiting attention has yet to read."""
+    with Cache(pkg, "bf16", [64, 40], max_streams=3, spare=0, max_context=80) as c:
+        c.fill()
+        dec, (a, b), st, other = c.dec, c.streams, torch.cuda.Stream(), torch.cuda.Stream()
+        base_a, base_b = [[t.clone() for t in c.values(0, s, n)] for s, n in ((a, 64), (b, 40))]
+        qkv, out = torch.zeros((1, 1, QKV), device="cuda"), torch.zeros((1, 1, HQ * D), device="cuda")
+        q = Queue(c, st)
+        q.prepare(1)
+        q.lists_of(b, 40, 5)
+        was = set(int(x) for x in dec.pages(b))
+        busy(st)
+        q.attend(b, 40, base_b)
+        dec.truncate(b, 0, st.cuda_stream)
+        if taker == "fork":
+            s = dec.fork(a, 20, other.cuda_stream)
+        else:
+            dec.kv_step([a], qkv.data_ptr(), out.data_ptr(), other.cuda_stream)
+            s = a
+        assert int(dec.pages(s)[-1]) in was and not st.query()
+        dec.sync()
+        q.check()
+        n = 20 if taker == "fork" else 64
+        assert all(torch.equal(x[:n], y[:n]) for x, y in zip(c.values(0, s, n), base_a))
