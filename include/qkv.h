@@ -341,7 +341,8 @@ int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
  * A row that sees nothing gives zeros.  q and out: [rows][Hq*D] bf16, 16-byte
  * aligned, q post-RoPE and unscaled; rows outside every chunk are left as they
  * are.  K and V of the lens[i] tokens must be finite, V below 2^64 in
- * magnitude; what lies behind them does not matter.  A slot may be listed more
+ * magnitude, an 8-bit cache's scales not negative; what lies behind them does
+ * not matter.  A slot may be listed more
  * than once.  An entry that breaks these rules is reported (qkv_sync) and
  * skipped; one whose lens[i] reaches pages that the stream does not have is
  * reported, and its rows are not defined.  QKV_ERR_STATE for an f32 cache

@@ -984,7 +984,10 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                                         (t >> 4) * (2 * kPageTokens) + (t & 15);
                 const bool live = kt * kKeys + t < s.len_end;
                 const uint32_t ring = tile % L::kScaleRing;
-                scale_ring[ring * 2 * kKeys + t] = live ? rs[0] * p.scale_log2 : 1.0f;   // (masked: times -infinity)
+                // A hidden key's score, -infinity, is multiplied by this, so it must not be zero: a vector stored with
+                // scale 0 gets the least f32 instead, which moves a finite score by 2^-21 at most.
+                const float fk = rs[0] * p.scale_log2;
+                scale_ring[ring * 2 * kKeys + t] = !live ? 1.0f : (fk != 0.0f ? fk : __uint_as_float(1u));
                 scale_ring[ring * 2 * kKeys + kKeys + t] = live ? rs[kPageTokens] : 0.0f;
                 mbar_arrive(&tail->scale_full[ring]);
             }
