@@ -338,7 +338,8 @@ int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
  * cached tokens, already appended.  Each row sees the tokens before the chunk
  * and, inside it, those up to its own; with mask (uint64 per row, nullable;
  * chunks of at most 64 rows), bit b says whether it sees the chunk's token b.
- * A row that sees nothing gives zeros.  q and out: [rows][Hq*D] bf16, 16-byte
+ * A row that sees nothing (or whose scores are all -infinity) gives zeros, one
+ * with a score of NaN or +infinity NaN, in the heads concerned.  q and out: [rows][Hq*D] bf16, 16-byte
  * aligned, q post-RoPE and unscaled; rows outside every chunk are left as they
  * are.  K and V of the lens[i] tokens must be finite, V below 2^64 in
  * magnitude, an 8-bit cache's scales not negative; what lies behind them does

@@ -4,6 +4,9 @@
 //
 // out[r] = sum_k softmax_k(q_r . k / sqrt(128)) v over the visible tokens; zero
 // where none is visible.  bf16 and 8-bit caches, tensor cores (tcgen05, TMEM).
+// A sum of exponentials is 0 only where nothing is visible (or every score is
+// -infinity), so every division and skip asks for 0 and lets a NaN, from scores
+// of NaN or +infinity, through to its row.
 //
 // A K/V tile is 128 keys (8 pages) of one kv head g, fetched once for the two q
 // heads it serves.  Two lanes (a softmax warpgroup, an S region and an O region
@@ -1419,9 +1422,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
             if (l == 0 && r < kCols) {
                 const float2 v0 = tail->ml[0][r], v1 = n > 1 ? tail->ml[1][r] : make_float2(-INFINITY, 0.0f);
                 const float m = fmaxf(v0.x, v1.x);
-                const float a0 = v0.y > 0.0f ? ex2_approx(v0.x - m) : 0.0f, a1 = v1.y > 0.0f ? ex2_approx(v1.x - m) : 0.0f;
+                const float a0 = v0.y != 0.0f ? ex2_approx(v0.x - m) : 0.0f, a1 = v1.y != 0.0f ? ex2_approx(v1.x - m) : 0.0f;
                 const float sum = a0 * v0.y + a1 * v1.y;
-                const float norm = whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+                const float norm = whole ? (sum != 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
                 factor[r] = make_float2(a0 * norm, a1 * norm);
                 if (!whole && r < real) p.part_ml[piece * kPieceRows + r] = make_float2(m, sum);
             }
@@ -1491,14 +1494,14 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                     bar_sync(kBarBoth, 256);
                     const float2 v0 = tail->ml[0][r], v1 = n > 1 ? tail->ml[1][r] : make_float2(-INFINITY, 0.0f);
                     m_tot = fmaxf(v0.x, v1.x);
-                    a0 = v0.y > 0.0f ? ex2_approx(v0.x - m_tot) : 0.0f;
-                    a1 = v1.y > 0.0f ? ex2_approx(v1.x - m_tot) : 0.0f;
+                    a0 = v0.y != 0.0f ? ex2_approx(v0.x - m_tot) : 0.0f;
+                    a1 = v1.y != 0.0f ? ex2_approx(v1.x - m_tot) : 0.0f;
                     l_tot = a0 * v0.y + a1 * v1.y;
                 }
                 fence_after();
                 const bool real = r < 2 * nq && !*failed;
                 if (active) {
-                    const float norm = whole ? (l_tot > 0.0f ? 1.0f / l_tot : 0.0f) : 1.0f;
+                    const float norm = whole ? (l_tot != 0.0f ? 1.0f / l_tot : 0.0f) : 1.0f;
                     a0 *= norm;
                     a1 *= norm;
                     const int c0 = s.pair() ? 0 : 2 * l, c1 = s.pair() ? 4 : c0 + 2;   // 32-column chunks
@@ -1613,14 +1616,14 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_c
                 float top = m;
 #pragma unroll
                 for (int b = 0; b < kJoinBatch; ++b) top = ml[b].y > 0.0f ? fmaxf(top, ml[b].x) : top;
-                const float keep = l > 0.0f ? exp2f(m - top) : 0.0f;
+                const float keep = l != 0.0f ? exp2f(m - top) : 0.0f;
                 m = top;
                 l *= keep;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) o[q] *= keep;
 #pragma unroll
                 for (int b = 0; b < kJoinBatch; ++b) {
-                    if (!(ml[b].y > 0.0f)) continue;   // (a piece that saw nothing of the row)
+                    if (ml[b].y == 0.0f) continue;   // (a piece that saw nothing of the row)
                     const float a = exp2f(ml[b].x - m);
                     l += a * ml[b].y;
                     o[0] += a * v[b].x;
@@ -1629,7 +1632,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_c
                     o[3] += a * v[b].w;
                 }
             }
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
             uint16_t *out = p.out + static_cast<size_t>(d.row0 + (r >> 1)) * kQDim + (2 * d.g + (r & 1)) * kHeadDim + 4 * c;
             *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
         }

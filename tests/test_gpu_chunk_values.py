@@ -5,7 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_chunk import D, HQ, PT, Cache, check_attend, run_attend, to_i64  # noqa: E402,F401
+from test_gpu_chunk import (D, HQ, PT, Cache, attend_oracle, attend_tolerance, check_attend, run_attend,  # noqa: E402
+                            visible)
 
 # rows of one call: up to 16, up to 64 and up to 128 at a time take three paths through the kernel; the long contexts
 # are cut between SMs, the short ones are not
@@ -42,3 +43,36 @@ def test_attend_vectors_with_scale_zero(pkg, kv, masked):
         q = queries(starts[-1])
         out = run_attend(c, chunks, q, starts, masks)
         check_attend(c, chunks, q, starts, out, masks)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "e4i8"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attend_queries_that_are_not_finite(pkg, kv, masked):
+    """NaN and infinite queries give NaN in their own row and head, as the formula does, and nothing elsewhere."""
+    chunks = [c for c in CHUNKS if c[1] <= 64] if masked else CHUNKS
+    lens, starts = layout(chunks)
+    masks = [(1 << (j + 1)) - 1 if j % 7 != 3 else 0 for _, m in chunks for j in range(m)] if masked else None
+    with Cache(pkg, kv, lens) as c:
+        c.fill()
+        c.poison_behind(lens)
+        clean = queries(starts[-1])
+        q = clean.clone().view(-1, HQ, D)
+        hit = torch.zeros((starts[-1], HQ), dtype=torch.bool, device="cuda")
+        for j, (base, m) in enumerate(chunks):
+            k, _ = c.values(0, c.streams[j], base + m)
+            for r, head, value in ((0, 3, "nan"), (1, 0, "first"), (m // 2, 8, "nan"), (m // 2, 15, "first"), (m - 1, 14, "last")):
+                # infinity with the sign of one visible token's key: that score is +infinity
+                token = 0 if value == "first" else base - 1
+                inf = float("inf") if k[token, head // 2, 77] >= 0 else -float("inf")
+                q[starts[j] + r, head, 77] = float("nan") if value == "nan" else inf
+                hit[starts[j] + r, head] = True
+        q = q.view(-1, HQ * D)
+        out = run_attend(c, chunks, q, starts, masks)
+        for j, (base, m) in enumerate(chunks):
+            rows = slice(starts[j], starts[j + 1])
+            k, v = c.values(0, c.streams[j], base + m)
+            seen = visible(base, m, masks[rows] if masks else None)
+            want, mag = attend_oracle(clean[rows].double().view(m, HQ, D), k, v, seen)
+            got, bad = out[rows].double().view(m, HQ, D), hit[rows]
+            assert torch.isnan(got[bad]).all(), (j, base, m)
+            assert not ((got - want).abs() > attend_tolerance(want, mag))[~bad].any() and torch.isfinite(got[~bad]).all(), (j, base, m)
