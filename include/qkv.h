@@ -364,8 +364,9 @@ int qkv_pages_copy(qkv_handle *h, int32_t n, const int32_t *src_dev, const int32
  * included: of group i (n <= 65535), token src_bases[i] + keep[starts[i] + k]
  * of stream src_slots[i] goes to position dst_bases[i] + k of stream
  * dst_slots[i].  keep[rows] ascends within a group.  The two streams may be the
- * same with dst_bases[i] <= src_bases[i]: the accepted path of a draft tree
- * moves together before qkv_stream_truncate drops the rest.  Groups must not
+ * same, or share the pages written to after a fork, with dst_bases[i] <=
+ * src_bases[i]: the accepted path of a draft tree moves together before
+ * qkv_stream_truncate drops the rest.  Groups must not
  * touch each other's tokens, and pages that streams share after a fork are
  * written for all of them.  A group outside these rules is reported and not
  * moved. */

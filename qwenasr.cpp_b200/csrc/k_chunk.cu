@@ -236,9 +236,9 @@ static_assert(kPageHalfElems * 2 % kCopyBlockBytes == 0, "a page of any cache ty
 // Group i: its k-th listed token, (src_slots[i], src_bases[i] + keep[starts[i]
 // + k]), goes to (dst_slots[i], dst_bases[i] + k), in every layer.  Each thread
 // owns one 16-byte piece of the token vectors of one (layer, K|V) and takes the
-// tokens in order, eight loads before their stores; within one stream the list
-// ascends and targets lie at or below their sources, so no store reaches a
-// token that is still to be read.  Bound by latency for one stream (a chain of
+// tokens in order, eight loads before their stores; within one stream, and in
+// pages that the two streams share, the list ascends and targets lie at or below
+// their sources, so no store reaches a token that is still to be read.  Bound by latency for one stream (a chain of
 // three dependent loads), by memory for many.
 constexpr int kMoveBatch = 8;
 
@@ -267,6 +267,8 @@ __global__ void __launch_bounds__(kHkv * kHeadDim * kElem / 16) tokens_move_kern
             }
             const int pa = from_pt[a / kPageTokens], pb = to_pt[b / kPageTokens];
             if (pa < 0 || pa >= p.n_pages || pb < 0 || pb >= p.n_pages) bad = true;
+            // Streams share pages at equal places only: is the target's page a page of the source stream, too?
+            if (to_base > from_base && pb == from_pt[b / kPageTokens]) bad = true;
         }
     }
     if (__syncthreads_or(bad)) {   // every block of the group decides alike: nothing of it moves

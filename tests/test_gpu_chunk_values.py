@@ -5,8 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_chunk import (D, HQ, PT, Cache, attend_oracle, attend_tolerance, check_attend, run_attend,  # noqa: E402
-                            visible)
+from test_gpu_chunk import (D, HQ, PT, Cache, attend_oracle, attend_tolerance, check_attend, raw, run_attend,  # noqa: E402
+                            run_move, visible)
 
 # rows of one call: up to 16, up to 64 and up to 128 at a time take three paths through the kernel; the long contexts
 # are cut between SMs, the short ones are not
@@ -76,3 +76,36 @@ def test_attend_queries_that_are_not_finite(pkg, kv, masked):
             got, bad = out[rows].double().view(m, HQ, D), hit[rows]
             assert torch.isnan(got[bad]).all(), (j, base, m)
             assert not ((got - want).abs() > attend_tolerance(want, mag))[~bad].any() and torch.isfinite(got[~bad]).all(), (j, base, m)
+
+
+@pytest.mark.parametrize("kv", ["f32", "bf16", "e4i8"])
+def test_tokens_move_between_streams_that_share_pages(pkg, kv):
+    """Down within shared pages: as within one stream.  Up into them: reported, nothing moves.  Past them: any way."""
+    with Cache(pkg, kv, [90], layers=2, max_streams=2, spare=8, max_context=128) as c:
+        c.fill()
+        dec, a = c.dec, c.streams[0]
+        b = dec.fork(a, 70)                    # four shared pages, the fifth of its own
+        dec.sync()
+        before, sc = c.pool.clone(), c.scales.clone() if c.scales is not None else None
+        for g in ((a, 3, b, 10, list(range(0, 30))), (a, 0, b, 1, [0]), (b, 20, a, 60, list(range(0, 20)))):
+            with pytest.raises(pkg.QkvError) as ei:
+                run_move(c, [g])
+            assert ei.value.code == 5
+            assert torch.equal(raw(c.pool), raw(before)) and (sc is None or torch.equal(c.scales, sc)), g
+        for src, from_base, dst, to_base, keep in ((a, 30, b, 10, list(range(0, 40, 2))), (b, 5, a, 0, list(range(0, 60))),
+                                                   (a, 3, b, 64, [0, 2, 30, 61, 66])):
+            want = [[t.clone() for t in c.values(1, s, 70)] for s in (a, b)]
+            n, at = len(keep), [from_base + t for t in keep]
+            for s, kv_of in ((a, want[0]), (b, want[1])):
+                for x, y in zip(want[0 if src == a else 1], kv_of):
+                    moved = x[at].clone() if s == dst else None
+                    if s == dst:
+                        y[to_base:to_base + n] = moved
+            shared = 64                        # what one stream has there, the other has
+            if to_base < shared:
+                for x, y in zip(want[0 if dst == a else 1], want[1 if dst == a else 0]):
+                    y[to_base:min(to_base + n, shared)] = x[to_base:min(to_base + n, shared)]
+            run_move(c, [(src, from_base, dst, to_base, keep)])
+            for s, kv_of in ((a, want[0]), (b, want[1])):
+                for x, y in zip(c.values(1, s, 70), kv_of):
+                    assert torch.equal(x, y), (src, dst, to_base)
