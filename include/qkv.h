@@ -393,8 +393,10 @@ int qkv_kv_step_host(qkv_handle *h, int32_t n, const int32_t *stream_ids, const 
                      float *out_host);
 
 /* Grow an open stream's length by `tokens` without writing K/V (pages are
- * allocated; their contents are whatever the pool holds).  For benches that
- * need long contexts quickly. */
+ * allocated; their contents are whatever the pool holds).  For chunks of tokens
+ * that qkv_chunk_append then writes, and benches that need long contexts
+ * quickly.  The next decode step needs in_ids: the stream's last greedy id
+ * followed the tokens before these. */
 int qkv_stream_extend(qkv_handle *h, int32_t stream_id, int32_t tokens);
 
 /* Fill every page currently owned by open streams, in every layer, with

@@ -2263,6 +2263,7 @@ int qkv_stream_extend(qkv_handle *h, int32_t stream_id, int32_t tokens) {
     CK(cudaSetDevice(h->device));
     int rc = grow_streams(h, 1, &stream_id, &tokens, h->stream);
     if (rc) return rc;
+    if (tokens > 0) h->last_id[static_cast<size_t>(stream_id)] = -1;   // it followed the tokens before these
     CK(cudaStreamSynchronize(h->stream));
     return QKV_OK;
 }

@@ -1,5 +1,6 @@
 """Streams that fork, give tokens back and grow while earlier calls still wait on the caller's stream: each call sees
 the page table and the pages as they were when it was enqueued."""
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -176,3 +177,26 @@ def test_pages_given_back_on_one_stream_and_taken_on_another(pkg, taker):
         q.check()
         n = 20 if taker == "fork" else 64
         assert all(torch.equal(x[:n], y[:n]) for x, y in zip(c.values(0, s, n), base_a))
+
+
+def test_decode_after_extend_needs_ids(pkg, synth, tiny_files):
+    """The greedy id from before a chunk does not follow it: not in the stream, and not in a fork of it."""
+    _, files = tiny_files
+    path = files[("bf16", "one_plus")]
+    x, _ = synth.prompt_rows(synth.read_gguf(path)["text.token_embd.weight"], 20, np.random.default_rng(3), audio_rows=8,
+                             audio_start=4)
+    rt = pkg.runtime_config(device=0, weight_dtype=pkg.BF16, kv_dtype=pkg.BF16, max_streams=2, max_context=64)
+    with pkg.Decoder.from_gguf(path, rt) as dec:
+        a = dec.open()
+        first = int(dec.prefill([a], [x])[0])
+        dec.extend(a, 0)
+        dec.decode_step([a])
+        dec.extend(a, 3)
+        dec.truncate(a, 24)                    # everything accepted
+        b = dec.fork(a, 24)
+        for s in (a, b):
+            with pytest.raises(pkg.QkvError) as ei:
+                dec.decode_step([s])
+            assert ei.value.code == 1 and dec.length(s) == 24
+        ids = dec.decode_step([a, b], in_ids=[first, first])
+        assert ids[0] == ids[1] and dec.decode_step([a]) is not None
