@@ -130,13 +130,15 @@ int qkv_pool_stats(const qkv_handle *h, int64_t *free_pages, int64_t *total_page
  * read-only: do not append at a position below `tokens` of either stream.
  * After a fork at src's full length a decode step may continue from src's
  * last greedy id.  QKV_ERR_CAPACITY / QKV_ERR_OUT_OF_PAGES without a free
- * slot / page, QKV_ERR_STATE while `stream` is captured; nothing changed
- * then. */
+ * slot / page, QKV_ERR_STATE while `stream` is captured, QKV_ERR_CUDA when a
+ * CUDA call failed; there is no new stream then and src is as it was. */
 int qkv_stream_fork(qkv_handle *h, int32_t src, int32_t tokens, int32_t *stream_id, void *stream);
 /* Give back the tokens of a stream past the first `tokens` (rejected drafts):
  * pages that only they used become free.  When the new last page is partly
  * filled and shared, the stream gets its own copy of it (one free page; the
- * ones given back count).  Ordering and refusals as for qkv_stream_fork; the
+ * ones given back count).  Ordering and refusals as for qkv_stream_fork, and the
+ * stream is as it was, but for QKV_ERR_CUDA: the tokens are given back then, the
+ * device may not know, and the stream is good for qkv_stream_close alone.  The
  * next decode step needs in_ids. */
 int qkv_stream_truncate(qkv_handle *h, int32_t stream_id, int32_t tokens, void *stream);
 /* The handle's pool in device memory, for callers that move pages in or out of

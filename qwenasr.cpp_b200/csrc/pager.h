@@ -71,4 +71,21 @@ private:
     std::vector<int32_t> free_slots_;    // stack of closed stream ids
 };
 
+// A fork with its work outside the page lists: apply(stream, copy_src, copy_dst)
+// returns a status.  When it fails the new stream is closed again, so that its
+// slot and pages are free, and *stream_id is not set.
+template <typename Apply>
+int fork_and_apply(Pager &pager, int32_t src, int32_t tokens, int32_t *stream_id, std::string *err, Apply &&apply) {
+    int32_t s = -1, from = -1, to = -1;
+    int rc = pager.fork(src, tokens, &s, &from, &to, err);
+    if (rc != 0) return rc;
+    rc = apply(s, from, to);
+    if (rc != 0) {
+        pager.close(s, nullptr);
+        return rc;
+    }
+    *stream_id = s;
+    return 0;
+}
+
 }  // namespace qkv

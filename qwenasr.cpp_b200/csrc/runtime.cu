@@ -2026,15 +2026,21 @@ int qkv_stream_fork(qkv_handle *h, int32_t src, int32_t tokens, int32_t *stream_
     if (rc) return rc;
     return host_alloc_guard(h, [&]() -> int {
         std::string e;
-        int32_t from = -1, to = -1, s = -1;
-        int r = h->pager->fork(src, tokens, &s, &from, &to, &e);
-        if (r) return fail(h, r, e);
-        // The next decode step continues from src's last greedy id only where
-        // the whole of src is shared.
-        h->last_id[static_cast<size_t>(s)] = tokens == stream_len(h, src) ? h->last_id[static_cast<size_t>(src)] : -1;
-        if ((r = apply_pages(h, s, 0, h->pager->pages(s)->size(), from, to, st))) return r;
-        *stream_id = s;
-        return QKV_OK;
+        const int r = fork_and_apply(*h->pager, src, tokens, stream_id, &e, [&](int32_t s, int32_t from, int32_t to) -> int {
+            // The next decode step continues from src's last greedy id only where
+            // the whole of src is shared.
+            h->last_id[static_cast<size_t>(s)] = tokens == stream_len(h, src) ? h->last_id[static_cast<size_t>(src)] : -1;
+            const size_t pages = h->pager->pages(s)->size();
+            const int failed = apply_pages(h, s, 0, pages, from, to, st);
+            if (failed) {   // nothing of this call may reach the pages once they are another's
+                cudaStreamSynchronize(st);
+                int *row = h->h_page_table + static_cast<size_t>(s) * h->maxp;
+                std::fill(row, row + pages, -1);
+                e = h->last_error;
+            }
+            return failed;
+        });
+        return r ? fail(h, r, e) : QKV_OK;
     });
 }
 
