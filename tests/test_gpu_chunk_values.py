@@ -109,3 +109,21 @@ def test_tokens_move_between_streams_that_share_pages(pkg, kv):
             for s, kv_of in ((a, want[0]), (b, want[1])):
                 for x, y in zip(c.values(1, s, 70), kv_of):
                     assert torch.equal(x, y), (src, dst, to_base)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_attend_one_chunk_of_many_rows(pkg, kv):
+    """A whole prompt as one chunk, and a second one behind it: rows of every block against the oracle."""
+    chunks = [(77, 9000), (0, 2500)]
+    lens, starts = layout(chunks)
+    with Cache(pkg, kv, lens) as c:
+        c.fill()
+        c.poison_behind(lens)
+        q = queries(starts[-1])
+        out = run_attend(c, chunks, q, starts)
+        for j, (base, m) in enumerate(chunks):
+            k, v = c.values(0, c.streams[j], base + m)
+            rows = torch.arange(m % 61, m, 61, device="cuda")
+            seen = torch.arange(base + m, device="cuda")[None] <= base + rows[:, None]
+            want, mag = attend_oracle(q[starts[j] + rows].double().view(-1, HQ, D), k, v, seen)
+            assert not ((out[starts[j] + rows].double().view(-1, HQ, D) - want).abs() > attend_tolerance(want, mag)).any(), j
