@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 2) chunk_append_kernel(cons
 #pragma unroll
                     for (int o = 8; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                     // scale and codes as K1 sets them (append_kv_unit)
-                    const float scale = amax > 0.0f ? __fdiv_rn(amax, i8 ? kI8Max : kE4m3Max) : 1.0f;
+                    const float scale = vector_scale(amax, i8 ? kI8Max : kE4m3Max);
                     inv_scale = amax > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
                     if (l == 0) a.scales[vec] = scale;
                 }

@@ -121,7 +121,7 @@ __device__ __forceinline__ void append_kv_unit(float (&x)[8], int kv, int g, int
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         const float qmax = (kv == 1 && v_int8) ? kI8Max : kE4m3Max;
-        const float scale = amax > 0.0f ? __fdiv_rn(amax, qmax) : 1.0f;
+        const float scale = vector_scale(amax, qmax);
         inv_scale = amax > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
         if (l16 == 0) scales[((static_cast<size_t>(page) * 2 + kv) * kHkv + g) * kPageTokens + tok] = scale;
     }

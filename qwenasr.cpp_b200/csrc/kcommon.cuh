@@ -113,6 +113,13 @@ __device__ __forceinline__ uint8_t f_to_e4m3(float v) {
     return static_cast<uint8_t>(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
 }
 constexpr float kE4m3Max = 448.0f;
+// Scale of an 8-bit vector from its largest magnitude; 1 for a zero vector.  At
+// least the smallest normal f32, whose reciprocal is still finite: below it 1 /
+// scale was infinite, and a vector's zeros became NaN codes.
+constexpr float kMinScale = 1.17549435e-38f;   // 2^-126
+__device__ __forceinline__ float vector_scale(float amax, float qmax) {
+    return amax > 0.0f ? fmaxf(__fdiv_rn(amax, qmax), kMinScale) : 1.0f;
+}
 
 // ---- int8 V of the e4m3-K / int8-V cache ----
 // A V element is one excess-128 byte u = q + 128 with q = round(v / scale)

@@ -5,8 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_chunk import (D, HQ, PT, Cache, attend_oracle, attend_tolerance, check_attend, raw, run_attend,  # noqa: E402
-                            run_move, visible)
+from test_gpu_chunk import (D, HKV, HQ, PT, QKV, Cache, append_oracle, attend_oracle,  # noqa: E402
+                            attend_tolerance, check_attend, i32, raw, run_attend, run_move, visible)
 
 # rows of one call: up to 16, up to 64 and up to 128 at a time take three paths through the kernel; the long contexts
 # are cut between SMs, the short ones are not
@@ -127,3 +127,42 @@ def test_attend_one_chunk_of_many_rows(pkg, kv):
             seen = torch.arange(base + m, device="cuda")[None] <= base + rows[:, None]
             want, mag = attend_oracle(q[starts[j] + rows].double().view(-1, HQ, D), k, v, seen)
             assert not ((out[starts[j] + rows].double().view(-1, HQ, D) - want).abs() > attend_tolerance(want, mag)).any(), j
+
+
+@pytest.mark.parametrize("kv", ["fp8", "e4i8"])
+@pytest.mark.parametrize("chunk", [True, False])
+def test_append_of_vectors_near_the_end_of_the_range(pkg, kv, chunk):
+    """8-bit caches: vectors of 1e-30 down to the smallest f32 and zeros among them; chunk_append and kv_append alike."""
+    sizes = [1e-30, 1e-35, 1e-36, 1e-37, 1e-38, 1e-40, 1e-42, 1e-44, 0.0]
+    n = len(sizes)
+    with Cache(pkg, kv, [n]) as c:
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        qkv = torch.randn((n, QKV), device="cuda", generator=gen)
+        # k goes through the norm, which divides vectors this small by sqrt(eps): 1000 times as large
+        qkv[:, HQ * D:] *= torch.tensor(sizes, device="cuda")[:, None]
+        qkv[:, HQ * D::5] = 0.0
+        slots, pos = i32([c.streams[0]] * n), i32(range(n))
+        axes = torch.zeros((3, n), dtype=torch.int32, device="cuda")
+        q = torch.empty((n, HQ * D), device="cuda")
+        if chunk:
+            c.dec.chunk_append(0, n, slots.data_ptr(), pos.data_ptr(), axes.data_ptr(), (64, 0, 0), False, qkv.data_ptr(),
+                               q.data_ptr(), pkg.F32)
+        else:
+            axes = torch.stack([pos] * 3).contiguous()
+            c.dec.kv_append(0, n, slots.data_ptr(), pos.data_ptr(), qkv.data_ptr(), q.data_ptr())
+        c.dec.sync()
+        want_k, mag = append_oracle(qkv[:, HQ * D:(HQ + HKV) * D].double().view(n, HKV, D),
+                                    torch.tensor(c.kn[0], device="cuda").double(), axes, [0] * 64)
+        want_v = qkv[:, (HQ + HKV) * D:].double().view(n, HKV, D)
+        page = int(c.dec.pages(c.streams[0])[0])
+        assert torch.isfinite(c.scales[0, page]).all() and (c.scales[0, page] > 0).all()
+        for got, want, arith, top in zip(c.values(0, c.streams[0], n), (want_k, want_v),
+                                         (2.0 ** -19 * mag + 2.0 ** -145, torch.zeros_like(want_v)),
+                                         (448.0, 127.0 if kv == "e4i8" else 448.0)):
+            assert torch.isfinite(got).all()
+            # half a step (of e4m3, or its subnormals, or int8) at the scale max(amax / top, 2^-126); the arithmetic
+            # before it, in f32 down to its subnormals; the quotient's 3 U of up to `top` steps
+            amax = want.abs().amax(-1, keepdim=True)
+            scale = (amax / top).clamp_min(2.0 ** -126)
+            step = 0.5 * scale if top == 127.0 else torch.maximum(want.abs() * 2.0 ** -4, scale * 2.0 ** -10)
+            assert not ((got - want).abs() > step * (1 + 2.0 ** -6) + 2 * arith + 2.0 ** -19 * amax).any()
