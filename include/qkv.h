@@ -245,6 +245,10 @@ int qkv_layer_forward(qkv_handle *h, int32_t layer, int32_t tokens, const float 
  * Device pointers; `stream` is the cudaStream_t to launch on (NULL = the CUDA
  * legacy default stream, as in the CUDA runtime API).  Consecutive calls on a
  * handle must use the same stream (its per-call row staging is stream-ordered).
+ * Model-level calls, qkv_stream_close and qkv_compact run on the handle's own
+ * stream, which does not wait for these calls (it does for a fork or truncate
+ * and all that `stream` holds before one): wait for them first (qkv_sync) where
+ * one needs, moves or gives back the pages of the other.
  * Rows: slots[i] is an open stream id, positions[i] its token position. */
 
 /* K1: qkv[n][Hq*D + 2*Hkv*D] f32 (raw projections) -> QK-RMSNorm + NEOX RoPE;
@@ -341,19 +345,18 @@ int qkv_chunk_append(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slo
  * and, inside it, those up to its own; with mask (uint64 per row, nullable;
  * chunks of at most 64 rows), bit b says whether it sees the chunk's token b.
  * A row that sees nothing (or whose scores are all -infinity) gives zeros, one
- * with a score of NaN or +infinity NaN, in the heads concerned.  q and out: [rows][Hq*D] bf16, 16-byte
- * aligned, q post-RoPE and unscaled; rows outside every chunk are left as they
- * are.  K and V of the lens[i] tokens must be finite, V below 2^64 in
- * magnitude, an 8-bit cache's scales not negative; what lies behind them does
- * not matter.  A slot may be listed more
- * than once.  An entry that breaks these rules is reported (qkv_sync) and
- * skipped; one whose lens[i] reaches pages that the stream does not have is
+ * with a score of NaN or +infinity NaN, in the heads concerned.  q and out:
+ * [rows][Hq*D] bf16, 16-byte aligned, q post-RoPE and unscaled; rows outside
+ * every chunk are left as they are.  K and V of the lens[i] tokens must be
+ * finite, V below 2^64 in magnitude, an 8-bit cache's scales not negative; what
+ * lies behind them does not matter.  A slot may be listed more than once.  An
+ * entry that breaks these rules is reported (qkv_sync) and skipped; one whose lens[i] reaches pages that the stream does not have is
  * reported, and its rows are not defined.  QKV_ERR_STATE for an f32 cache
  * (qkv_prefill_attend serves it), QKV_ERR_CAPACITY for more than 2^20 rows, or
- * so many with a max_context past 2^20 that their work passes 2^31 tiles.  Uses
- * the handle's workspace: calls on one handle, captured ones too, must not
- * overlap.  The prompt half of text-decoder.cpp:322-334 for any number of rows
- * at any context. */
+ * so many with a max_context past 2^20 that their work passes 2^31 tiles.  For a
+ * single row of each of many streams qkv_kv_attend is faster.  Uses the handle's
+ * workspace: calls on one handle, captured ones too, must not overlap.  The
+ * prompt half of text-decoder.cpp:322-334 for any number of rows at any context. */
 int qkv_chunk_attend(qkv_handle *h, int32_t layer, int32_t n, const int32_t *slots_dev, const int32_t *starts_dev,
                      const int32_t *lens_dev, int32_t rows, const uint64_t *mask_dev, const void *q_dev, void *out_dev,
                      void *stream);

@@ -23,8 +23,8 @@
 // bf16 and is the A operand of P V in TMEM.  That costs a thread 128
 // exponentials a tile however few rows are real, which a short chunk, bound by
 // reading its context, cannot hide (64 draft trees of 3 to 12 rows on contexts
-// of 150 to 2100 tokens: 186 us, 77 us in thin mode, 53 us to read them); in
-// thin mode a thread has one key and computes 16 or 32.
+// of 150 to 2100 tokens: 186 us when thin mode was added, 76 us in it now, 53 us
+// to read them); in thin mode a thread has one key and computes 16 or 32.
 //
 // Work split.  A unit's work is w T: T key tiles, w = 2 in pair mode and 1
 // elsewhere.  All units laid end to end are cut into equal parts, one per CTA
@@ -34,9 +34,9 @@
 // captured call serves other lengths.  One warp walks a CTA's segments and
 // hands them to the others through a ring in shared memory.
 //
-// Softmax.  P is taken against a reference that moves only when a tile exceeds
-// it by more than 2^kRescaleLog2 (then O and the sum are rescaled); P, the sum
-// and O are floating-point numbers and lose nothing to a common factor.  P is
+// Softmax.  P is taken against a reference that moves only when a tile's scores
+// exceed it by more than 2^kRescaleLog2 (thin mode) or its sum leaves the range
+// of kSumMax (then O and the sum are rescaled); P, the sum and O are floating-point numbers and lose nothing to a common factor.  P is
 // rounded to bf16 once (2^-8 of the weight at most); sums stay in f32 and take
 // the unrounded values.  8-bit caches: the codes are exact in bf16; a key's
 // scale multiplies its scores, a value's scale its P.
@@ -50,18 +50,26 @@
 // and end cost was mostly code fetched afresh, so those parts are kept short or
 // rolled up.
 //
-// What bounds it.  2048 bf16 rows on 16000 tokens: 250 to 295 us (by the card's
-// clock), 0.97 to 1.14 PFLOP/s; of a pair step's 3220 cycles the tensor cores
-// work 2100 and each softmax warp 2060, which is its 128 exponentials a row at
-// the pipe's rate, and the rest is one lane waiting where neither covers the
-// other.  The draft trees above: 4.5 TB/s, the rest their segments' starts and
-// ends.  Six 8-bit contexts of 9000 to 33000 tokens: 101 us, 3.1 TB/s, of
-// a CTA's 125 K and V tiles 864 cycles each in the converting warps (88 us without them).
-// Ragged e4m3 segments of 17 to 390 rows: 156 us; a pair step takes 6300 cycles,
-// as each softmax warp reads two scales a key besides and shares its scheduler
-// with the converting warps.  Five rows on 512 tokens: 9.4 us, a chain of
-// latencies (plan 3300 cycles, K tile in place at 7100, P V done at 9200,
-// epilogue 2100, then the join).
+// What bounds it (device time of calls in a graph, L2 warm; cycles by clock64 in
+// the MMA warp, fitted as a tile's and a segment's over all segments).
+// 2048 bf16 rows on 16000 tokens: 400 000 cycles a CTA, 251 us in bursts of some
+// ms (1.14 PFLOP/s), 295 us after seconds at the power cap (0.97).  A pair step
+// takes 3200 cycles, of which the tensor cores work 2100 and each softmax warp
+// 2060, which is its 128 exponentials a row at the pipe's rate; the rest is one
+// lane waiting where neither covers the other.
+// Alternate mode, 16 chunks of 40 bf16 rows on 2000 tokens: 41 us, 2200 cycles a
+// tile and 7800 a segment.
+// The draft trees above: 4.6 TB/s; 1850 cycles a tile and 7500 to 8000 a segment,
+// its start and end.
+// Six 8-bit contexts of 9000 to 33000 tokens: 98 us, 3.2 TB/s; 2400 cycles a
+// tile, of which the converting warps work 864 for each of K and V (with the
+// conversion left out, 88 us of what was 101 then).
+// 24 ragged segments of 17 to 390 rows on 400 to 3000 tokens: 105 us bf16, 155 us
+// e4m3; a pair step of the latter takes 5900 to 6100 cycles, as each softmax
+// warp reads two scales a key besides and shares its scheduler with the
+// converting warps.
+// Five rows on 512 tokens: 9.6 us, a chain of latencies (plan 3300 cycles, K tile
+// in place at 7100, P V done at 9200, epilogue 2100, then the join).
 // All waits bounded; a softmax warp whose wait ran out goes on without waiting,
 // so that the named barriers stay matched.
 #include <cuda.h>
@@ -92,9 +100,10 @@ constexpr uint32_t kThinQ = kTileBytes, kThinQBytes = 8192, kThinQBlk = 4096;
 constexpr uint32_t kThinP = kTileBytes + 16384, kThinPBytes = 8192;
 constexpr int kMinCost = 2;                // least work of a CTA (tiles of alternate mode)
 static_assert(kMinCost >= 2, "every CTA between a unit's first and last holds one of its tiles");
-// Work of a unit besides its tiles.  Measured: 2640 cycles a tile and 9000 a unit in thin mode, 3260 a tile (counted
-// double) and 9200 a unit in pair mode.  Of (2, 3), (3, 6) and (5, 9), the last gave 64 draft trees 95 us against 99 and
-// 97, ragged segments 187 against 194 and 196, and a 2048-row piece 269 against 267 and 267.
+// Work of a unit besides its tiles, for all modes and cache types: 5000 to 8000 cycles and 1850 to 3200 a tile outside
+// pair mode, 9000 to 11500 and 3200 to 6000 a tile (counted double) in it.  Of (2, 3), (3, 6), (5, 9) and (8, 14): 64
+// draft trees 80, 80, 76, 76 us; ragged bf16 segments 118, 115, 105, 106; ragged e4m3 160, 162, 155, 163; six long 8-bit
+// contexts 97, 97, 98, 99; 16 chunks of 40 rows on 2000 tokens 41, 41, 41, 40; a 2048-row piece 251, 251, 251, 253.
 constexpr int kUnitCost = 5, kPairUnitCost = 9;
 constexpr int kPieceRows = 256;            // rows of a workspace piece (pair mode: both lanes)
 
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
 
     // ---- this CTA's part of the work ----
     // Running maximum of the ends and running sum of the costs over the entries: up to 32 by the plan warp itself (its
-    // part of a small call is a chain of latencies, and begins here), more by all threads, four to a thread (n <= 1024).
+    // part of a small call is a chain of latencies, and begins here), more by all threads, kPer to a thread (n <= 1024).
     int total = 0;
     if (p.n > 32) {
         constexpr int kPer = (kAttnMaxRows + kThreads - 1) / kThreads;
@@ -1102,7 +1111,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
         };
 
         // Then P of the chunks [c, c1) by the new reference, over their S; their sums.  (Apart from the usual path: a
-        // loop around that one, to go through it again, took 16 of 186 us of ragged 8-bit segments.)
+        // loop around that one, to go through it again, took 16 of the 186 us that ragged 8-bit segments needed then.)
         auto redo = [&](int c, int c1, const float *ks, const float *vs, float m_ref) -> float {
             const float sub = m_ref == -INFINITY ? 0.0f : m_ref;
             float sum = 0.0f;
@@ -1173,7 +1182,7 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 uint32_t sr[2][32];
                 tmem_ld32_issue(tS, sr[0]);
                 // The whole tile unrolled, two chunks of S in registers, and P stored at its end, over S that is intact
-                // until then: a 2048-row piece takes 265 us, 320 with the short loop below.
+                // until then: a 2048-row piece took 265 us when this was chosen, 320 with the short loop below.
                 uint32_t pk[4][16];
 #pragma unroll 1
                 for (int again = 0; again < 2; ++again) {
@@ -1215,8 +1224,8 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
                 tmem_wait_st();
                 return;
             }
-            // The shortest code wins where the converting warps fetch theirs, too: ragged segments take 162 us, 170 with two
-            // chunks unrolled and 195 with the whole tile.
+            // The shortest code wins where the converting warps fetch theirs, too: ragged e4m3 segments take 155 us, 157 with
+            // two chunks unrolled and 187 with the whole tile (158 and 188 against 153 with int8 V).
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t sv[32], pk[16];
@@ -1580,9 +1589,9 @@ __global__ void __launch_bounds__(Layout<k8>::kThreads, 1)
 // at most.  Thread = (row, four dims), in the order the pieces lie in memory:
 // thin mode's row by row, the others' four dims of all rows together.  Bound by
 // the latency of a launch and its dependent loads; kJoinBatch pieces' are in
-// flight together.  With one piece at a time by the first CTA's blocks alone, 100
-// rows on 3000 tokens (some 20 pieces a unit) took 47 us instead of 20, 5 rows on
-// 512 tokens 11.2 us instead of 10.1.  More or larger blocks cost the small
+// flight together.  When that was one piece at a time by the first CTA's blocks
+// alone, 100 rows on 3000 tokens (some 20 pieces a unit) took 47 us instead of
+// 20, 5 rows on 512 tokens 11.2 us instead of 10.1.  More or larger blocks cost the small
 // launch what they give the large one.
 constexpr int kJoinThreads = 128, kJoinBatch = 6, kJoinRows = 8;
 

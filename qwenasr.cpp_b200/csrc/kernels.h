@@ -97,8 +97,8 @@ struct AttendParams {
     // 1: the kernel(s) just before this launch on the stream wrote only each
     // row's LAST page (one new token per row: K1, or the previous layer's K2
     // with the append-ahead), and the row arrays and page table came from
-    // copies that finished before them, so K2 may set up and stream the other
-    // pages before its grid dependency wait.  0: everything waits (any caller).
+    // copies and kernels that finished before them, so K2 may set up and
+    // stream the other pages before its grid dependency wait.  0: everything waits (any caller).
     int early;
     // Append-ahead (KV steps, where every layer's projections are on the
     // device before the step starts): with next.n > 0, K2 of layer l also
