@@ -166,3 +166,29 @@ def test_append_of_vectors_near_the_end_of_the_range(pkg, kv, chunk):
             scale = (amax / top).clamp_min(2.0 ** -126)
             step = 0.5 * scale if top == 127.0 else torch.maximum(want.abs() * 2.0 ** -4, scale * 2.0 ** -10)
             assert not ((got - want).abs() > step * (1 + 2.0 ** -6) + 2 * arith + 2.0 ** -19 * amax).any()
+
+
+@pytest.mark.parametrize("sections,interleaved,pairs_of", [
+    ((24, 20, 20), False, [range(0, 24), range(24, 44), range(44, 64)]),
+    ((24, 20, 20), True, [[*range(0, 60, 3), 60, 61, 62, 63], range(1, 60, 3), range(2, 60, 3)]),
+    ((62, 1, 1), True, [[0, *range(3, 64)], [1], [2]]),
+    ((22, 21, 21), True, [range(0, 64, 3), range(1, 64, 3), range(2, 64, 3)]),
+    ((0, 0, 64), False, [[], [], range(0, 64)])])
+def test_append_turns_the_pairs_of_an_axis(pkg, sections, interleaved, pairs_of):
+    """With a position on one axis alone, the listed pairs turn and the others stay as they are."""
+    with Cache(pkg, "f32", [3]) as c:
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        qkv = torch.randn((1, QKV), device="cuda", generator=gen).expand(3, -1).contiguous()
+        q = torch.empty((4, HQ * D), device="cuda")
+        slots, pos = i32([c.streams[0]] * 3), i32(range(3))
+        for rows, axes, out in ((3, [[5, 0, 0], [0, 5, 0], [0, 0, 5]], q[:3]), (1, [[0]] * 3, q[3:])):
+            a = i32(axes)
+            c.dec.chunk_append(0, rows, slots.data_ptr(), pos.data_ptr(), a.data_ptr(), sections, interleaved, qkv.data_ptr(),
+                               out.data_ptr(), pkg.F32)
+            c.dec.sync()
+        lo, hi = q.view(4, HQ, 2, 64).unbind(2)
+        for axis, pairs in enumerate(pairs_of):
+            turned = torch.zeros(64, dtype=torch.bool, device="cuda")
+            turned[list(pairs)] = True
+            same = ((lo[axis] == lo[3]) & (hi[axis] == hi[3])).all(0)
+            assert torch.equal(same, ~turned), axis
